@@ -117,6 +117,22 @@
 (defrstq silu-mul-quant-act* "rstq_silu_mul_quant_act"  I [P P P P P P L])
 (defrstq gelu-mul-quant-act* "rstq_gelu_mul_quant_act"  I [P P P P P P L])
 ;; ---- sharded weights
+(defrstq paged-rope-append*  "rstq_paged_rope_append" I [P P P P P P P P P P L L L L L L L L L L D I I])
+                             ; ctx q k v qout kcache vcache table lens cu rows seqs n-q n-kv head-dim page n-pages max-pages ldq ldkv theta in-dtype dtype
+(defrstq paged-decode-attention* "rstq_paged_decode_attention" I [P P P P P P P L L L L L L L L L D I])
+                             ; ctx q kcache vcache out table lens seqs n-q group n-kv head-dim page n-pages max-pages ldq scale dtype
+(defrstq prompt-attention*   "rstq_prompt_attention"  I [P P P P P P P L L L L L L L L L D I I])
+                             ; ctx q k v out cu-q cu-k rows kv-rows seqs n-q group n-kv head-dim ldq ldk scale causal dtype
+(defrstq paged-prompt-attention* "rstq_paged_prompt_attention" I [P P P P P P P P L L L L L L L L L L D I I])
+                             ; ctx q kcache vcache out table cu-q lens rows seqs n-q group n-kv head-dim page n-pages max-pages ldq scale causal dtype
+(defrstq pages-free*         "rstq_pages_free"        I [P P P P P P L L L L L])      ; ctx table lens refs list info n seqs n-pages max-pages page
+(defrstq pages-extend*       "rstq_pages_extend"      I [P P P P P P P L L L L L])    ; ctx table lens refs list counts info n seqs n-pages max-pages page
+(defrstq pages-fork*         "rstq_pages_fork"        I [P P P P P P P P P L L L L L L L])
+                             ; ctx kcache vcache table lens refs src dst info n seqs n-pages max-pages page layers row-bytes
+(defrstq pages-compact*      "rstq_pages_compact"     I [P P P P P P P P P L L L L L L])
+                             ; ctx kcache vcache table lens refs table-out refs-out info seqs n-pages max-pages page layers row-bytes
+(defrstq pages-copy*         "rstq_pages_copy"        I [P P P P P P L L L L])        ; ctx kcache vcache src dst info n n-pages layers page-bytes
+
 (defrstq tp-region-bytes*    "rstq_tp_region_bytes"   L [I L])
 (defrstq tp-attach*          "rstq_tp_attach"         I [P P P I I I L])           ; ctx regions tp** dev rank nranks region-bytes
 (defrstq tp-create-local*    "rstq_tp_create_local"   I [P P P I L])               ; ctx devs tps nranks max-payload

@@ -52,7 +52,8 @@ typedef struct rstq_event rstq_event;
 #define RSTQ_E_DEVICE (-8)   /* handles live on different devices             */
 #define RSTQ_E_STATE (-9)    /* call not legal now (e.g. sync during capture) */
 #define RSTQ_E_LIMIT (-10)   /* problem exceeds a stated fixed limit          */
-#define RSTQ_E_RANGE (-11)   /* offset + bytes beyond the buffer              */
+#define RSTQ_E_RANGE (-11)   /* offset + bytes beyond the buffer; from rstq_sync: a table of a paged cache
+                                named no page of the pool, or a row had no page  */
 #define RSTQ_E_WAIT (-12)    /* a time-bounded wait inside a kernel ran out; results of that
                                 launch are invalid (reported by rstq_sync)     */
 
@@ -437,6 +438,82 @@ RSTQ_API int32_t rstq_gelu_mul_quant_act(rstq_ctx* ctx, rstq_buf* gate, rstq_buf
 RSTQ_API int32_t rstq_gqa_decode_attention(rstq_ctx* ctx, rstq_buf* q, rstq_buf* k, rstq_buf* v, rstq_buf* out,
                                            rstq_buf* clenbuf, int64_t cache_len, int64_t n_q, int64_t group,
                                            int64_t n_kv, int64_t head_dim, int64_t maxpos, double scale);
+
+/* ---- serving many sequences from one paged cache.  No counterpart in the reference, whose caches hold one sequence
+ *      (src/raster/dl/attention.clj:413-575): these are its attention steps for packed rows of many.
+ *
+ * Elements are RSTQ_F32 or RSTQ_BF16 (`dtype`), one type for q, K, V and out; sums, softmax statistics and angles are held in
+ * 32 bits or more and a result is rounded once.  head_dim % 8 == 0 and <= 256; n_q = group * n_kv.
+ *
+ * Pool: kcache and vcache hold n_pages pages of `page` positions (16, 32, 64, 128 or 256), a position n_kv heads of
+ *   head_dim: rows as in the contiguous caches [position][n_kv][head_dim], of which a pool with a table that counts up is
+ *   one.  n_pages, max_pages <= 2^20.
+ * table int32 [seqs][max_pages]: the pages of each sequence in order, what lies behind them is not read.  lens int32 [seqs]:
+ *   positions of each sequence, the call's own rows among them; beyond max_pages * page it counts as that.
+ * cu int32 [seqs + 1]: rows of a packed array, sequence b has rows [cu[b], cu[b+1]).  Its rows are its LAST ones: row t
+ *   stands at position lens[b] - (cu[b+1] - t).  Rows that no sequence has are left as they were.
+ * seqs <= 65536; all of these arrays are read on the device, so one recorded graph serves every step.
+ *
+ * What they hold cannot make a call read or write outside its buffers: an entry of a table that names no page
+ * of the pool counts as positions that nobody sees (and are not written), as does a row whose position has no page; the
+ * next rstq_sync then returns RSTQ_E_RANGE.
+ * ldq, ldk, ldkv: elements from a row of q (of k and v) to the next, 0 = packed; rows start on 16-byte boundaries, so a
+ * slice of a fused q|k|v matmul's result can be handed over.  Scratch is the context's: calls that could overlap on the GPU
+ * (graphs replayed on two streams) need a context each.
+ *
+ *   rstq_paged_rope_append       q turned to qout [rows][n_q][head_dim]; k turned and v written to their pages, in `dtype`
+ *                                (q, k, v are in_dtype).  cu may be NULL: rows == seqs, one per sequence.  qout may be q.
+ *   rstq_paged_decode_attention  one row of q per sequence against all its positions; a sequence of none gives zeros.
+ *   rstq_prompt_attention        rows of packed sequences (cu_q) against packed keys and values [kv_rows][n_kv][head_dim]
+ *                                (cu_k; may be cu_q); causal = 1: a row sees the keys up to its own place, the last row
+ *                                all of them; 0: every row sees all.  Rows that see nothing are zeros.
+ *   rstq_paged_prompt_attention  the same with keys and values from the pages: prompts behind a cached prefix.
+ * Keys and values that a row does not see never reach it, NaN and infinities included. */
+RSTQ_API int32_t rstq_paged_rope_append(rstq_ctx* ctx, rstq_buf* q, rstq_buf* k, rstq_buf* v, rstq_buf* qout, rstq_buf* kcache,
+                                        rstq_buf* vcache, rstq_buf* table, rstq_buf* lens, rstq_buf* cu, int64_t rows,
+                                        int64_t seqs, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t page,
+                                        int64_t n_pages, int64_t max_pages, int64_t ldq, int64_t ldkv, double theta,
+                                        int32_t in_dtype, int32_t dtype);
+RSTQ_API int32_t rstq_paged_decode_attention(rstq_ctx* ctx, rstq_buf* q, rstq_buf* kcache, rstq_buf* vcache, rstq_buf* out,
+                                             rstq_buf* table, rstq_buf* lens, int64_t seqs, int64_t n_q, int64_t group,
+                                             int64_t n_kv, int64_t head_dim, int64_t page, int64_t n_pages,
+                                             int64_t max_pages, int64_t ldq, double scale, int32_t dtype);
+RSTQ_API int32_t rstq_prompt_attention(rstq_ctx* ctx, rstq_buf* q, rstq_buf* k, rstq_buf* v, rstq_buf* out, rstq_buf* cu_q,
+                                       rstq_buf* cu_k, int64_t rows, int64_t kv_rows, int64_t seqs, int64_t n_q,
+                                       int64_t group, int64_t n_kv, int64_t head_dim, int64_t ldq, int64_t ldk,
+                                       double scale, int32_t causal, int32_t dtype);
+RSTQ_API int32_t rstq_paged_prompt_attention(rstq_ctx* ctx, rstq_buf* q, rstq_buf* kcache, rstq_buf* vcache, rstq_buf* out,
+                                             rstq_buf* table, rstq_buf* cu_q, rstq_buf* lens, int64_t rows, int64_t seqs,
+                                             int64_t n_q, int64_t group, int64_t n_kv, int64_t head_dim, int64_t page,
+                                             int64_t n_pages, int64_t max_pages, int64_t ldq, double scale, int32_t causal,
+                                             int32_t dtype);
+/* Pages of such a cache, on the device and in stream order (a graph may hold these calls).  refs int32 [n_pages]: how many
+ * sequences hold a page, 0 = free; a new cache has lens and refs of zeros and a table of -1.  A sequence of n positions holds
+ * ceil(n / page) pages.  Free pages are taken lowest first, in the list's order.  kcache and vcache: [layers] pools one behind
+ * the other, rows of row_bytes bytes (n_kv * head_dim elements; a page's bytes are a multiple of 16).  Lists: int32 [n], n <= 65536.
+ * info int32 [4], written by every call: [0] = 0 done, else nothing was changed: 1 = too few free pages ([3] = pages wanted),
+ * 2 = an entry of the list is no sequence (page), is there twice, or may not be there ([3] = its place), 3 = no room in the table,
+ * 4 = the positions would go to a page that another sequence holds too; [1] = pages in use; [2] = pages copied.
+ *   rstq_pages_free     the listed sequences end: their pages lose a holder, their rows of the table become -1, lens 0.
+ *   rstq_pages_extend   room for counts[i] more positions of sequence list[i] (lens grows by them).
+ *   rstq_pages_fork     dst[i], a sequence of length 0, becomes src[i]: full pages shared, a partial last page copied to a page
+ *                       of its own.  No sequence may be both in src and in dst.
+ *   rstq_pages_compact  pages in use that lie behind the first info[1] ones move, in order, to the free ones among those;
+ *                       table_out and refs_out (which may be table and refs) say the new places, lens stays.
+ *   rstq_pages_copy     page dst[i] = page src[i] of every layer, K and V; no page twice in dst, none in both lists ([1] = 0). */
+RSTQ_API int32_t rstq_pages_free(rstq_ctx* ctx, rstq_buf* table, rstq_buf* lens, rstq_buf* refs, rstq_buf* list, rstq_buf* info,
+                                 int64_t n, int64_t seqs, int64_t n_pages, int64_t max_pages, int64_t page);
+RSTQ_API int32_t rstq_pages_extend(rstq_ctx* ctx, rstq_buf* table, rstq_buf* lens, rstq_buf* refs, rstq_buf* list,
+                                   rstq_buf* counts, rstq_buf* info, int64_t n, int64_t seqs, int64_t n_pages,
+                                   int64_t max_pages, int64_t page);
+RSTQ_API int32_t rstq_pages_fork(rstq_ctx* ctx, rstq_buf* kcache, rstq_buf* vcache, rstq_buf* table, rstq_buf* lens,
+                                 rstq_buf* refs, rstq_buf* src, rstq_buf* dst, rstq_buf* info, int64_t n, int64_t seqs,
+                                 int64_t n_pages, int64_t max_pages, int64_t page, int64_t layers, int64_t row_bytes);
+RSTQ_API int32_t rstq_pages_compact(rstq_ctx* ctx, rstq_buf* kcache, rstq_buf* vcache, rstq_buf* table, rstq_buf* lens,
+                                    rstq_buf* refs, rstq_buf* table_out, rstq_buf* refs_out, rstq_buf* info, int64_t seqs,
+                                    int64_t n_pages, int64_t max_pages, int64_t page, int64_t layers, int64_t row_bytes);
+RSTQ_API int32_t rstq_pages_copy(rstq_ctx* ctx, rstq_buf* kcache, rstq_buf* vcache, rstq_buf* src, rstq_buf* dst,
+                                 rstq_buf* info, int64_t n, int64_t n_pages, int64_t layers, int64_t page_bytes);
 
 /* ---- tensor-parallel exchange of the sharded operator.  No counterpart in the reference: it
  *      extends the placement / plan vocabulary (src/raster/compiler/passes/placement.clj:21-89)

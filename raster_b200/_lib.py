@@ -82,6 +82,15 @@ SIGNATURES = {
     "rstq_gelu_mul_quant_act": [vp, vp, vp, vp, vp, vp, i64],
     "rstq_kv_append": [vp, vp, vp, vp, i64, i64, i64],
     "rstq_gqa_decode_attention": [vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, C.c_double],
+    "rstq_paged_rope_append": [vp] * 10 + [i64] * 10 + [C.c_double, i32, i32],
+    "rstq_paged_decode_attention": [vp] * 7 + [i64] * 9 + [C.c_double, i32],
+    "rstq_prompt_attention": [vp] * 7 + [i64] * 9 + [C.c_double, i32, i32],
+    "rstq_paged_prompt_attention": [vp] * 8 + [i64] * 10 + [C.c_double, i32, i32],
+    "rstq_pages_free": [vp] * 6 + [i64] * 5,
+    "rstq_pages_extend": [vp] * 7 + [i64] * 5,
+    "rstq_pages_fork": [vp] * 9 + [i64] * 7,
+    "rstq_pages_compact": [vp] * 9 + [i64] * 6,
+    "rstq_pages_copy": [vp] * 6 + [i64] * 4,
     "rstq_tp_region_bytes": [i32, i64],
     "rstq_tp_attach": [vp, pp, pp, i32, i32, i32, i64],
     "rstq_tp_create_local": [vp, C.POINTER(i32), pp, i32, i64],

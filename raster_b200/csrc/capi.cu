@@ -626,6 +626,7 @@ int32_t rstq_init(const int32_t* devices, rstq_ctx** ctxp, int32_t ndev) {
             if ((r = gemm_configure(ds)) != RSTQ_OK) return r;
             if ((r = dx_configure()) != RSTQ_OK) return r;
             if ((r = attn_configure(ds)) != RSTQ_OK) return r;
+            if ((r = pages_configure(ds)) != RSTQ_OK) return r;
             RSTQ_CUDA(cudaStreamSynchronize(ds.stream));
             return RSTQ_OK;
         };
@@ -666,6 +667,7 @@ int32_t rstq_shutdown(rstq_ctx* ctx) {
         if (ds.gemm_scratch) cudaFree(ds.gemm_scratch);
         if (ds.attn_scratch) cudaFree(ds.attn_scratch);
         if (ds.attn_slots) cudaFree(ds.attn_slots);
+        if (ds.page_scratch) cudaFree(ds.page_scratch);
         if (ds.kq_scratch) cudaFree(ds.kq_scratch);
         if (ds.f_image) cudaFree(ds.f_image);
         if (ds.bind_stage) cudaFree(ds.bind_stage);
@@ -742,12 +744,13 @@ int32_t rstq_sync(rstq_ctx* ctx, int32_t dev) {
     int32_t rc = use_dev(ctx, dev);
     if (rc != RSTQ_OK) return rc;
     DeviceState& ds = ctx->devs[dev];
-    int st = 0;
-    RSTQ_CUDA(cudaMemcpyAsync(&st, ds.status, 4, cudaMemcpyDeviceToHost, ds.stream));
+    int words[2] = {0, 0};
+    RSTQ_CUDA(cudaMemcpyAsync(words, ds.status, 8, cudaMemcpyDeviceToHost, ds.stream));
     RSTQ_CUDA(cudaStreamSynchronize(ds.stream));
+    const int st = words[0];
+    // the flags are sticky until read: clear them so the context stays usable
+    if (st != 0 || words[1] != 0) RSTQ_CUDA(cudaMemsetAsync(ds.status, 0, 8, ds.stream));
     if (st != 0) {
-        // the flag is sticky until read: clear it so the context stays usable
-        RSTQ_CUDA(cudaMemsetAsync(ds.status, 0, 4, ds.stream));
         // a launch that gave up may have left hand-over flags set: the next launch must not take them
         RSTQ_CUDA(cudaMemsetAsync(ds.counters, 0, (size_t)ds.counters_len * 4, ds.stream));
         if (ds.attn_slots) RSTQ_CUDA(cudaMemsetAsync(ds.attn_slots, 0xFF, (size_t)ds.attn_slots_bytes, ds.stream));
@@ -755,6 +758,12 @@ int32_t rstq_sync(rstq_ctx* ctx, int32_t dev) {
         set_error("a time-bounded wait inside a kernel ran out (status %d); results since the "
                   "last rstq_sync are invalid", st);
         return RSTQ_E_WAIT;
+    }
+    if (words[1] != 0) {
+        RSTQ_CUDA(cudaStreamSynchronize(ds.stream));
+        set_error("a table of a paged cache named no page of the pool, or a row's position had no page: those positions were "
+                  "neither read nor written");
+        return RSTQ_E_RANGE;
     }
     return RSTQ_OK;
 }

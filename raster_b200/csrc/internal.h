@@ -105,6 +105,7 @@ struct DeviceState {
     int64_t attn_slots_bytes = 0;
     int attn_clusters[9] = {};     // ... and how many clusters of 2 .. 8 of its thread blocks the device holds at once,
     int attn_narrow_clusters[9] = {};   // or of its blocks of a quarter of the warps
+    void* page_scratch = nullptr;  // paged caches: lists of pages between the launches of one call
     void* pinned = nullptr;        // host staging for the host-array entry points
     int64_t pinned_bytes = 0;
     void* io_dev = nullptr;        // device staging for the host-array entry points
@@ -119,7 +120,8 @@ struct DeviceState {
     // arrays of weights that are gone, kept for the next one of the same size: at most kWeightKeep bytes
     std::vector<std::pair<void*, int64_t>> spare_weights;
     int64_t spare_bytes = 0;
-    int* status = nullptr;         // device status word: nonzero after a bounded wait ran out
+    int* status = nullptr;         // device status words: [0] nonzero after a bounded wait ran out, [1] after a page table
+                                   // named no page
     // Instantiated graphs hold the scratch addresses of the launches they recorded.  While any is
     // alive, scratch that has to grow is parked here instead of freed, so a replay never touches
     // memory that went back to the allocator; the blocks are released when the last graph is gone.
@@ -352,6 +354,8 @@ int32_t launch_gemm(rstq_ctx* ctx, DeviceState& ds, const rstq_weight* w, const 
 int32_t gemm_configure(DeviceState& ds);
 // attn.cu
 int32_t attn_configure(DeviceState& ds);  // scratch, shared-memory attributes and cluster counts, once per device
+// pages.cu
+int32_t pages_configure(DeviceState& ds);  // scratch, shared-memory attributes, once per device
 // dx.cu
 int32_t dx_configure();  // shared-memory attributes, once per device
 int32_t launch_qlinear_q8_dx(rstq_ctx* ctx, DeviceState& ds, const float* dy, const int8_t* codes,

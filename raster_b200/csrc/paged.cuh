@@ -1,0 +1,139 @@
+// What the kernels over a paged cache share: where a sequence's rows are, element types, argument checks.
+//
+// A pool holds n_pages pages of `page` positions (a power of two), a position n_kv heads of head_dim elements: the rows
+// of the contiguous caches [position][n_kv][head_dim], cut into pages.  A sequence's row of the table names its pages in
+// order, so a contiguous cache is the pool whose table counts up.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "internal.h"
+
+namespace rstq {
+
+constexpr int kMaxSeqs = 65536;
+constexpr int64_t kMaxPages = 1 << 20;      // of a pool
+constexpr int64_t kMaxRows = 1ll << 30;     // packed rows of a call
+constexpr int kStatusPage = 1;              // word of DeviceState::status: a table named a page outside the pool
+constexpr int kPagedGroup = 16;             // query heads of a KV head that one thread block of the decode kernel serves
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+    static constexpr int kVec = 4;   // elements of 16 bytes
+    static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    }
+};
+template <>
+struct Elem<__nv_bfloat16> {
+    static constexpr int kVec = 8;
+    static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[8]) {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+};
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {   // rounded to nearest, ties to even
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// four consecutive elements
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xFFFF0000u), __uint_as_float(x.y << 16),
+                       __uint_as_float(x.y & 0xFFFF0000u));
+}
+__device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(bf16_pair(v.x, v.y), bf16_pair(v.z, v.w));
+}
+
+// The rows of the sequences' keys and values: in the pages of a pool, or packed one sequence after the other.
+struct KvPlace {
+    const int32_t* table;   // [seqs][width]; null: packed
+    const int32_t* lens;    // paged: positions of each sequence, this call's own among them
+    const int32_t* cu;      // packed: first row of each sequence, and the end of the last
+    int64_t rows;           // packed: rows there are
+    int64_t n_pages;
+    int64_t ld;             // elements from a row to the next
+    int width, shift;       // pages of a row of the table; log2 of a page's positions
+    int* status;
+};
+__device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
+// Rows of sequence b of a packed array: whatever the words of `cu` hold, inside [0, rows].
+__device__ __forceinline__ void packed_range(const int32_t* cu, int b, int64_t rows, int64_t* first, int64_t* last) {
+    *first = clamp64(cu[b], 0, rows);
+    *last = clamp64(cu[b + 1], *first, rows);
+}
+// Positions of sequence b; packed: *row0 = its first row.  A length beyond the sequence's pages counts as their end.
+__device__ __forceinline__ int64_t kv_length(const KvPlace& kv, int b, int64_t* row0) {
+    if (kv.table) {
+        *row0 = 0;
+        return clamp64(kv.lens[b], 0, (int64_t)kv.width << kv.shift);
+    }
+    int64_t last;
+    packed_range(kv.cu, b, kv.rows, row0, &last);
+    return last - *row0;
+}
+// Row of the pool (of the packed array) that holds position `pos` of sequence b; -1: the table names no page of the pool.
+__device__ __forceinline__ int64_t kv_row(const KvPlace& kv, int b, int64_t row0, int64_t pos) {
+    if (!kv.table) return row0 + pos;
+    const int page = kv.table[(int64_t)b * kv.width + (pos >> kv.shift)];
+    if ((uint32_t)page >= (uint64_t)kv.n_pages) return -1;
+    return ((int64_t)page << kv.shift) + (pos & ((1 << kv.shift) - 1));
+}
+// The sequence of a packed row: the last one that begins at or before it; -1: none holds it.
+__device__ __forceinline__ int row_sequence(const int32_t* cu, int seqs, int64_t row) {
+    int lo = 0, hi = seqs;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (cu[mid] <= row) lo = mid + 1;
+        else hi = mid;
+    }
+    const int b = lo - 1;
+    return b >= 0 && row < cu[b + 1] ? b : -1;
+}
+
+// ---- argument checks of the entry points ----
+inline bool paged_buf(const rstq_buf* b, const rstq_ctx* ctx, int64_t bytes) {
+    return b && b->magic == kBufMagic && b->ctx == ctx && b->bytes >= bytes && ((uintptr_t)b->ptr & 15) == 0;
+}
+inline int elem_bytes(int32_t dtype) { return dtype == RSTQ_BF16 ? 2 : 4; }
+inline int log2_of(int64_t v) {
+    int s = 0;
+    while ((1ll << s) < v) ++s;
+    return s;
+}
+// n_q = group x n_kv heads of head_dim, of a type these kernels take
+int32_t check_heads(int64_t n_q, int64_t group, int64_t n_kv, int64_t head_dim, int32_t dtype);
+// a pool's and a table's sizes
+int32_t check_pages(int64_t seqs, int64_t page, int64_t n_pages, int64_t max_pages);
+template <typename... B>
+inline bool same_device(const rstq_buf* a, const B*... rest) {
+    return ((rest == nullptr || rest->dev == a->dev) && ...);
+}
+
+struct PromptArgs {
+    const void *q, *k, *v;
+    void* out;
+    const int32_t* cu_q;    // null: one row per sequence
+    KvPlace kv;
+    int64_t rows, ldq;
+    int seqs, n_q, group, n_kv, head_dim;
+    float scale;
+    int causal;
+    int32_t dtype;
+    int64_t kv_rows;        // rows of the pool or of the packed arrays
+};
+// paged_attn.cu: any head_dim and length, a warp per position
+int32_t launch_attention_rows(DeviceState& ds, const PromptArgs& a);
+
+}  // namespace rstq

@@ -277,6 +277,16 @@ def _builtin():
     r("gqa-decode-attention-buf!",
       lambda c, a, s: c.gqa_decode_attention(a[0], a[1], a[2], a[3], 0, s[0], s[1], s[2], s[3], s[4], s[5], clenbuf=a[5]),
       6, 6)
+    # many sequences over one paged cache (no counterpart in the reference): arrays, then scalars, as Context takes them
+    r("paged-rope-append!", lambda c, a, s: c.paged_rope_append(*a, *s), 9)
+    r("paged-decode-attention!", lambda c, a, s: c.paged_decode_attention(*a, *s), 6)
+    r("prompt-attention!", lambda c, a, s: c.prompt_attention(*a, *s), 6)
+    r("paged-prompt-attention!", lambda c, a, s: c.paged_prompt_attention(*a, *s), 7)
+    r("pages-free!", lambda c, a, s: c.pages_free(*a, *s), 5, 5)
+    r("pages-extend!", lambda c, a, s: c.pages_extend(*a, *s), 6, 5)
+    r("pages-fork!", lambda c, a, s: c.pages_fork(*a, *s), 8, 7)
+    r("pages-compact!", lambda c, a, s: c.pages_compact(*a, *s), 8, 6)
+    r("pages-copy!", lambda c, a, s: c.pages_copy(*a, *s), 5, 4)
 
 
 _builtin()

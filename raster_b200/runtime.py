@@ -401,6 +401,59 @@ class Context:
                                                    clenbuf.handle if clenbuf is not None else None, cache_len,
                                                    n_q, group, n_kv, head_dim, maxpos, scale))
 
+    # -- paged cache of many sequences: rows in, attention, pages -------------------
+    def paged_rope_append(self, q, k, v, qout, kcache, vcache, table, lens, cu, rows, seqs, n_q, n_kv, head_dim, page,
+                          n_pages, max_pages, theta, in_dtype=L.F32, dtype=L.F32, ldq=0, ldkv=0) -> None:
+        """Rows of many sequences turned and written to their pages (cu None: one row per sequence)."""
+        L.check(self.lib.rstq_paged_rope_append(
+            self.handle, q.handle, k.handle, v.handle, qout.handle, kcache.handle, vcache.handle, table.handle, lens.handle,
+            cu.handle if cu is not None else None, rows, seqs, n_q, n_kv, head_dim, page, n_pages, max_pages, ldq, ldkv, theta,
+            in_dtype, dtype))
+
+    def paged_decode_attention(self, q, kcache, vcache, out, table, lens, seqs, n_q, group, n_kv, head_dim, page, n_pages,
+                               max_pages, scale, dtype=L.F32, ldq=0) -> None:
+        """One new token per sequence against all positions of its pages."""
+        L.check(self.lib.rstq_paged_decode_attention(
+            self.handle, q.handle, kcache.handle, vcache.handle, out.handle, table.handle, lens.handle, seqs, n_q, group, n_kv,
+            head_dim, page, n_pages, max_pages, ldq, scale, dtype))
+
+    def prompt_attention(self, q, k, v, out, cu_q, cu_k, rows, kv_rows, seqs, n_q, group, n_kv, head_dim, scale, causal=True,
+                         dtype=L.F32, ldq=0, ldk=0) -> None:
+        """Packed prompts against packed keys and values."""
+        L.check(self.lib.rstq_prompt_attention(
+            self.handle, q.handle, k.handle, v.handle, out.handle, cu_q.handle, cu_k.handle, rows, kv_rows, seqs, n_q, group, n_kv,
+            head_dim, ldq, ldk, scale, int(causal), dtype))
+
+    def paged_prompt_attention(self, q, kcache, vcache, out, table, cu_q, lens, rows, seqs, n_q, group, n_kv, head_dim, page,
+                               n_pages, max_pages, scale, causal=True, dtype=L.F32, ldq=0) -> None:
+        """Packed new rows of sequences against the keys and values of their pages."""
+        L.check(self.lib.rstq_paged_prompt_attention(
+            self.handle, q.handle, kcache.handle, vcache.handle, out.handle, table.handle, cu_q.handle, lens.handle, rows, seqs,
+            n_q, group, n_kv, head_dim, page, n_pages, max_pages, ldq, scale, int(causal), dtype))
+
+    def pages_free(self, table, lens, refs, seq_list, info, n, seqs, n_pages, max_pages, page) -> None:
+        L.check(self.lib.rstq_pages_free(self.handle, table.handle, lens.handle, refs.handle, seq_list.handle, info.handle, n, seqs,
+                                         n_pages, max_pages, page))
+
+    def pages_extend(self, table, lens, refs, seq_list, counts, info, n, seqs, n_pages, max_pages, page) -> None:
+        L.check(self.lib.rstq_pages_extend(self.handle, table.handle, lens.handle, refs.handle, seq_list.handle, counts.handle,
+                                           info.handle, n, seqs, n_pages, max_pages, page))
+
+    def pages_fork(self, kcache, vcache, table, lens, refs, src, dst, info, n, seqs, n_pages, max_pages, page, layers,
+                   row_bytes) -> None:
+        L.check(self.lib.rstq_pages_fork(self.handle, kcache.handle, vcache.handle, table.handle, lens.handle, refs.handle,
+                                         src.handle, dst.handle, info.handle, n, seqs, n_pages, max_pages, page, layers, row_bytes))
+
+    def pages_compact(self, kcache, vcache, table, lens, refs, table_out, refs_out, info, seqs, n_pages, max_pages, page,
+                      layers, row_bytes) -> None:
+        L.check(self.lib.rstq_pages_compact(self.handle, kcache.handle, vcache.handle, table.handle, lens.handle, refs.handle,
+                                            table_out.handle, refs_out.handle, info.handle, seqs, n_pages, max_pages, page, layers,
+                                            row_bytes))
+
+    def pages_copy(self, kcache, vcache, src, dst, info, n, n_pages, layers, page_bytes) -> None:
+        L.check(self.lib.rstq_pages_copy(self.handle, kcache.handle, vcache.handle, src.handle, dst.handle, info.handle, n, n_pages,
+                                         layers, page_bytes))
+
     # -- graphs / events / misc ------------------------------------------------
     def graph_begin(self, dev=0) -> None:
         L.check(self.lib.rstq_graph_begin(self.handle, dev))
