@@ -354,6 +354,8 @@ int32_t launch_gemm(rstq_ctx* ctx, DeviceState& ds, const rstq_weight* w, const 
 int32_t gemm_configure(DeviceState& ds);
 // attn.cu
 int32_t attn_configure(DeviceState& ds);  // scratch, shared-memory attributes and cluster counts, once per device
+// paged_decode.cu
+int32_t decode_configure(DeviceState& ds);  // shared-memory attributes, once per device
 // pages.cu
 int32_t pages_configure(DeviceState& ds);  // scratch, shared-memory attributes, once per device
 // dx.cu

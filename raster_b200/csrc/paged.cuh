@@ -135,5 +135,7 @@ struct PromptArgs {
 };
 // paged_attn.cu: any head_dim and length, a warp per position
 int32_t launch_attention_rows(DeviceState& ds, const PromptArgs& a);
+// paged_decode.cu: one row per sequence, paged, head_dim <= 128
+int32_t launch_paged_decode(DeviceState& ds, const PromptArgs& a);
 
 }  // namespace rstq

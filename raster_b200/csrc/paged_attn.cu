@@ -351,7 +351,9 @@ int32_t rstq_paged_decode_attention(rstq_ctx* ctx, rstq_buf* q, rstq_buf* kcache
     int32_t rc = attention_args(ctx, q, kcache, vcache, out, table, nullptr, lens, seqs, n_pages * page, seqs, n_q, group, n_kv, head_dim,
                                 page, n_pages, max_pages, ldq, 0, scale, 0, dtype, false, &a);
     if (rc != RSTQ_OK) return rc;
-    if ((rc = launch_attention_rows(ctx->devs[q->dev], a)) != RSTQ_OK) return rc;
+    DeviceState& ds = ctx->devs[q->dev];
+    rc = head_dim <= 128 ? launch_paged_decode(ds, a) : launch_attention_rows(ds, a);
+    if (rc != RSTQ_OK) return rc;
     ctx->launches++;
     return RSTQ_OK;
 }
