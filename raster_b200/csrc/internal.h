@@ -356,6 +356,8 @@ int32_t gemm_configure(DeviceState& ds);
 int32_t attn_configure(DeviceState& ds);  // scratch, shared-memory attributes and cluster counts, once per device
 // paged_decode.cu
 int32_t decode_configure(DeviceState& ds);  // shared-memory attributes, once per device
+// prompt_attn.cu
+int32_t prompt_configure();  // shared-memory attributes, once per device
 // pages.cu
 int32_t pages_configure(DeviceState& ds);  // scratch, shared-memory attributes, once per device
 // dx.cu

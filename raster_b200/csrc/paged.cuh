@@ -4,6 +4,7 @@
 // of the contiguous caches [position][n_kv][head_dim], cut into pages.  A sequence's row of the table names its pages in
 // order, so a contiguous cache is the pool whose table counts up.
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include "internal.h"
@@ -133,6 +134,101 @@ struct PromptArgs {
     int32_t dtype;
     int64_t kv_rows;        // rows of the pool or of the packed arrays
 };
+// ---- a row's attention by one warp, any shape ----
+// The lanes hold 16-byte pieces of the head, a dot product is a sum over them; kRowPos positions at a time, the softmax runs
+// along.  Only positions that the row sees are read, so what lies elsewhere (NaN too) cannot reach it.  Every sum in f32.
+constexpr int kRowPos = 4;
+template <typename T>
+struct RowState {
+    static constexpr int V = Elem<T>::kVec, C = 256 / (32 * V) < 1 ? 1 : 256 / (32 * V);   // elements of a piece; pieces of a lane
+    float o[C][V], m, l;
+};
+// Row `row` of head h, `behind` rows from its sequence's end (its own among them), against positions first .. first + kRowPos - 1, and
+// so on every `step`.  True: a position had no page.
+template <typename T>
+__device__ __forceinline__ bool attend_row(const PromptArgs& p, int b, int64_t row, int h, int64_t behind, int64_t first, int64_t step,
+                                           RowState<T>* st) {
+    constexpr int V = RowState<T>::V, C = RowState<T>::C;
+    const int lane = threadIdx.x & 31, hd = p.head_dim, hkv = h / p.group;
+    int64_t row0, len = kv_length(p.kv, b, &row0);
+    if (p.causal) len = clamp64(len - behind + 1, 0, len);
+    float q[C][V];
+    st->m = -INFINITY;
+    st->l = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int e = (c * 32 + lane) * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) q[c][i] = st->o[c][i] = 0.f;
+        if (e < hd) Elem<T>::load((const T*)p.q + row * p.ldq + (int64_t)h * hd + e, q[c]);
+    }
+    bool bad = false;
+    const float scale2 = p.scale * 1.4426950408889634f;
+    for (int64_t j0 = first; j0 < len; j0 += step) {
+        float s[kRowPos];
+        int64_t at[kRowPos];
+#pragma unroll
+        for (int u = 0; u < kRowPos; ++u) {
+            at[u] = j0 + u < len ? kv_row(p.kv, b, row0, j0 + u) : -1;
+            bad |= j0 + u < len && at[u] < 0;
+            s[u] = 0.f;
+            if (at[u] >= 0) {
+                const T* k = (const T*)p.k + at[u] * p.kv.ld + (int64_t)hkv * hd;
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const int e = (c * 32 + lane) * V;
+                    float x[V];
+                    if (e < hd) {
+                        Elem<T>::load(k + e, x);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) s[u] = fmaf(q[c][i], x[i], s[u]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1)
+#pragma unroll
+            for (int u = 0; u < kRowPos; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], d);
+        float top = st->m;
+#pragma unroll
+        for (int u = 0; u < kRowPos; ++u) {
+            s[u] = at[u] >= 0 ? s[u] * scale2 : -INFINITY;
+            top = s[u] > top || s[u] != s[u] ? s[u] : top;     // (a NaN stays one)
+        }
+        if (top == -INFINITY) continue;
+        const float w = exp2f(st->m - top);
+        st->l *= w;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < V; ++i) st->o[c][i] *= w;
+        st->m = top;
+#pragma unroll
+        for (int u = 0; u < kRowPos; ++u) {
+            if (at[u] < 0) continue;
+            const float e2 = exp2f(s[u] - top);
+            st->l += e2;
+            const T* v = (const T*)p.v + at[u] * p.kv.ld + (int64_t)hkv * hd;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int e = (c * 32 + lane) * V;
+                float x[V];
+                if (e < hd) {
+                    Elem<T>::load(v + e, x);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) st->o[c][i] = fmaf(e2, x[i], st->o[c][i]);
+                }
+            }
+        }
+    }
+    return bad;
+}
+
+// A pool (or packed rows) as [rows][heads][head_dim], read in boxes of 128 bytes x `box` rows of one head.
+int32_t rows_tensor_map(CUtensorMap* m, const void* base, int32_t dtype, int64_t rows, int64_t ld, int heads, int head_dim, int box);
+// prompt_attn.cu: bf16, head_dim <= 128, scale > 0
+int32_t launch_prompt(DeviceState& ds, const PromptArgs& a);
 // paged_attn.cu: any head_dim and length, a warp per position
 int32_t launch_attention_rows(DeviceState& ds, const PromptArgs& a);
 // paged_decode.cu: one row per sequence, paged, head_dim <= 128

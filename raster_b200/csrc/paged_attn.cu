@@ -110,23 +110,19 @@ paged_rope_append_kernel(const AppendParams p, const int per_block) {
 }
 
 // ---- attention, any shape -----------------------------------------------------------------------
-// One query row and head per thread block.  A warp takes every fourth position, four at a time: its lanes hold 16-byte
-// pieces of the head, a dot product is a sum over the lanes; the softmax runs along (running maximum and sum per warp), and the
-// four warps' states are joined through shared memory.  Only positions that the row sees are read, so what lies
-// elsewhere (NaN too) cannot reach it.  Every sum in f32.
+// One query row and head per thread block: its four warps take four positions in turn (attend_row), and their states are joined
+// through shared memory.
 constexpr int kRowWarps = 4;
-constexpr int kRowPos = 4;
 template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32)
 attention_rows_kernel(const PromptArgs p) {
-    constexpr int V = Elem<T>::kVec, C = 256 / (32 * V) < 1 ? 1 : 256 / (32 * V);   // pieces of a lane
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     __shared__ float s_o[kRowWarps][256];
     __shared__ float s_ml[kRowWarps][2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hd = p.head_dim;
     const int64_t item = blockIdx.x, row = item / p.n_q;
-    const int h = (int)(item - row * p.n_q), hkv = h / p.group;
+    const int h = (int)(item - row * p.n_q);
     int b = (int)row;
     int64_t behind = 1;
     if (p.cu_q) {
@@ -134,85 +130,16 @@ attention_rows_kernel(const PromptArgs p) {
         if (b < 0) return;
         behind = (int64_t)p.cu_q[b + 1] - row;
     }
-    int64_t row0, len = kv_length(p.kv, b, &row0);
-    if (p.causal) len = clamp64(len - behind + 1, 0, len);
-    float q[C][V], o[C][V], m = -INFINITY, l = 0.f;
+    RowState<T> st;
+    if (attend_row(p, b, row, h, behind, warp * kRowPos, kRowWarps * kRowPos, &st) && lane == 0) p.kv.status[kStatusPage] = 1;
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const int e = (c * 32 + lane) * V;
+    for (int c = 0; c < RowState<T>::C; ++c)
 #pragma unroll
-        for (int i = 0; i < V; ++i) q[c][i] = o[c][i] = 0.f;
-        if (e < hd) Elem<T>::load((const T*)p.q + row * p.ldq + (int64_t)h * hd + e, q[c]);
-    }
-    bool bad = false;
-    const float scale2 = p.scale * 1.4426950408889634f;
-    for (int64_t j0 = warp * kRowPos; j0 < len; j0 += kRowWarps * kRowPos) {
-        float s[kRowPos];
-        int64_t at[kRowPos];
-#pragma unroll
-        for (int u = 0; u < kRowPos; ++u) {
-            at[u] = j0 + u < len ? kv_row(p.kv, b, row0, j0 + u) : -1;
-            bad |= j0 + u < len && at[u] < 0;
-            s[u] = 0.f;
-            if (at[u] >= 0) {
-                const T* k = (const T*)p.k + at[u] * p.kv.ld + (int64_t)hkv * hd;
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const int e = (c * 32 + lane) * V;
-                    float x[V];
-                    if (e < hd) {
-                        Elem<T>::load(k + e, x);
-#pragma unroll
-                        for (int i = 0; i < V; ++i) s[u] = fmaf(q[c][i], x[i], s[u]);
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int d = 16; d; d >>= 1)
-#pragma unroll
-            for (int u = 0; u < kRowPos; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], d);
-        float top = m;
-#pragma unroll
-        for (int u = 0; u < kRowPos; ++u) {
-            s[u] = at[u] >= 0 ? s[u] * scale2 : -INFINITY;
-            top = s[u] > top || s[u] != s[u] ? s[u] : top;     // (a NaN stays one)
-        }
-        if (top == -INFINITY) continue;
-        const float w = exp2f(m - top);
-        l *= w;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int i = 0; i < V; ++i) o[c][i] *= w;
-        m = top;
-#pragma unroll
-        for (int u = 0; u < kRowPos; ++u) {
-            if (at[u] < 0) continue;
-            const float e2 = exp2f(s[u] - m);
-            l += e2;
-            const T* v = (const T*)p.v + at[u] * p.kv.ld + (int64_t)hkv * hd;
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int e = (c * 32 + lane) * V;
-                float x[V];
-                if (e < hd) {
-                    Elem<T>::load(v + e, x);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) o[c][i] = fmaf(e2, x[i], o[c][i]);
-                }
-            }
-        }
-    }
-    if (bad && lane == 0) p.kv.status[kStatusPage] = 1;
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if ((c * 32 + lane) * V < hd) s_o[warp][(c * 32 + lane) * V + i] = o[c][i];
+        for (int i = 0; i < RowState<T>::V; ++i)
+            if ((c * 32 + lane) * RowState<T>::V < hd) s_o[warp][(c * 32 + lane) * RowState<T>::V + i] = st.o[c][i];
     if (lane == 0) {
-        s_ml[warp][0] = m;
-        s_ml[warp][1] = l;
+        s_ml[warp][0] = st.m;
+        s_ml[warp][1] = st.l;
     }
     __syncthreads();
     float top = -INFINITY, total = 0.f, w[kRowWarps];
@@ -360,7 +287,8 @@ int32_t rstq_paged_decode_attention(rstq_ctx* ctx, rstq_buf* q, rstq_buf* kcache
 
 static int32_t run_prompt(rstq_ctx* ctx, rstq_buf* q, const PromptArgs& a) {
     if (a.rows == 0) return RSTQ_OK;
-    const int32_t rc = launch_attention_rows(ctx->devs[q->dev], a);
+    DeviceState& ds = ctx->devs[q->dev];
+    const int32_t rc = a.dtype == RSTQ_BF16 && a.head_dim <= 128 && a.scale > 0.f && a.kv_rows > 0 ? launch_prompt(ds, a) : launch_attention_rows(ds, a);
     if (rc == RSTQ_OK) ctx->launches++;
     return rc;
 }

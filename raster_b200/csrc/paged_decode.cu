@@ -712,12 +712,11 @@ int32_t decode_configure(DeviceState& ds) {
     return RSTQ_OK;
 }
 
-// A pool (or packed rows) as [rows][n_kv][head_dim], read in boxes of 128 bytes x `box` rows of one head.
-int32_t kv_tensor_map(CUtensorMap* m, const void* base, int32_t dtype, int64_t rows, int64_t ld, int n_kv, int head_dim, int box) {
+int32_t rows_tensor_map(CUtensorMap* m, const void* base, int32_t dtype, int64_t rows, int64_t ld, int heads, int head_dim, int box) {
     const EncodeTiledFn enc = encode_tiled_fn();
     RSTQ_REQUIRE(enc, RSTQ_E_CUDA, "cuTensorMapEncodeTiled is not available");
     const cuuint64_t es = (cuuint64_t)elem_bytes(dtype);
-    const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)n_kv, (cuuint64_t)(rows > 0 ? rows : 1)};
+    const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)(rows > 0 ? rows : 1)};
     const cuuint64_t strides[2] = {head_dim * es, (cuuint64_t)ld * es};
     const cuuint32_t bx[3] = {(cuuint32_t)(128 / es), 1u, (cuuint32_t)box}, ones[3] = {1u, 1u, 1u};
     const CUresult r = enc(m, dtype == RSTQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(base), dims,
@@ -742,8 +741,8 @@ int32_t launch_paged_decode(DeviceState& ds, const PromptArgs& a) {
     const int page = 1 << a.kv.shift, tile = a.dtype == RSTQ_BF16 ? dec_tile<__nv_bfloat16>() : dec_tile<float>();
     p.box = std::min(page, tile);
     CUtensorMap kmap, vmap;
-    int32_t rc = kv_tensor_map(&kmap, a.k, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
-    if (rc == RSTQ_OK) rc = kv_tensor_map(&vmap, a.v, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
+    int32_t rc = rows_tensor_map(&kmap, a.k, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
+    if (rc == RSTQ_OK) rc = rows_tensor_map(&vmap, a.v, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc != RSTQ_OK) return rc;
     const int64_t blocks = 2 * (int64_t)ds.sm_count;
     static_assert(2 * dec_slot<128>() >= 2 * dec_slot<64>(), "slots");

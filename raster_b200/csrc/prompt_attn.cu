@@ -1,0 +1,513 @@
+// Causal attention of whole prompts, bf16, head_dim up to 128, on the tcgen05 tensor cores.
+//
+//   out[i] = sum_j p_ij V[j] / sum_j p_ij,   p_ij = exp(scale q_i.K_j - m_i),   j <= i + (keys - rows) of its sequence
+//
+// A thread block has 256 query rows of one sequence and head as two tiles of 128, and walks the sequence's keys in tiles of 128:
+//
+//   S = Q K^T   (tcgen05, Q and K from shared memory, S in tensor memory)
+//   P = exp2(scale2 S - m)   (a warpgroup per query tile, a thread per row: S from tensor memory, P back over it in bf16)
+//   O += P V    (tcgen05, P from tensor memory, V from shared memory as it lies: an operand with head_dim innermost)
+//
+// While one tile's warpgroup is at its exponentials the tensor core works for the other tile.  The running maximum of a row moves
+// only when it grows by more than 2^8: until then P is up to 256 and O need not be rescaled (sums are f32; P's relative rounding
+// does not depend on its size), so O is read and written back for a few tiles at the start of a row and hardly ever after.
+// P is rounded to bf16, the type of V (2^-9 rms of each weight, no more than the result's own rounding); its sum is taken before that.
+//
+// K and V come by TMA through one ring, a box of 128 packed rows or one per page.  Keys a row does not see get -inf before the
+// maximum.  V's rows behind a sequence's end (another sequence's, a stale page's) are zeroed in shared memory before the product, for
+// 0 * NaN is NaN; what lies above the diagonal cannot be zeroed, it belongs to other rows: a warp looks through those few tiles, and where
+// it finds an infinity or NaN the block's rows are computed again one by one, from the positions they see alone (attend_row).
+// So are those of a block whose table names no page.
+#include <algorithm>
+
+#include "paged.cuh"
+#include "sync_helpers.cuh"
+#include "tcgen05_helpers.cuh"
+
+namespace rstq {
+
+constexpr int kPrThreads = 384;      // two warpgroups of softmax; copies, MMAs, V's edges
+constexpr int kPrRows = 128;         // rows of a query tile, keys of a tile
+template <int HD>
+struct PromptShape {
+    static constexpr int blks = HD / 64, tile = kPrRows * HD * 2, stages = HD == 128 ? 5 : 8;
+    static constexpr int smem = 1024 + (2 + stages) * tile;
+};
+constexpr float kGrow = 8.f;         // log2 of how far a row's largest weight may go beyond 1
+
+struct PromptParams {
+    PromptArgs a;
+    int tiles;                       // query tiles of a block: 1 or 2
+    int box;                         // rows of a box of keys
+    float scale2;
+    int* status;
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+        "%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+          "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+        "%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+        "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem desc]
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.b32 p, %4, 0; "
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// V as it lies, [keys][head_dim] in blocks of 64 columns: an operand whose N is innermost.  128-byte swizzle; 64-column blocks
+// `block` bytes apart, groups of eight keys 1024.
+__device__ __forceinline__ uint64_t smem_desc_rows(uint32_t saddr, uint32_t block) {
+    uint64_t d = smem_desc_sw128(saddr);
+    d &= ~(0x3FFFull << 16);
+    return d | (uint64_t)(block >> 4) << 16;
+}
+__device__ __forceinline__ float ex2f(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// What a block works on: rows [first, first + n) of the packed q, sequence b.
+struct PromptItem {
+    int b, rows;           // sequence, rows of it in this block (0: nothing to do)
+    int64_t row;           // the first one, packed
+    int behind;            // rows from the first one to the sequence's end
+    int keys, row0;        // keys of the sequence; packed: the first one's row
+};
+// Block `item` of those of all sequences, `per` rows each; counted from the end, so that the blocks with most keys of a
+// long sequence come first.  A warp's lanes work together and get the same answer.
+__device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, int per, int item) {
+    const int lane = threadIdx.x & 31;
+    auto rows_of = [&](int b, int64_t* first) {
+        int64_t last;
+        *first = 0;
+        if (b >= a.seqs) return 0;
+        packed_range(a.cu_q, b, a.rows, first, &last);
+        return (int)(last - *first);
+    };
+    PromptItem it;
+    it.rows = 0;
+    int base = 0;
+    for (int b0 = (a.seqs - 1) & ~31; b0 >= 0; b0 -= 32) {
+        int64_t first;
+        const int b = b0 + 31 - lane, n = rows_of(b, &first), m = (n + per - 1) / per;
+        int x = m;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += y;
+        }
+        const unsigned behind = __ballot_sync(0xffffffffu, base + x > item);
+        if (behind) {
+            const int src = __ffs((int)behind) - 1;
+            const int end = __shfl_sync(0xffffffffu, base + x, src), rows = __shfl_sync(0xffffffffu, n, src);
+            const int block = end - 1 - item;              // (of the sequence, from its start)
+            if (block < 0 || (int64_t)block * per >= rows) return it;     // (sequences that overlap beyond counting)
+            it.b = b0 + 31 - src;
+            it.row = __shfl_sync(0xffffffffu, (int)first, src) + (int64_t)block * per;
+            it.behind = rows - block * per;
+            it.rows = it.behind < per ? it.behind : per;
+            int64_t row0;
+            it.keys = (int)kv_length(a.kv, it.b, &row0);
+            it.row0 = (int)row0;
+            return it;
+        }
+        base += __shfl_sync(0xffffffffu, x, 31);
+    }
+    return it;
+}
+
+// The block's rows one by one, from the positions they see alone.
+__device__ __noinline__ void prompt_rows(const PromptArgs& a, const PromptItem& it, int h, int warp, int warps) {
+    const int lane = threadIdx.x & 31;
+    using S = RowState<__nv_bfloat16>;
+    bool bad = false;
+    for (int r = warp; r < it.rows; r += warps) {
+        S st;
+        bad |= attend_row(a, it.b, it.row + r, h, it.behind - r, 0, kRowPos, &st);
+        const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
+        if (lane * S::V < a.head_dim)
+#pragma unroll
+            for (int i = 0; i < S::V; i += 4)
+                store4((__nv_bfloat16*)a.out + ((it.row + r) * a.n_q + h) * a.head_dim + lane * S::V + i,
+                       make_float4(st.o[0][i] * inv, st.o[0][i + 1] * inv, st.o[0][i + 2] * inv, st.o[0][i + 3] * inv));
+    }
+    if (bad && lane == 0) a.kv.status[kStatusPage] = 1;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kPrThreads, 1)
+prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+              const __grid_constant__ CUtensorMap vmap) {
+    using Sh = PromptShape<HD>;
+    constexpr int NST = Sh::stages, TILE = Sh::tile, BLK = kPrRows * 128;     // 64 columns of a tile
+    extern __shared__ uint8_t s_raw0[];
+    uint8_t* s_raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw0) + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(8) uint64_t s_bar[2 * NST + 9];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort, s_again;
+    __shared__ PromptItem s_item;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t sq = smem_u32(s_raw), ring = sq + 2 * TILE;
+    // full / empty: a stage of the ring (empty: by the MMAs that read it and by the warp at V's edges); qfull; sfull[t]: S of a tile is
+    // there; pfull[t]: P is, and O has its scale; odone[t]: P V is added; vfix: the last V's edge is zeroed; fixed: no V will
+    // be looked at any more
+    const uint32_t full = smem_u32(s_bar), empty = full + 8 * NST, qfull = empty + 8 * NST, sfull = qfull + 8, pfull = sfull + 16,
+                   odone = pfull + 16, vfix = odone + 16, fixed = vfix + 8;
+    volatile int* abort_flag = &s_abort;
+    const int h = blockIdx.x % p.a.n_q, hkv = h / p.a.group;
+    if (tid == 0) {
+        s_abort = s_again = 0;
+        for (int i = 0; i < NST; ++i) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, 2);
+        }
+        mbar_init(qfull, 1);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(sfull + 8 * t, 1);
+            mbar_init(pfull + 8 * t, 4);
+            mbar_init(odone + 8 * t, 1);
+        }
+        mbar_init(vfix, 1);
+        mbar_init(fixed, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    if (warp == 9) {
+        tmem_alloc(smem_u32(&s_tmem), 512);
+        tmem_relinquish();
+    }
+    if (tid == 8 * 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qmap)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (warp == 8) {
+        const PromptItem it = prompt_item(p.a, p.tiles * kPrRows, blockIdx.x / p.a.n_q);
+        if (lane == 0) s_item = it;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // (not before this block has its tensor memory)
+    const PromptItem it = s_item;
+    // Keys that row r of the block sees: the first `see0 + r` (causal), at least 0 and at most all.
+    const int see0 = p.a.causal ? it.keys - it.behind + 1 : it.keys, grow = p.a.causal;
+    auto sees = [&](int r) { return min(max(see0 + grow * r, 0), it.keys); };
+    int nt[2];
+    for (int t = 0; t < 2; ++t) {
+        const int last = min(it.rows, (t + 1) * kPrRows) - 1;
+        nt[t] = t < p.tiles && last >= t * kPrRows ? (sees(last) + kPrRows - 1) / kPrRows : 0;
+    }
+    const int n = max(nt[0], nt[1]);
+    const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + HD};
+
+    if (warp < 8) {
+        // ---- softmax: a thread per row ----
+        const int t = warp >> 2, steps = nt[t];
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int r = t * kPrRows + (warp & 3) * 32 + lane;
+        const int mine = sees(r), least = sees(t * kPrRows);      // keys of this row, of the tile's first
+        float m = -INFINITY, m2 = 0.f, sum = 0.f;                 // running maximum of S; scale2 times it (0: nothing seen yet)
+        bool ok = true;
+        for (int j = 0; j < steps; ++j) {
+            if (ok) ok = __all_sync(0xffffffffu, mbar_spin(sfull + 8 * t, j & 1, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t s[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(tS[t] + lanes + c * 32, s[c]);
+            tmem_ld_wait();
+            if ((j + 1) * kPrRows > least) {                      // some row of the tile does not see all of these keys
+                const int lim = mine - j * kPrRows;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) s[c][i] = c * 32 + i < lim ? s[c][i] : 0xFF800000u;
+            }
+            float top[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                top[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+                for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
+            }
+            const float rowmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            const bool grown = rowmax > m && !(rowmax * p.scale2 <= m2 + kGrow && m != -INFINITY);
+            if (__any_sync(0xffffffffu, grown)) {
+                float f = 1.f;
+                if (grown) {
+                    const float next = rowmax * p.scale2;
+                    f = m == -INFINITY ? 0.f : ex2f(m2 - next);
+                    m = rowmax;
+                    m2 = next;
+                    sum *= f;
+                }
+                if (j > 0) {
+                    ok = __all_sync(0xffffffffu, mbar_spin(odone + 8 * t, (j - 1) & 1, abort_flag));
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(tO[t] + lanes + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st32(tO[t] + lanes + c, o);
+                    }
+                }
+            }
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t w[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float a = ex2f(fmaf(__uint_as_float(s[2 * c + (i >> 4)][(2 * i) & 31]), p.scale2, -m2));
+                    const float b = ex2f(fmaf(__uint_as_float(s[2 * c + (i >> 4)][(2 * i + 1) & 31]), p.scale2, -m2));
+                    part[i & 1] += a;
+                    part[2 + (i & 1)] += b;
+                    w[i] = bf16_pair(a, b);
+                }
+                tmem_st32(tS[t] + lanes + c * 32, w);
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pfull + 8 * t);
+        }
+        // ---- the rows' results ----
+        if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_spin(fixed, 0, abort_flag));
+        if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_spin(odone + 8 * t, (steps - 1) & 1, abort_flag));
+        tc_fence_after();
+        if (ok && !*(volatile int*)&s_again) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            __nv_bfloat16* out = (__nv_bfloat16*)p.a.out + ((it.row + r) * p.a.n_q + h) * p.a.head_dim;
+#pragma unroll
+            for (int c = 0; c < HD; c += 32) {
+                uint32_t o[32];
+                if (steps > 0) {
+                    tmem_ld32(tO[t] + lanes + c, o);
+                    tmem_ld_wait();
+                }
+                if (r < it.rows && t < p.tiles)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        if (c + i >= p.a.head_dim) continue;
+                        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                        if (sum != 0.f) {
+                            auto x = [&](int e) { return __uint_as_float(o[i + e]) * inv; };
+                            v = make_uint4(bf16_pair(x(0), x(1)), bf16_pair(x(2), x(3)), bf16_pair(x(4), x(5)), bf16_pair(x(6), x(7)));
+                        }
+                        *reinterpret_cast<uint4*>(out + c + i) = v;
+                    }
+            }
+        }
+        if (ok && *(volatile int*)&s_again) prompt_rows(p.a, it, h, warp, 8);
+    } else if (warp == 8) {
+        // ---- copies: Q, then K and V tile by tile ----
+        bool ok = n > 0;
+        if (ok && lane == 0) {
+            mbar_expect_tx(qfull, (uint32_t)(p.tiles * TILE));
+            for (int t = 0; t < p.tiles; ++t)
+                for (int c = 0; c < Sh::blks; ++c) tma_load_3d(sq + t * TILE + c * BLK, &qmap, c * 64, h, (int)it.row + t * kPrRows, qfull);
+        }
+        const int boxes = kPrRows / p.box;
+        int s = 0;
+        uint32_t ph = 0;
+        for (int j = 0; j < n && ok; ++j) {
+            // rows of the boxes, a lane each; none behind the last key
+            int y = -1;
+            const int pos = j * kPrRows + lane * p.box;
+            if (lane < boxes && pos < it.keys) {
+                y = (int)kv_row(p.a.kv, it.b, it.row0, pos);
+                if (y < 0) s_again = 1;
+            }
+            __syncwarp();
+            const unsigned there = __ballot_sync(0xffffffffu, y >= 0);
+            const uint32_t bytes = (uint32_t)(__popc(there) * p.box * 128 * Sh::blks);
+            for (int kv = 0; kv < 2 && ok; ++kv) {
+                ok = __all_sync(0xffffffffu, mbar_block(empty + 8 * s, ph ^ 1u, abort_flag));
+                if (!ok) break;
+                const uint32_t bar = full + 8 * s, dst = ring + s * TILE;
+                if (lane == 0) {
+                    if (bytes) mbar_expect_tx(bar, bytes);
+                    else mbar_arrive(bar);
+                }
+                for (int g = 0; g < boxes; ++g) {
+                    const int row = __shfl_sync(0xffffffffu, y, g);
+                    if (lane == 0 && row >= 0)
+                        for (int c = 0; c < Sh::blks; ++c) tma_load_3d(dst + c * BLK + g * p.box * 128, kv ? &vmap : &kmap, c * 64, hkv, row, bar);
+                }
+                if (++s == NST) { s = 0; ph ^= 1u; }
+            }
+        }
+        if (!ok && n > 0) {      // copies under way are waited for (again with a limit)
+            volatile int none = 0;
+            mbar_wait(qfull, 0, const_cast<volatile int*>(&none));
+            for (int i = 0; i < NST; ++i) mbar_wait(full + 8 * i, ph ^ (i >= s ? 1u : 0u), const_cast<volatile int*>(&none));
+        }
+    } else if (warp == 9) {
+        // ---- MMAs ----
+        constexpr uint32_t id_s = idesc_bf16(128), id_o = idesc_bf16(HD) | (1u << 16);     // (bit 16: B with N innermost)
+        const uint32_t leader = lane == 0;
+        bool ok = n > 0;
+        int s = 0;                                            // the ring's next stage
+        uint32_t ph = 0;
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+            if (ok) ok = __all_sync(0xffffffffu, mbar_spin(bar, parity, abort_flag));
+            tc_fence_after();
+        };
+        auto step = [&]() { if (++s == NST) { s = 0; ph ^= 1u; } };
+        auto product_s = [&](int t, int stage) {
+            if (ok && leader) {
+                const uint64_t a = smem_desc_sw128(sq + t * TILE), b = smem_desc_sw128(ring + stage * TILE);
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) {
+                    const uint64_t o = (uint64_t)((k >> 2) * (BLK >> 4) + (k & 3) * 2);
+                    umma_f16(tS[t], a + o, b + o, id_s, k > 0);
+                }
+                umma_commit(sfull + 8 * t);
+            }
+            __syncwarp();
+        };
+        wait(qfull, 0);
+        wait(full + 8 * s, ph);
+        for (int t = 0; t < 2; ++t)
+            if (nt[t] > 0) product_s(t, s);
+        if (ok) umma_commit_if(empty + 8 * s, leader);
+        step();
+        for (int j = 0; j < n && ok; ++j) {
+            const int vs = s;
+            const uint32_t vph = ph;
+            step();
+            const int ks = s;
+            const uint32_t kph = ph;
+            if (j + 1 < n) step();
+            wait(full + 8 * vs, vph);
+            if (j == n - 1) wait(vfix, 0);
+            bool have_k = false;
+            for (int t = 0; t < 2 && ok; ++t) {
+                if (j < nt[t]) {
+                    wait(pfull + 8 * t, j & 1);
+                    if (ok && leader) {
+                        const uint64_t b = smem_desc_rows(ring + vs * TILE, BLK);
+#pragma unroll
+                        for (int k = 0; k < kPrRows / 16; ++k) umma_f16_ts(tO[t], tS[t] + k * 8, b + (uint64_t)(k * (2048 >> 4)), id_o, j > 0 || k > 0);
+                        umma_commit(odone + 8 * t);
+                    }
+                    __syncwarp();
+                }
+                if (t == 1 && ok) umma_commit_if(empty + 8 * vs, leader);
+                if (j + 1 < nt[t]) {
+                    if (!have_k) wait(full + 8 * ks, kph);
+                    have_k = true;
+                    product_s(t, ks);
+                }
+                if (t == 1 && j + 1 < n && ok) umma_commit_if(empty + 8 * ks, leader);
+            }
+        }
+        if (!ok && n > 0) {      // products under way are waited for (with a limit) before the memory they use is given up
+            volatile int none = 0;
+            umma_commit_if(vfix, leader);
+            mbar_wait(vfix, 0, const_cast<volatile int*>(&none));
+        }
+    } else if (warp == 10) {
+        // ---- V's edges ----
+        bool ok = n > 0;
+        const int seen_by_all = sees(0);
+        int s = 0;
+        uint32_t ph = 0;
+        for (int i = 0; i < 2 * n && ok; ++i) {
+            ok = __all_sync(0xffffffffu, mbar_block(full + 8 * s, ph, abort_flag));
+            if (!ok) break;
+            if (i & 1) {
+                const int j = i >> 1;
+                const uint32_t v = ring + s * TILE;
+                const int end = min(it.keys - j * kPrRows, kPrRows);
+                for (int e = end * 8 * Sh::blks + lane; e < kPrRows * 8 * Sh::blks; e += 32) {     // behind the last key: zeros
+                    const int row = e / (8 * Sh::blks), c = e - row * (8 * Sh::blks);
+                    sts128(v + (c >> 3) * BLK + row * 128 + ((c & 7) << 4), 0u, 0u, 0u, 0u);
+                }
+                if (j == n - 1) {
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(vfix);
+                }
+                // keys that some rows see and some do not
+                const int from = max(seen_by_all - j * kPrRows, 0);
+                uint32_t found = 0;
+                if (from < end) {
+#pragma unroll 8
+                    for (int e = from * 8 * Sh::blks + lane; e < end * 8 * Sh::blks; e += 32) {
+                        const int row = e / (8 * Sh::blks), c = e - row * (8 * Sh::blks);
+                        uint32_t x[4];
+                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(v + (c >> 3) * BLK + row * 128 + ((c & 7) << 4)));
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) found |= ((x[u] & 0x7FFF7FFFu) + 0x00800080u) & 0x80008000u;   // exponent of ones
+                    }
+                }
+                if (found) s_again = 1;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + 8 * s);
+            if (++s == NST) { s = 0; ph ^= 1u; }
+        }
+        if (lane == 0) mbar_arrive(fixed);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) tmem_dealloc(tmem, 512);
+    if (tid == 0 && s_abort) atomicExch(p.status, 2);
+}
+
+int32_t prompt_configure() {
+    constexpr auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    RSTQ_CUDA(cudaFuncSetAttribute(prompt_kernel<64>, attr, PromptShape<64>::smem));
+    RSTQ_CUDA(cudaFuncSetAttribute(prompt_kernel<128>, attr, PromptShape<128>::smem));
+    return RSTQ_OK;
+}
+
+int32_t launch_prompt(DeviceState& ds, const PromptArgs& a) {
+    PromptParams p;
+    p.a = a;
+    p.scale2 = a.scale * 1.4426950408889634f;
+    p.status = ds.status;
+    p.box = a.kv.table ? std::min(1 << a.kv.shift, kPrRows) : kPrRows;
+    // Two query tiles per block keep the tensor core busy; with fewer blocks than SMs one each does the rows sooner.
+    p.tiles = a.rows * a.n_q <= 2 * kPrRows * (int64_t)ds.sm_count / 2 ? 1 : 2;
+    const int per = p.tiles * kPrRows;
+    const int64_t blocks = (a.rows / per + std::min<int64_t>(a.seqs, a.rows)) * a.n_q;     // no sequence has more than this of them
+    RSTQ_REQUIRE(blocks < (1ll << 31), RSTQ_E_LIMIT, "%lld thread blocks", (long long)blocks);
+    CUtensorMap qmap, kmap, vmap;
+    int32_t rc = rows_tensor_map(&qmap, a.q, a.dtype, a.rows, a.ldq, a.n_q, a.head_dim, kPrRows);
+    if (rc == RSTQ_OK) rc = rows_tensor_map(&kmap, a.k, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
+    if (rc == RSTQ_OK) rc = rows_tensor_map(&vmap, a.v, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
+    if (rc != RSTQ_OK) return rc;
+    const dim3 grid((unsigned)blocks), block(kPrThreads);
+    RSTQ_CUDA(a.head_dim <= 64 ? launch_pdl(prompt_kernel<64>, grid, block, (size_t)PromptShape<64>::smem, ds, p, qmap, kmap, vmap)
+                               : launch_pdl(prompt_kernel<128>, grid, block, (size_t)PromptShape<128>::smem, ds, p, qmap, kmap, vmap));
+    return RSTQ_OK;
+}
+
+}  // namespace rstq
