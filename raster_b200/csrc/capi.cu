@@ -628,6 +628,7 @@ int32_t rstq_init(const int32_t* devices, rstq_ctx** ctxp, int32_t ndev) {
             if ((r = attn_configure(ds)) != RSTQ_OK) return r;
             if ((r = decode_configure(ds)) != RSTQ_OK) return r;
             if ((r = prompt_configure()) != RSTQ_OK) return r;
+            if ((r = prompt_f32_configure()) != RSTQ_OK) return r;
             if ((r = pages_configure(ds)) != RSTQ_OK) return r;
             RSTQ_CUDA(cudaStreamSynchronize(ds.stream));
             return RSTQ_OK;

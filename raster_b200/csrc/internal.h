@@ -357,7 +357,8 @@ int32_t attn_configure(DeviceState& ds);  // scratch, shared-memory attributes a
 // paged_decode.cu
 int32_t decode_configure(DeviceState& ds);  // shared-memory attributes, once per device
 // prompt_attn.cu
-int32_t prompt_configure();  // shared-memory attributes, once per device
+int32_t prompt_configure();      // shared-memory attributes, once per device
+int32_t prompt_f32_configure();
 // pages.cu
 int32_t pages_configure(DeviceState& ds);  // scratch, shared-memory attributes, once per device
 // dx.cu

@@ -288,7 +288,9 @@ int32_t rstq_paged_decode_attention(rstq_ctx* ctx, rstq_buf* q, rstq_buf* kcache
 static int32_t run_prompt(rstq_ctx* ctx, rstq_buf* q, const PromptArgs& a) {
     if (a.rows == 0) return RSTQ_OK;
     DeviceState& ds = ctx->devs[q->dev];
-    const int32_t rc = a.dtype == RSTQ_BF16 && a.head_dim <= 128 && a.scale > 0.f && a.kv_rows > 0 ? launch_prompt(ds, a) : launch_attention_rows(ds, a);
+    int32_t rc;
+    if (a.head_dim > 128 || a.scale <= 0.f || a.kv_rows == 0) rc = launch_attention_rows(ds, a);
+    else rc = a.dtype == RSTQ_BF16 ? launch_prompt(ds, a) : launch_prompt_f32(ds, a);
     if (rc == RSTQ_OK) ctx->launches++;
     return rc;
 }

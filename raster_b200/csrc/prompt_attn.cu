@@ -20,9 +20,7 @@
 // So are those of a block whose table names no page.
 #include <algorithm>
 
-#include "paged.cuh"
-#include "sync_helpers.cuh"
-#include "tcgen05_helpers.cuh"
+#include "prompt.cuh"
 
 namespace rstq {
 
@@ -33,7 +31,6 @@ struct PromptShape {
     static constexpr int blks = HD / 64, tile = kPrRows * HD * 2, stages = HD == 128 ? 5 : 8;
     static constexpr int smem = 1024 + (2 + stages) * tile;
 };
-constexpr float kGrow = 8.f;         // log2 of how far a row's largest weight may go beyond 1
 
 struct PromptParams {
     PromptArgs a;
@@ -43,114 +40,6 @@ struct PromptParams {
     int* status;
 };
 
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
-        "%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
-          "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
-        "%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
-        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
-        "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-        : "memory");
-}
-// D[tmem] (+)= A[tmem] * B[smem desc]
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{ .reg .pred p; setp.ne.b32 p, %4, 0; "
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// V as it lies, [keys][head_dim] in blocks of 64 columns: an operand whose N is innermost.  128-byte swizzle; 64-column blocks
-// `block` bytes apart, groups of eight keys 1024.
-__device__ __forceinline__ uint64_t smem_desc_rows(uint32_t saddr, uint32_t block) {
-    uint64_t d = smem_desc_sw128(saddr);
-    d &= ~(0x3FFFull << 16);
-    return d | (uint64_t)(block >> 4) << 16;
-}
-__device__ __forceinline__ float ex2f(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// What a block works on: rows [first, first + n) of the packed q, sequence b.
-struct PromptItem {
-    int b, rows;           // sequence, rows of it in this block (0: nothing to do)
-    int64_t row;           // the first one, packed
-    int behind;            // rows from the first one to the sequence's end
-    int keys, row0;        // keys of the sequence; packed: the first one's row
-};
-// Block `item` of those of all sequences, `per` rows each; counted from the end, so that the blocks with most keys of a
-// long sequence come first.  A warp's lanes work together and get the same answer.
-__device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, int per, int item) {
-    const int lane = threadIdx.x & 31;
-    auto rows_of = [&](int b, int64_t* first) {
-        int64_t last;
-        *first = 0;
-        if (b >= a.seqs) return 0;
-        packed_range(a.cu_q, b, a.rows, first, &last);
-        return (int)(last - *first);
-    };
-    PromptItem it;
-    it.rows = 0;
-    int base = 0;
-    for (int b0 = (a.seqs - 1) & ~31; b0 >= 0; b0 -= 32) {
-        int64_t first;
-        const int b = b0 + 31 - lane, n = rows_of(b, &first), m = (n + per - 1) / per;
-        int x = m;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, x, d);
-            if (lane >= d) x += y;
-        }
-        const unsigned behind = __ballot_sync(0xffffffffu, base + x > item);
-        if (behind) {
-            const int src = __ffs((int)behind) - 1;
-            const int end = __shfl_sync(0xffffffffu, base + x, src), rows = __shfl_sync(0xffffffffu, n, src);
-            const int block = end - 1 - item;              // (of the sequence, from its start)
-            if (block < 0 || (int64_t)block * per >= rows) return it;     // (sequences that overlap beyond counting)
-            it.b = b0 + 31 - src;
-            it.row = __shfl_sync(0xffffffffu, (int)first, src) + (int64_t)block * per;
-            it.behind = rows - block * per;
-            it.rows = it.behind < per ? it.behind : per;
-            int64_t row0;
-            it.keys = (int)kv_length(a.kv, it.b, &row0);
-            it.row0 = (int)row0;
-            return it;
-        }
-        base += __shfl_sync(0xffffffffu, x, 31);
-    }
-    return it;
-}
-
-// The block's rows one by one, from the positions they see alone.
-__device__ __noinline__ void prompt_rows(const PromptArgs& a, const PromptItem& it, int h, int warp, int warps) {
-    const int lane = threadIdx.x & 31;
-    using S = RowState<__nv_bfloat16>;
-    bool bad = false;
-    for (int r = warp; r < it.rows; r += warps) {
-        S st;
-        bad |= attend_row(a, it.b, it.row + r, h, it.behind - r, 0, kRowPos, &st);
-        const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
-        if (lane * S::V < a.head_dim)
-#pragma unroll
-            for (int i = 0; i < S::V; i += 4)
-                store4((__nv_bfloat16*)a.out + ((it.row + r) * a.n_q + h) * a.head_dim + lane * S::V + i,
-                       make_float4(st.o[0][i] * inv, st.o[0][i + 1] * inv, st.o[0][i + 2] * inv, st.o[0][i + 3] * inv));
-    }
-    if (bad && lane == 0) a.kv.status[kStatusPage] = 1;
-}
-
 template <int HD>
 __global__ void __launch_bounds__(kPrThreads, 1)
 prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -159,7 +48,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     constexpr int NST = Sh::stages, TILE = Sh::tile, BLK = kPrRows * 128;     // 64 columns of a tile
     extern __shared__ uint8_t s_raw0[];
     uint8_t* s_raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw0) + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) uint64_t s_bar[2 * NST + 9];
+    __shared__ __align__(8) uint64_t s_bar[2 * NST + 10];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_again;
     __shared__ PromptItem s_item;
@@ -167,9 +56,9 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     const uint32_t sq = smem_u32(s_raw), ring = sq + 2 * TILE;
     // full / empty: a stage of the ring (empty: by the MMAs that read it and by the warp at V's edges); qfull; sfull[t]: S of a tile is
     // there; pfull[t]: P is, and O has its scale; odone[t]: P V is added; vfix: the last V's edge is zeroed; fixed: no V will
-    // be looked at any more
+    // be looked at any more; over: all products are done, after a wait ran out
     const uint32_t full = smem_u32(s_bar), empty = full + 8 * NST, qfull = empty + 8 * NST, sfull = qfull + 8, pfull = sfull + 16,
-                   odone = pfull + 16, vfix = odone + 16, fixed = vfix + 8;
+                   odone = pfull + 16, vfix = odone + 16, fixed = vfix + 8, over = fixed + 8;
     volatile int* abort_flag = &s_abort;
     const int h = blockIdx.x % p.a.n_q, hkv = h / p.a.group;
     if (tid == 0) {
@@ -186,6 +75,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         }
         mbar_init(vfix, 1);
         mbar_init(fixed, 1);
+        mbar_init(over, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
     }
@@ -323,7 +213,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     }
             }
         }
-        if (ok && *(volatile int*)&s_again) prompt_rows(p.a, it, h, warp, 8);
+        if (ok && *(volatile int*)&s_again) prompt_rows<__nv_bfloat16>(p.a, it, h, warp, 8);
     } else if (warp == 8) {
         // ---- copies: Q, then K and V tile by tile ----
         bool ok = n > 0;
@@ -429,8 +319,8 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         }
         if (!ok && n > 0) {      // products under way are waited for (with a limit) before the memory they use is given up
             volatile int none = 0;
-            umma_commit_if(vfix, leader);
-            mbar_wait(vfix, 0, const_cast<volatile int*>(&none));
+            umma_commit_if(over, leader);
+            mbar_wait(over, 0, const_cast<volatile int*>(&none));
         }
     } else if (warp == 10) {
         // ---- V's edges ----

@@ -1,0 +1,373 @@
+// Causal attention of whole prompts, f32, head_dim up to 128, on the tcgen05 tensor cores: prompt_attn.cu's walk with every operand as
+// three bf16 terms.
+//
+//   x = x1 + x2 + x3, each the leading 8 bits of what is left (24 bits in all: exact);
+//   x y = x1 y1 + (x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1)          to 2^-24 of it
+//
+// for Q K^T and for P V alike: six MMAs instead of one.  The first product has a sum of its own in tensor memory and the five small ones
+// another: the tensor core's additions lose a little each, and so only every sixth counts (1000 keys: 3e-7 of the result,
+// against 2e-6 with one sum).  f32 FMAs would be bound by 72 TFLOP/s of the whole device, the six MMAs by a sixth of bf16's rate.
+//
+// A block has 128 query rows of one sequence and head.  Four warps fetch K and V, a tile of 64 keys at a time and one ahead in
+// registers, split them and write the terms to shared memory, swizzled as the tensor core wants them (zeros behind the last key);
+// four warps are the softmax, a thread per row, P's three terms over S in tensor memory; one thread issues.  With head_dim above 64 there
+// are two places for S and P, and the next tile's S is formed while this one's exponentials are; up to 64 two blocks share an SM.
+// An infinity or NaN has no such terms: a block that meets one (in keys or values its rows may not even see) computes its rows one by one
+// (attend_row), and so does one whose table names no page.
+#include <algorithm>
+
+#include "prompt.cuh"
+
+namespace rstq {
+
+constexpr int kPfThreads = 288;      // softmax, split, MMA
+constexpr int kPfRows = 128, kPfKeys = 64;
+template <int HD>
+struct PromptShapeF {
+    static constexpr int blks = HD / 64, qblk = kPfRows * 128, kblk = kPfKeys * 128;     // 64 columns of a term
+    static constexpr int qplane = blks * qblk, kplane = blks * kblk;
+    static constexpr int bufs = HD == 128 ? 2 : 1, cols = HD == 128 ? 512 : 256;          // places for S; tensor memory
+    static constexpr int smem = 1024 + 3 * (qplane + 2 * kplane);
+};
+
+struct PromptParamsF {
+    PromptArgs a;
+    float scale2;
+    int* status;
+};
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+                 "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+                 : "memory");
+}
+// The next eight bits of a pair of values, as bf16 pair; the values become what is left.
+__device__ __forceinline__ uint32_t next_term(float& a, float& b) {
+    const uint32_t w = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+    a -= __uint_as_float(w << 16);
+    b -= __uint_as_float(w & 0xFFFF0000u);
+    return w;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kPfThreads, PromptShapeF<HD>::bufs == 1 ? 2 : 1)
+prompt_f32_kernel(const PromptParamsF p) {
+    using Sh = PromptShapeF<HD>;
+    constexpr int NB = Sh::bufs;
+    extern __shared__ uint8_t s_raw0[];
+    uint8_t* s_raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw0) + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(8) uint64_t s_bar[11];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort, s_again;
+    __shared__ PromptItem s_item;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t sq = smem_u32(s_raw), sk = sq + 3 * Sh::qplane, sv = sk + 3 * Sh::kplane;
+    // qfull, kfull, vfull: the terms are written; kfree, vfree: the products that read them are done; sfull, pfull: S, P of a place;
+    // odone: P V is added; over: everything is, after a wait ran out
+    const uint32_t qfull = smem_u32(s_bar), kfull = qfull + 8, kfree = qfull + 16, vfull = qfull + 24, vfree = qfull + 32, sfull = qfull + 40,
+                   pfull = qfull + 56, odone = qfull + 72, over = qfull + 80;
+    volatile int* abort_flag = &s_abort;
+    const int h = blockIdx.x % p.a.n_q, hkv = h / p.a.group;
+    if (tid == 0) {
+        s_abort = s_again = 0;
+        mbar_init(qfull, 4);
+        mbar_init(kfull, 4);
+        mbar_init(kfree, 1);
+        mbar_init(vfull, 4);
+        mbar_init(vfree, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(sfull + 8 * i, 1);
+            mbar_init(pfull + 8 * i, 4);
+        }
+        mbar_init(odone, 1);
+        mbar_init(over, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    if (warp == 8) {
+        tmem_alloc(smem_u32(&s_tmem), Sh::cols);
+        tmem_relinquish();
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (warp == 0) {
+        const PromptItem it = prompt_item(p.a, kPfRows, blockIdx.x / p.a.n_q);
+        if (lane == 0) s_item = it;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // (not before this block has its tensor memory)
+    const PromptItem it = s_item;
+    const int see0 = p.a.causal ? it.keys - it.behind + 1 : it.keys, grow = p.a.causal;      // row r sees the first see0 + r keys
+    auto sees = [&](int r) { return min(max(see0 + grow * r, 0), it.keys); };
+    const int n = it.rows > 0 ? (sees(it.rows - 1) + kPfKeys - 1) / kPfKeys : 0;
+    const uint32_t tO = tmem + NB * 128;
+
+    if (warp < 4) {
+        // ---- softmax: a thread per row ----
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        const int r = warp * 32 + lane, mine = sees(r), least = sees(0);
+        float m = -INFINITY, m2 = 0.f, sum = 0.f;
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            const int buf = j % NB;
+            const uint32_t tS = tmem + buf * 128 + lanes;
+            if (ok) ok = __all_sync(0xffffffffu, mbar_spin(sfull + 8 * buf, (j / NB) & 1, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            float s[64];
+#pragma unroll
+            for (int c = 0; c < 64; c += 16) {
+                uint32_t a[16], b[16];
+                tmem_ld16(tS + c, a);
+                tmem_ld16(tS + 64 + c, b);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[c + i] = __uint_as_float(a[i]) + __uint_as_float(b[i]);
+            }
+            if ((j + 1) * kPfKeys > least) {
+                const int lim = mine - j * kPfKeys;
+#pragma unroll
+                for (int i = 0; i < 64; ++i) s[i] = i < lim ? s[i] : -INFINITY;
+            }
+            float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int i = 4; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
+            const float rowmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            const bool grown = rowmax > m && !(rowmax * p.scale2 <= m2 + kGrow && m != -INFINITY);
+            if (__any_sync(0xffffffffu, grown)) {
+                float f = 1.f;
+                if (grown) {
+                    const float next = rowmax * p.scale2;
+                    f = m == -INFINITY ? 0.f : ex2f(m2 - next);
+                    m = rowmax;
+                    m2 = next;
+                    sum *= f;
+                }
+                if (j > 0) {
+                    ok = __all_sync(0xffffffffu, mbar_spin(odone, (j - 1) & 1, abort_flag));
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < 2 * HD; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(tO + lanes + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st16(tO + lanes + c, o);
+                    }
+                }
+            }
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t w[3][16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float a = ex2f(fmaf(s[c * 32 + 2 * i], p.scale2, -m2)), b = ex2f(fmaf(s[c * 32 + 2 * i + 1], p.scale2, -m2));
+                    part[i & 1] += a;
+                    part[2 + (i & 1)] += b;
+                    w[0][i] = next_term(a, b);
+                    w[1][i] = next_term(a, b);
+                    w[2][i] = next_term(a, b);
+                }
+#pragma unroll
+                for (int x = 0; x < 3; ++x) tmem_st16(tS + x * 32 + c * 16, w[x]);
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            tmem_st_wait();
+            tc_fence_before();
+            // Two places: S of the last tile came before the last P V but one was done.  That is waited for here, while the last one cannot
+            // be done yet: afterwards a parity would not tell the two apart.
+            if (NB == 2 && j == n - 1 && j > 0) ok = __all_sync(0xffffffffu, mbar_spin(odone, (j - 1) & 1, abort_flag));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pfull + 8 * buf);
+        }
+        if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_spin(odone, (n - 1) & 1, abort_flag));
+        tc_fence_after();
+        // (s_again is set before the terms it is about are handed on, and the last product came after all of them)
+        if (ok && !*(volatile int*)&s_again) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            float* out = (float*)p.a.out + ((it.row + r) * p.a.n_q + h) * p.a.head_dim;
+#pragma unroll
+            for (int c = 0; c < HD; c += 16) {
+                uint32_t a[16], b[16];
+                if (n > 0) {
+                    tmem_ld16(tO + lanes + c, a);
+                    tmem_ld16(tO + lanes + HD + c, b);
+                    tmem_ld_wait();
+                }
+                if (r < it.rows)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        if (c + i >= p.a.head_dim) continue;
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        auto x = [&](int e) { return (__uint_as_float(a[i + e]) + __uint_as_float(b[i + e])) * inv; };
+                        if (sum != 0.f) v = make_float4(x(0), x(1), x(2), x(3));
+                        store4(out + c + i, v);
+                    }
+            }
+        }
+        if (ok && *(volatile int*)&s_again) prompt_rows<float>(p.a, it, h, warp, 4);
+    } else if (warp < 8) {
+        // ---- split ----
+        constexpr int LPR = HD / 4, RPI = 32 / LPR, NI = 16 / RPI;      // lanes of a row; rows of a load; loads of a warp's 16 rows
+        const int w = warp - 4, d = (lane % LPR) * 4, sub = lane / LPR;
+        const bool in = d < p.a.head_dim;
+        uint32_t top = 0;             // largest magnitude seen, as bits
+        auto write = [&](uint32_t base, int plane, int blk, int row, float4 x) {
+            top = max(max(top, max(__float_as_uint(x.x) & 0x7FFFFFFFu, __float_as_uint(x.y) & 0x7FFFFFFFu)),
+                      max(__float_as_uint(x.z) & 0x7FFFFFFFu, __float_as_uint(x.w) & 0x7FFFFFFFu));
+            const uint32_t at = base + (d >> 6) * blk + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 4) * 2;
+#pragma unroll
+            for (int t = 0; t < 3; ++t) {
+                const uint32_t a = next_term(x.x, x.y), b = next_term(x.z, x.w);
+                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + t * plane), "r"(a), "r"(b) : "memory");
+            }
+        };
+        auto hand = [&](uint32_t bar) {
+            if (top >= 0x7F800000u) s_again = 1;
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        bool ok = n > 0;
+        // this warp's 16 rows of a tile of K and V: their places, a lane each
+        auto places = [&](int j) {
+            const int pos = j * kPfKeys + w * 16 + (lane & 15);
+            int64_t row = -1;
+            if (j < n && pos < it.keys) {
+                row = kv_row(p.a.kv, it.b, it.row0, pos);
+                if (row < 0) s_again = 1;
+            }
+            return (int)row;
+        };
+        auto fetch = [&](float4 (&x)[NI], const void* base, int rows) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int row = __shfl_sync(0xffffffffu, rows, i * RPI + sub);
+                x[i] = in && row >= 0 ? *reinterpret_cast<const float4*>((const float*)base + (int64_t)row * p.a.kv.ld + (int64_t)hkv * p.a.head_dim + d)
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        };
+        float4 k[NI], v[NI];
+        int rows = places(0);
+        if (ok) {
+            fetch(k, p.a.k, rows);
+            for (int half = 0; half < 2; ++half) {
+                float4 x[NI];
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    const int row = w * 32 + half * 16 + i * RPI + sub;
+                    x[i] = in && row < it.rows ? *reinterpret_cast<const float4*>((const float*)p.a.q + (it.row + row) * p.a.ldq + (int64_t)h * p.a.head_dim + d)
+                                               : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int i = 0; i < NI; ++i) write(sq, Sh::qplane, Sh::qblk, w * 32 + half * 16 + i * RPI + sub, x[i]);
+            }
+            hand(qfull);
+        }
+        for (int j = 0; j < n && ok; ++j) {
+            fetch(v, p.a.v, rows);
+            rows = places(j + 1);
+            ok = __all_sync(0xffffffffu, mbar_block(kfree, (j & 1) ^ 1u, abort_flag));
+            if (!ok) break;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) write(sk, Sh::kplane, Sh::kblk, w * 16 + i * RPI + sub, k[i]);
+            hand(kfull);
+            if (j + 1 < n) fetch(k, p.a.k, rows);
+            ok = __all_sync(0xffffffffu, mbar_block(vfree, (j & 1) ^ 1u, abort_flag));
+            if (!ok) break;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) write(sv, Sh::kplane, Sh::kblk, w * 16 + i * RPI + sub, v[i]);
+            hand(vfull);
+        }
+    } else {
+        // ---- MMAs ----
+        constexpr uint32_t id_s = idesc_bf16(kPfKeys), id_o = idesc_bf16(HD) | (1u << 16);     // (bit 16: B with N innermost)
+        const uint32_t leader = lane == 0;
+        bool ok = n > 0;
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+            if (ok) ok = __all_sync(0xffffffffu, mbar_spin(bar, parity, abort_flag));
+            tc_fence_after();
+        };
+        // terms of the products: the first to the first sum, the others to the second
+        constexpr int ta[6] = {0, 0, 1, 1, 0, 2}, tb[6] = {0, 1, 0, 1, 2, 0};
+        auto product_s = [&](int j) {
+            const uint32_t tS = tmem + (j % NB) * 128;
+            wait(kfull, j & 1);
+            if (ok && leader) {
+                for (int x = 0; x < 6; ++x) {
+                    const uint64_t a = smem_desc_sw128(sq + ta[x] * Sh::qplane), b = smem_desc_sw128(sk + tb[x] * Sh::kplane);
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k)
+                        umma_f16(tS + (x ? 64 : 0), a + (uint64_t)((k >> 2) * (Sh::qblk >> 4) + (k & 3) * 2),
+                                 b + (uint64_t)((k >> 2) * (Sh::kblk >> 4) + (k & 3) * 2), id_s, x > 1 || k > 0);
+                }
+                umma_commit(sfull + 8 * (j % NB));
+                umma_commit(kfree);
+            }
+            __syncwarp();
+        };
+        wait(qfull, 0);
+        if (n > 0) product_s(0);
+        for (int j = 0; j < n && ok; ++j) {
+            const uint32_t tP = tmem + (j % NB) * 128;
+            if (NB == 2 && j + 1 < n) product_s(j + 1);
+            wait(vfull, j & 1);
+            wait(pfull + 8 * (j % NB), (j / NB) & 1);
+            if (ok && leader) {
+                for (int x = 0; x < 6; ++x) {
+                    const uint64_t b = smem_desc_rows(sv + tb[x] * Sh::kplane, Sh::kblk);
+#pragma unroll
+                    for (int k = 0; k < kPfKeys / 16; ++k)
+                        umma_f16_ts(tO + (x ? HD : 0), tP + ta[x] * 32 + k * 8, b + (uint64_t)(k * (2048 >> 4)), id_o, j > 0 || x > 1 || k > 0);
+                }
+                umma_commit(odone);
+                umma_commit(vfree);
+            }
+            __syncwarp();
+            if (NB == 1 && j + 1 < n) product_s(j + 1);
+        }
+        if (!ok && n > 0) {      // products under way are waited for (with a limit) before the memory they use is given up
+            volatile int none = 0;
+            umma_commit_if(over, leader);
+            mbar_wait(over, 0, const_cast<volatile int*>(&none));
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) tmem_dealloc(tmem, Sh::cols);
+    if (tid == 0 && s_abort) atomicExch(p.status, 2);
+}
+
+int32_t prompt_f32_configure() {
+    constexpr auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    RSTQ_CUDA(cudaFuncSetAttribute(prompt_f32_kernel<64>, attr, PromptShapeF<64>::smem));
+    RSTQ_CUDA(cudaFuncSetAttribute(prompt_f32_kernel<128>, attr, PromptShapeF<128>::smem));
+    return RSTQ_OK;
+}
+
+int32_t launch_prompt_f32(DeviceState& ds, const PromptArgs& a) {
+    PromptParamsF p;
+    p.a = a;
+    p.scale2 = a.scale * 1.4426950408889634f;
+    p.status = ds.status;
+    const int64_t blocks = (a.rows / kPfRows + std::min<int64_t>(a.seqs, a.rows)) * a.n_q;
+    RSTQ_REQUIRE(blocks < (1ll << 31), RSTQ_E_LIMIT, "%lld thread blocks", (long long)blocks);
+    const dim3 grid((unsigned)blocks), block(kPfThreads);
+    RSTQ_CUDA(a.head_dim <= 64 ? launch_pdl(prompt_f32_kernel<64>, grid, block, (size_t)PromptShapeF<64>::smem, ds, p)
+                               : launch_pdl(prompt_f32_kernel<128>, grid, block, (size_t)PromptShapeF<128>::smem, ds, p));
+    return RSTQ_OK;
+}
+
+}  // namespace rstq
