@@ -48,16 +48,16 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     constexpr int NST = Sh::stages, TILE = Sh::tile, BLK = kPrRows * 128;     // 64 columns of a tile
     extern __shared__ uint8_t s_raw0[];
     uint8_t* s_raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw0) + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) uint64_t s_bar[2 * NST + 10];
+    __shared__ __align__(8) uint64_t s_bar[2 * NST + 12];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_again;
     __shared__ PromptItem s_item;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;      // (the same in all lanes, for the compiler too)
     const uint32_t sq = smem_u32(s_raw), ring = sq + 2 * TILE;
     // full / empty: a stage of the ring (empty: by the MMAs that read it and by the warp at V's edges); qfull; sfull[t]: S of a tile is
-    // there; pfull[t]: P is, and O has its scale; odone[t]: P V is added; vfix: the last V's edge is zeroed; fixed: no V will
+    // there; phalf[t], pfull[t]: half of P is, all of it, and O has its scale; odone[t]: P V is added; vfix: the last V's edge is zeroed; fixed: no V will
     // be looked at any more; over: all products are done, after a wait ran out
-    const uint32_t full = smem_u32(s_bar), empty = full + 8 * NST, qfull = empty + 8 * NST, sfull = qfull + 8, pfull = sfull + 16,
+    const uint32_t full = smem_u32(s_bar), empty = full + 8 * NST, qfull = empty + 8 * NST, sfull = qfull + 8, phalf = sfull + 16, pfull = phalf + 16,
                    odone = pfull + 16, vfix = odone + 16, fixed = vfix + 8, over = fixed + 8;
     volatile int* abort_flag = &s_abort;
     const int h = blockIdx.x % p.a.n_q, hkv = h / p.a.group;
@@ -70,6 +70,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         mbar_init(qfull, 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(sfull + 8 * t, 1);
+            mbar_init(phalf + 8 * t, 4);
             mbar_init(pfull + 8 * t, 4);
             mbar_init(odone + 8 * t, 1);
         }
@@ -112,6 +113,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
 
     if (warp < 8) {
         // ---- softmax: a thread per row ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int t = warp >> 2, steps = nt[t];
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const int r = t * kPrRows + (warp & 3) * 32 + lane;
@@ -119,27 +121,24 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         float m = -INFINITY, m2 = 0.f, sum = 0.f;                 // running maximum of S; scale2 times it (0: nothing seen yet)
         bool ok = true;
         for (int j = 0; j < steps; ++j) {
-            if (ok) ok = __all_sync(0xffffffffu, mbar_spin(sfull + 8 * t, j & 1, abort_flag));
+            if (ok) ok = wait_phase(sfull + 8 * t, j & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
-            uint32_t s[4][32];
+            uint32_t s[128];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(tS[t] + lanes + c * 32, s[c]);
-            tmem_ld_wait();
+            for (int c = 0; c < 128; c += 32) tmem_ld32_wait(tS[t] + lanes + c, s + c);
             if ((j + 1) * kPrRows > least) {                      // some row of the tile does not see all of these keys
                 const int lim = mine - j * kPrRows;
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) s[c][i] = c * 32 + i < lim ? s[c][i] : 0xFF800000u;
+                for (int i = 0; i < 128; ++i) s[i] = i < lim ? s[i] : 0xFF800000u;
             }
             float top[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                top[c] = __uint_as_float(s[c][0]);
+            for (int c = 0; c < 4; ++c) top[c] = fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 4]));
 #pragma unroll
-                for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
-            }
+            for (int i = 8; i < 128; i += 8)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) top[c] = fmaxf(fmaxf(top[c], __uint_as_float(s[i + c])), __uint_as_float(s[i + 4 + c]));
             const float rowmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             const bool grown = rowmax > m && !(rowmax * p.scale2 <= m2 + kGrow && m != -INFINITY);
             if (__any_sync(0xffffffffu, grown)) {
@@ -152,7 +151,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     sum *= f;
                 }
                 if (j > 0) {
-                    ok = __all_sync(0xffffffffu, mbar_spin(odone + 8 * t, (j - 1) & 1, abort_flag));
+                    ok = wait_phase(odone + 8 * t, (j - 1) & 1, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
@@ -166,29 +165,35 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     }
                 }
             }
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint64_t scale = pack2(p.scale2, p.scale2), minus = pack2(-m2, -m2);
+            uint64_t part[2] = {0ull, 0ull};
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                uint32_t w[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float a = ex2f(fmaf(__uint_as_float(s[2 * c + (i >> 4)][(2 * i) & 31]), p.scale2, -m2));
-                    const float b = ex2f(fmaf(__uint_as_float(s[2 * c + (i >> 4)][(2 * i + 1) & 31]), p.scale2, -m2));
-                    part[i & 1] += a;
-                    part[2 + (i & 1)] += b;
-                    w[i] = bf16_pair(a, b);
+              for (int hh = 0; hh < 2; ++hh) {
+                uint32_t w[16];
+#pragma unroll
+                for (int i0 = 0; i0 < 16; ++i0) { const int i = hh * 16 + i0;
+                    float a, b;
+                    unpack2(fma2(pack2(__uint_as_float(s[64 * c + 2 * i]), __uint_as_float(s[64 * c + 2 * i + 1])), scale, minus), a, b);
+                    a = ex2f(a);
+                    b = ex2f(b);
+                    part[i & 1] = add2(part[i & 1], pack2(a, b));
+                    w[i0] = bf16_pair(a, b);
                 }
-                tmem_st32(tS[t] + lanes + c * 32, w);
+                tmem_st16(tS[t] + lanes + c * 32 + hh * 16, w); }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive((c ? pfull : phalf) + 8 * t);
             }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(pfull + 8 * t);
+            float a, b;
+            unpack2(add2(part[0], part[1]), a, b);
+            sum += a + b;
         }
         // ---- the rows' results ----
-        if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_spin(fixed, 0, abort_flag));
-        if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_spin(odone + 8 * t, (steps - 1) & 1, abort_flag));
+        if (ok && n > 0) ok = wait_phase(fixed, 0, abort_flag);
+        if (ok && steps > 0) ok = wait_phase(odone + 8 * t, (steps - 1) & 1, abort_flag);
         tc_fence_after();
         if (ok && !*(volatile int*)&s_again) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -214,7 +219,9 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             }
         }
         if (ok && *(volatile int*)&s_again) prompt_rows<__nv_bfloat16>(p.a, it, h, warp, 8);
-    } else if (warp == 8) {
+    } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 8) {
         // ---- copies: Q, then K and V tile by tile ----
         bool ok = n > 0;
         if (ok && lane == 0) {
@@ -237,7 +244,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             const unsigned there = __ballot_sync(0xffffffffu, y >= 0);
             const uint32_t bytes = (uint32_t)(__popc(there) * p.box * 128 * Sh::blks);
             for (int kv = 0; kv < 2 && ok; ++kv) {
-                ok = __all_sync(0xffffffffu, mbar_block(empty + 8 * s, ph ^ 1u, abort_flag));
+                ok = wait_phase(empty + 8 * s, ph ^ 1u, abort_flag);
                 if (!ok) break;
                 const uint32_t bar = full + 8 * s, dst = ring + s * TILE;
                 if (lane == 0) {
@@ -254,8 +261,8 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         }
         if (!ok && n > 0) {      // copies under way are waited for (again with a limit)
             volatile int none = 0;
-            mbar_wait(qfull, 0, const_cast<volatile int*>(&none));
-            for (int i = 0; i < NST; ++i) mbar_wait(full + 8 * i, ph ^ (i >= s ? 1u : 0u), const_cast<volatile int*>(&none));
+            wait_phase(qfull, 0, const_cast<volatile int*>(&none));
+            for (int i = 0; i < NST; ++i) wait_phase(full + 8 * i, ph ^ (i >= s ? 1u : 0u), const_cast<volatile int*>(&none));
         }
     } else if (warp == 9) {
         // ---- MMAs ----
@@ -265,21 +272,21 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         int s = 0;                                            // the ring's next stage
         uint32_t ph = 0;
         auto wait = [&](uint32_t bar, uint32_t parity) {
-            if (ok) ok = __all_sync(0xffffffffu, mbar_spin(bar, parity, abort_flag));
+            if (ok) ok = wait_phase(bar, parity, abort_flag);
             tc_fence_after();
         };
         auto step = [&]() { if (++s == NST) { s = 0; ph ^= 1u; } };
+        // low words of descriptors (in 16 bytes) and their high word; V's: the blocks of 64 columns apart
+        const uint32_t hi = (uint32_t)(smem_desc_sw128(0) >> 32), lead = (uint32_t)smem_desc_sw128(0), lead_v = (uint32_t)smem_desc_rows(0, BLK);
         auto product_s = [&](int t, int stage) {
-            if (ok && leader) {
-                const uint64_t a = smem_desc_sw128(sq + t * TILE), b = smem_desc_sw128(ring + stage * TILE);
+            if (!ok) return;
+            const uint32_t a = lead + ((sq + t * TILE) >> 4), b = lead + ((ring + stage * TILE) >> 4);
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    const uint64_t o = (uint64_t)((k >> 2) * (BLK >> 4) + (k & 3) * 2);
-                    umma_f16(tS[t], a + o, b + o, id_s, k > 0);
-                }
-                umma_commit(sfull + 8 * t);
+            for (int k = 0; k < HD / 16; ++k) {
+                const uint32_t o = (k >> 2) * (BLK >> 4) + (k & 3) * 2;
+                umma_ss(tS[t], a + o, b + o, hi, id_s, k > 0, leader);
             }
-            __syncwarp();
+            umma_commit_if(sfull + 8 * t, leader);
         };
         wait(qfull, 0);
         wait(full + 8 * s, ph);
@@ -297,16 +304,18 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             wait(full + 8 * vs, vph);
             if (j == n - 1) wait(vfix, 0);
             bool have_k = false;
-            for (int t = 0; t < 2 && ok; ++t) {
-                if (j < nt[t]) {
-                    wait(pfull + 8 * t, j & 1);
-                    if (ok && leader) {
-                        const uint64_t b = smem_desc_rows(ring + vs * TILE, BLK);
 #pragma unroll
-                        for (int k = 0; k < kPrRows / 16; ++k) umma_f16_ts(tO[t], tS[t] + k * 8, b + (uint64_t)(k * (2048 >> 4)), id_o, j > 0 || k > 0);
-                        umma_commit(odone + 8 * t);
+            for (int t = 0; t < 2; ++t) {
+                if (j < nt[t]) {
+                    const uint32_t b = lead_v + ((ring + vs * TILE) >> 4);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {       // P's first half is there sooner
+                        wait((half ? pfull : phalf) + 8 * t, j & 1);
+                        if (!ok) break;
+#pragma unroll
+                        for (int k = half * 4; k < half * 4 + 4; ++k) umma_ts(tO[t], tS[t] + k * 8, b + k * (2048 >> 4), hi, id_o, j > 0 || k > 0, leader);
                     }
-                    __syncwarp();
+                    if (ok) umma_commit_if(odone + 8 * t, leader);
                 }
                 if (t == 1 && ok) umma_commit_if(empty + 8 * vs, leader);
                 if (j + 1 < nt[t]) {
@@ -320,7 +329,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         if (!ok && n > 0) {      // products under way are waited for (with a limit) before the memory they use is given up
             volatile int none = 0;
             umma_commit_if(over, leader);
-            mbar_wait(over, 0, const_cast<volatile int*>(&none));
+            wait_phase(over, 0, const_cast<volatile int*>(&none));
         }
     } else if (warp == 10) {
         // ---- V's edges ----
@@ -329,7 +338,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         int s = 0;
         uint32_t ph = 0;
         for (int i = 0; i < 2 * n && ok; ++i) {
-            ok = __all_sync(0xffffffffu, mbar_block(full + 8 * s, ph, abort_flag));
+            ok = wait_phase(full + 8 * s, ph, abort_flag);
             if (!ok) break;
             if (i & 1) {
                 const int j = i >> 1;
@@ -364,6 +373,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             if (++s == NST) { s = 0; ph ^= 1u; }
         }
         if (lane == 0) mbar_arrive(fixed);
+    }
     }
     tc_fence_before();
     __syncthreads();

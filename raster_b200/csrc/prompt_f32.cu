@@ -36,18 +36,6 @@ struct PromptParamsF {
     int* status;
 };
 
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
-                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-                 "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-                 : "memory");
-}
 // The next eight bits of a pair of values, as bf16 pair; the values become what is left.
 __device__ __forceinline__ uint32_t next_term(float& a, float& b) {
     const uint32_t w = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
@@ -67,7 +55,7 @@ prompt_f32_kernel(const PromptParamsF p) {
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_again;
     __shared__ PromptItem s_item;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;      // (the same in all lanes, for the compiler too)
     const uint32_t sq = smem_u32(s_raw), sk = sq + 3 * Sh::qplane, sv = sk + 3 * Sh::kplane;
     // qfull, kfull, vfull: the terms are written; kfree, vfree: the products that read them are done; sfull, pfull: S, P of a place;
     // odone: P V is added; over: everything is, after a wait ran out
@@ -120,7 +108,7 @@ prompt_f32_kernel(const PromptParamsF p) {
         for (int j = 0; j < n; ++j) {
             const int buf = j % NB;
             const uint32_t tS = tmem + buf * 128 + lanes;
-            if (ok) ok = __all_sync(0xffffffffu, mbar_spin(sfull + 8 * buf, (j / NB) & 1, abort_flag));
+            if (ok) ok = wait_phase(sfull + 8 * buf, (j / NB) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
             float s[64];
@@ -153,7 +141,7 @@ prompt_f32_kernel(const PromptParamsF p) {
                     sum *= f;
                 }
                 if (j > 0) {
-                    ok = __all_sync(0xffffffffu, mbar_spin(odone, (j - 1) & 1, abort_flag));
+                    ok = wait_phase(odone, (j - 1) & 1, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
@@ -188,11 +176,11 @@ prompt_f32_kernel(const PromptParamsF p) {
             tc_fence_before();
             // Two places: S of the last tile came before the last P V but one was done.  That is waited for here, while the last one cannot
             // be done yet: afterwards a parity would not tell the two apart.
-            if (NB == 2 && j == n - 1 && j > 0) ok = __all_sync(0xffffffffu, mbar_spin(odone, (j - 1) & 1, abort_flag));
+            if (NB == 2 && j == n - 1 && j > 0) ok = wait_phase(odone, (j - 1) & 1, abort_flag);
             __syncwarp();
             if (lane == 0) mbar_arrive(pfull + 8 * buf);
         }
-        if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_spin(odone, (n - 1) & 1, abort_flag));
+        if (ok && n > 0) ok = wait_phase(odone, (n - 1) & 1, abort_flag);
         tc_fence_after();
         // (s_again is set before the terms it is about are handed on, and the last product came after all of them)
         if (ok && !*(volatile int*)&s_again) {
@@ -279,13 +267,13 @@ prompt_f32_kernel(const PromptParamsF p) {
         for (int j = 0; j < n && ok; ++j) {
             fetch(v, p.a.v, rows);
             rows = places(j + 1);
-            ok = __all_sync(0xffffffffu, mbar_block(kfree, (j & 1) ^ 1u, abort_flag));
+            ok = wait_phase(kfree, (j & 1) ^ 1u, abort_flag);
             if (!ok) break;
 #pragma unroll
             for (int i = 0; i < NI; ++i) write(sk, Sh::kplane, Sh::kblk, w * 16 + i * RPI + sub, k[i]);
             hand(kfull);
             if (j + 1 < n) fetch(k, p.a.k, rows);
-            ok = __all_sync(0xffffffffu, mbar_block(vfree, (j & 1) ^ 1u, abort_flag));
+            ok = wait_phase(vfree, (j & 1) ^ 1u, abort_flag);
             if (!ok) break;
 #pragma unroll
             for (int i = 0; i < NI; ++i) write(sv, Sh::kplane, Sh::kblk, w * 16 + i * RPI + sub, v[i]);
@@ -297,26 +285,26 @@ prompt_f32_kernel(const PromptParamsF p) {
         const uint32_t leader = lane == 0;
         bool ok = n > 0;
         auto wait = [&](uint32_t bar, uint32_t parity) {
-            if (ok) ok = __all_sync(0xffffffffu, mbar_spin(bar, parity, abort_flag));
+            if (ok) ok = wait_phase(bar, parity, abort_flag);
             tc_fence_after();
         };
         // terms of the products: the first to the first sum, the others to the second
         constexpr int ta[6] = {0, 0, 1, 1, 0, 2}, tb[6] = {0, 1, 0, 1, 2, 0};
+        // low words of descriptors (in 16 bytes) and their high word; V's: the blocks of 64 columns apart
+        const uint32_t hi = (uint32_t)(smem_desc_sw128(0) >> 32), lead = (uint32_t)smem_desc_sw128(0), lead_v = (uint32_t)smem_desc_rows(0, Sh::kblk);
+        const uint32_t q0 = lead + (sq >> 4), k0 = lead + (sk >> 4), v0 = lead_v + (sv >> 4);
         auto product_s = [&](int j) {
             const uint32_t tS = tmem + (j % NB) * 128;
             wait(kfull, j & 1);
-            if (ok && leader) {
-                for (int x = 0; x < 6; ++x) {
-                    const uint64_t a = smem_desc_sw128(sq + ta[x] * Sh::qplane), b = smem_desc_sw128(sk + tb[x] * Sh::kplane);
+            if (!ok) return;
 #pragma unroll
-                    for (int k = 0; k < HD / 16; ++k)
-                        umma_f16(tS + (x ? 64 : 0), a + (uint64_t)((k >> 2) * (Sh::qblk >> 4) + (k & 3) * 2),
-                                 b + (uint64_t)((k >> 2) * (Sh::kblk >> 4) + (k & 3) * 2), id_s, x > 1 || k > 0);
-                }
-                umma_commit(sfull + 8 * (j % NB));
-                umma_commit(kfree);
-            }
-            __syncwarp();
+            for (int x = 0; x < 6; ++x)
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k)
+                    umma_ss(tS + (x ? 64 : 0), q0 + ta[x] * (Sh::qplane >> 4) + (k >> 2) * (Sh::qblk >> 4) + (k & 3) * 2,
+                            k0 + tb[x] * (Sh::kplane >> 4) + (k >> 2) * (Sh::kblk >> 4) + (k & 3) * 2, hi, id_s, x > 1 || k > 0, leader);
+            umma_commit_if(sfull + 8 * (j % NB), leader);
+            umma_commit_if(kfree, leader);
         };
         wait(qfull, 0);
         if (n > 0) product_s(0);
@@ -325,17 +313,15 @@ prompt_f32_kernel(const PromptParamsF p) {
             if (NB == 2 && j + 1 < n) product_s(j + 1);
             wait(vfull, j & 1);
             wait(pfull + 8 * (j % NB), (j / NB) & 1);
-            if (ok && leader) {
-                for (int x = 0; x < 6; ++x) {
-                    const uint64_t b = smem_desc_rows(sv + tb[x] * Sh::kplane, Sh::kblk);
+            if (!ok) break;
 #pragma unroll
-                    for (int k = 0; k < kPfKeys / 16; ++k)
-                        umma_f16_ts(tO + (x ? HD : 0), tP + ta[x] * 32 + k * 8, b + (uint64_t)(k * (2048 >> 4)), id_o, j > 0 || x > 1 || k > 0);
-                }
-                umma_commit(odone);
-                umma_commit(vfree);
-            }
-            __syncwarp();
+            for (int x = 0; x < 6; ++x)
+#pragma unroll
+                for (int k = 0; k < kPfKeys / 16; ++k)
+                    umma_ts(tO + (x ? HD : 0), tP + ta[x] * 32 + k * 8, v0 + tb[x] * (Sh::kplane >> 4) + k * (2048 >> 4), hi, id_o,
+                            j > 0 || x > 1 || k > 0, leader);
+            umma_commit_if(odone, leader);
+            umma_commit_if(vfree, leader);
             if (NB == 1 && j + 1 < n) product_s(j + 1);
         }
         if (!ok && n > 0) {      // products under way are waited for (with a limit) before the memory they use is given up
