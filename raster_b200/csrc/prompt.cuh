@@ -86,22 +86,31 @@ __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volati
         }
     }
 }
-// D[tmem] (+)= A * B by the lane whose `leader` is not 0; the whole warp is here, so that the operands stay in uniform registers (issued by one
-// lane in a branch of its own, an MMA of 64 cycles took 80).  Descriptors: low words, their common high word; A from shared or tensor memory.
-__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate, uint32_t leader) {
+// One lane of the warp, the same one every time: what it does in a branch on this is known to be done once, so operands stay in uniform
+// registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(r));
+    return r != 0;
+}
+// D[tmem] (+)= A * B, by the elected lane, from values that are the same in all lanes for the compiler too (a vote's or a reduction's result, not
+// what was read from memory): an MMA is then issued in 13 cycles, else in 65 - 80, more than it takes.  Descriptors: low words, their
+// common high word; A from shared or tensor memory.
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{ .reg .pred p, q; .reg .b64 a, b; setp.ne.b32 p, %5, 0; setp.ne.b32 q, %6, 0; mov.b64 a, {%1, %3}; mov.b64 b, {%2, %3}; "
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p; }" ::"r"(d),
-        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(leader)
+        "{ .reg .pred p; .reg .b64 a, b; setp.ne.b32 p, %5, 0; mov.b64 a, {%1, %3}; mov.b64 b, {%2, %3}; "
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p; }" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate, uint32_t leader) {
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{ .reg .pred p, q; .reg .b64 b; setp.ne.b32 p, %5, 0; setp.ne.b32 q, %6, 0; mov.b64 b, {%2, %3}; "
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p; }" ::"r"(d),
-        "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(leader)
+        "{ .reg .pred p; .reg .b64 b; setp.ne.b32 p, %5, 0; mov.b64 b, {%2, %3}; "
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p; }" ::"r"(d),
+        "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+__device__ __forceinline__ int uniform(int v) { return (int)__reduce_max_sync(0xffffffffu, v); }     // (the lanes' value is one already)
 // V as it lies, [keys][head_dim] in blocks of 64 columns: an operand whose N is innermost.  128-byte swizzle; 64-column blocks
 // `block` bytes apart, groups of eight keys 1024.
 __device__ __forceinline__ uint64_t smem_desc_rows(uint32_t saddr, uint32_t block) {

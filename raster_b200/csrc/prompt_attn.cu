@@ -97,7 +97,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = (uint32_t)uniform((int)s_tmem);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // (not before this block has its tensor memory)
     const PromptItem it = s_item;
     // Keys that row r of the block sees: the first `see0 + r` (causal), at least 0 and at most all.
@@ -106,7 +106,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     int nt[2];
     for (int t = 0; t < 2; ++t) {
         const int last = min(it.rows, (t + 1) * kPrRows) - 1;
-        nt[t] = t < p.tiles && last >= t * kPrRows ? (sees(last) + kPrRows - 1) / kPrRows : 0;
+        nt[t] = uniform(t < p.tiles && last >= t * kPrRows ? (sees(last) + kPrRows - 1) / kPrRows : 0);
     }
     const int n = max(nt[0], nt[1]);
     const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + HD};
@@ -267,7 +267,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     } else if (warp == 9) {
         // ---- MMAs ----
         constexpr uint32_t id_s = idesc_bf16(128), id_o = idesc_bf16(HD) | (1u << 16);     // (bit 16: B with N innermost)
-        const uint32_t leader = lane == 0;
+        const bool leader = elect_one();
         bool ok = n > 0;
         int s = 0;                                            // the ring's next stage
         uint32_t ph = 0;
@@ -284,7 +284,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k) {
                 const uint32_t o = (k >> 2) * (BLK >> 4) + (k & 3) * 2;
-                umma_ss(tS[t], a + o, b + o, hi, id_s, k > 0, leader);
+                if (leader) umma_ss(tS[t], a + o, b + o, hi, id_s, k > 0);
             }
             umma_commit_if(sfull + 8 * t, leader);
         };
@@ -313,7 +313,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                         wait((half ? pfull : phalf) + 8 * t, j & 1);
                         if (!ok) break;
 #pragma unroll
-                        for (int k = half * 4; k < half * 4 + 4; ++k) umma_ts(tO[t], tS[t] + k * 8, b + k * (2048 >> 4), hi, id_o, j > 0 || k > 0, leader);
+                        for (int k = half * 4; k < half * 4 + 4; ++k) if (leader) umma_ts(tO[t], tS[t] + k * 8, b + k * (2048 >> 4), hi, id_o, j > 0 || k > 0);
                     }
                     if (ok) umma_commit_if(odone + 8 * t, leader);
                 }

@@ -91,12 +91,12 @@ prompt_f32_kernel(const PromptParamsF p) {
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = (uint32_t)uniform((int)s_tmem);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // (not before this block has its tensor memory)
     const PromptItem it = s_item;
     const int see0 = p.a.causal ? it.keys - it.behind + 1 : it.keys, grow = p.a.causal;      // row r sees the first see0 + r keys
     auto sees = [&](int r) { return min(max(see0 + grow * r, 0), it.keys); };
-    const int n = it.rows > 0 ? (sees(it.rows - 1) + kPfKeys - 1) / kPfKeys : 0;
+    const int n = uniform(it.rows > 0 ? (sees(it.rows - 1) + kPfKeys - 1) / kPfKeys : 0);
     const uint32_t tO = tmem + NB * 128;
 
     if (warp < 4) {
@@ -282,7 +282,7 @@ prompt_f32_kernel(const PromptParamsF p) {
     } else {
         // ---- MMAs ----
         constexpr uint32_t id_s = idesc_bf16(kPfKeys), id_o = idesc_bf16(HD) | (1u << 16);     // (bit 16: B with N innermost)
-        const uint32_t leader = lane == 0;
+        const bool leader = elect_one();
         bool ok = n > 0;
         auto wait = [&](uint32_t bar, uint32_t parity) {
             if (ok) ok = wait_phase(bar, parity, abort_flag);
@@ -301,8 +301,8 @@ prompt_f32_kernel(const PromptParamsF p) {
             for (int x = 0; x < 6; ++x)
 #pragma unroll
                 for (int k = 0; k < HD / 16; ++k)
-                    umma_ss(tS + (x ? 64 : 0), q0 + ta[x] * (Sh::qplane >> 4) + (k >> 2) * (Sh::qblk >> 4) + (k & 3) * 2,
-                            k0 + tb[x] * (Sh::kplane >> 4) + (k >> 2) * (Sh::kblk >> 4) + (k & 3) * 2, hi, id_s, x > 1 || k > 0, leader);
+                    if (leader) umma_ss(tS + (x ? 64 : 0), q0 + ta[x] * (Sh::qplane >> 4) + (k >> 2) * (Sh::qblk >> 4) + (k & 3) * 2,
+                            k0 + tb[x] * (Sh::kplane >> 4) + (k >> 2) * (Sh::kblk >> 4) + (k & 3) * 2, hi, id_s, x > 1 || k > 0);
             umma_commit_if(sfull + 8 * (j % NB), leader);
             umma_commit_if(kfree, leader);
         };
@@ -318,8 +318,8 @@ prompt_f32_kernel(const PromptParamsF p) {
             for (int x = 0; x < 6; ++x)
 #pragma unroll
                 for (int k = 0; k < kPfKeys / 16; ++k)
-                    umma_ts(tO + (x ? HD : 0), tP + ta[x] * 32 + k * 8, v0 + tb[x] * (Sh::kplane >> 4) + k * (2048 >> 4), hi, id_o,
-                            j > 0 || x > 1 || k > 0, leader);
+                    if (leader) umma_ts(tO + (x ? HD : 0), tP + ta[x] * 32 + k * 8, v0 + tb[x] * (Sh::kplane >> 4) + k * (2048 >> 4), hi, id_o,
+                            j > 0 || x > 1 || k > 0);
             umma_commit_if(odone, leader);
             umma_commit_if(vfree, leader);
             if (NB == 1 && j + 1 < n) product_s(j + 1);
