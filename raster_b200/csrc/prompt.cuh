@@ -40,6 +40,16 @@ __device__ __forceinline__ void tmem_ld32_wait(uint32_t taddr, uint32_t* r) {
         : "r"(taddr)
         : "memory");
 }
+// 16 columns of this thread's row, there when the instruction is over.
+__device__ __forceinline__ void tmem_ld16_wait(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
 // pairs of f32 in one instruction
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
@@ -130,6 +140,10 @@ struct PromptItem {
     int64_t row;           // the first one, packed
     int behind;            // rows from the first one to the sequence's end
     int keys, row0;        // keys of the sequence; packed: the first one's row
+    // keys that row r of the block sees
+    __device__ __forceinline__ int sees(int r, int causal) const {
+        return causal ? min(max(keys - behind + 1 + r, 0), keys) : keys;
+    }
 };
 // Block `item` of those of all sequences, `per` rows each; counted from the end, so that the blocks with most keys of a
 // long sequence come first.  A warp's lanes work together and get the same answer.

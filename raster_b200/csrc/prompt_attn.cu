@@ -38,6 +38,12 @@ struct PromptParams {
     int box;                         // rows of a box of keys
     float scale2;
     int* status;
+    int* counters;                   // [0] items dealt out beyond the first of every block, [1] blocks that are done: zero between launches
+};
+// what a warp has to know of a block of rows
+struct PromptWork {
+    PromptItem it;
+    int h;                           // query head
 };
 
 template <int HD>
@@ -48,34 +54,39 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     constexpr int NST = Sh::stages, TILE = Sh::tile, BLK = kPrRows * 128;     // 64 columns of a tile
     extern __shared__ uint8_t s_raw0[];
     uint8_t* s_raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw0) + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) uint64_t s_bar[2 * NST + 12];
+    __shared__ __align__(8) uint64_t s_bar[2 * NST + 19];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort, s_again;
-    __shared__ PromptItem s_item;
+    __shared__ int s_abort;
+    __shared__ volatile int s_again[2];
+    __shared__ PromptWork s_work[2];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;      // (the same in all lanes, for the compiler too)
     const uint32_t sq = smem_u32(s_raw), ring = sq + 2 * TILE;
-    // full / empty: a stage of the ring (empty: by the MMAs that read it and by the warp at V's edges); qfull; sfull[t]: S of a tile is
-    // there; phalf[t], pfull[t]: half of P is, all of it, and O has its scale; odone[t]: P V is added; vfix: the last V's edge is zeroed; fixed: no V will
-    // be looked at any more; over: all products are done, after a wait ran out
-    const uint32_t full = smem_u32(s_bar), empty = full + 8 * NST, qfull = empty + 8 * NST, sfull = qfull + 8, phalf = sfull + 16, pfull = phalf + 16,
-                   odone = pfull + 16, vfix = odone + 16, fixed = vfix + 8, over = fixed + 8;
+    // full / empty: a stage of the ring (empty: by the MMAs that read it and by the warp at V's edges); qfull / qempty; sfull[t]: S of a
+    // tile is there; phalf[t], pfull[t]: half of P is, all of it, and O has its scale; odone[t]: P V is added; vfix[2]: the last V's edge is
+    // zeroed; fixed[2]: no V of these rows will be looked at any more; wfull[2] / wempty[2]: what to work on (all six by the number of the block
+    // of rows: a warp may be one ahead of another, never two); over: all products are done, after a wait ran out
+    const uint32_t full = smem_u32(s_bar), empty = full + 8 * NST, qfull = empty + 8 * NST, qempty = qfull + 8, sfull = qempty + 8,
+                   phalf = sfull + 16, pfull = phalf + 16, odone = pfull + 16, vfix = odone + 16, fixed = vfix + 16, wfull = fixed + 16,
+                   wempty = wfull + 16, over = wempty + 16;
     volatile int* abort_flag = &s_abort;
-    const int h = blockIdx.x % p.a.n_q, hkv = h / p.a.group;
     if (tid == 0) {
-        s_abort = s_again = 0;
+        s_abort = 0;
         for (int i = 0; i < NST; ++i) {
             mbar_init(full + 8 * i, 1);
             mbar_init(empty + 8 * i, 2);
         }
         mbar_init(qfull, 1);
+        mbar_init(qempty, 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(sfull + 8 * t, 1);
             mbar_init(phalf + 8 * t, 4);
             mbar_init(pfull + 8 * t, 4);
             mbar_init(odone + 8 * t, 1);
+            mbar_init(wfull + 8 * t, 1);
+            mbar_init(wempty + 8 * t, 10);
+            mbar_init(vfix + 8 * t, 1);
+            mbar_init(fixed + 8 * t, 1);
         }
-        mbar_init(vfix, 1);
-        mbar_init(fixed, 1);
         mbar_init(over, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
@@ -90,295 +101,360 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (warp == 8) {
-        const PromptItem it = prompt_item(p.a, p.tiles * kPrRows, blockIdx.x / p.a.n_q);
-        if (lane == 0) s_item = it;
-    }
+    PromptItem first;                // the block's first work, looked up while tensor memory is on its way
+    first.rows = 0;
+    if (warp == 8) first = prompt_item(p.a, p.tiles * kPrRows, blockIdx.x / p.a.n_q);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = (uint32_t)uniform((int)s_tmem);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // (not before this block has its tensor memory)
-    const PromptItem it = s_item;
-    // Keys that row r of the block sees: the first `see0 + r` (causal), at least 0 and at most all.
-    const int see0 = p.a.causal ? it.keys - it.behind + 1 : it.keys, grow = p.a.causal;
-    auto sees = [&](int r) { return min(max(see0 + grow * r, 0), it.keys); };
-    int nt[2];
-    for (int t = 0; t < 2; ++t) {
-        const int last = min(it.rows, (t + 1) * kPrRows) - 1;
-        nt[t] = uniform(t < p.tiles && last >= t * kPrRows ? (sees(last) + kPrRows - 1) / kPrRows : 0);
-    }
-    const int n = max(nt[0], nt[1]);
     const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + HD};
+    // steps of the two tiles of a block of rows: tiles of keys that some row of theirs sees
+    auto steps_of = [&](const PromptItem& it, int t) {
+        const int last = min(it.rows, (t + 1) * kPrRows) - 1;
+        return uniform(t < p.tiles && last >= t * kPrRows ? (it.sees(last, p.a.causal) + kPrRows - 1) / kPrRows : 0);
+    };
+    bool ok = true;
+    // The next block of rows, of which `w` is the number; false: there is none.
+    auto next_work = [&](int w, PromptWork* x) {
+        if (!wait_phase(wfull + 8 * (w & 1), (w >> 1) & 1, abort_flag)) {
+            ok = false;
+            return false;
+        }
+        *x = s_work[w & 1];
+        return uniform(x->it.rows) > 0;
+    };
+    auto done_work = [&](int w) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(wempty + 8 * (w & 1));
+    };
 
     if (warp < 8) {
         // ---- softmax: a thread per row ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        const int t = warp >> 2, steps = nt[t];
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int t = warp >> 2;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tSt = tS[0] + t * 128 + lanes, tOt = tO[0] + t * HD + lanes;
         const int r = t * kPrRows + (warp & 3) * 32 + lane;
-        const int mine = sees(r), least = sees(t * kPrRows);      // keys of this row, of the tile's first
-        float m = -INFINITY, m2 = 0.f, sum = 0.f;                 // running maximum of S; scale2 times it (0: nothing seen yet)
-        bool ok = true;
-        for (int j = 0; j < steps; ++j) {
-            if (ok) ok = wait_phase(sfull + 8 * t, j & 1, abort_flag);
-            if (!ok) break;
-            tc_fence_after();
-            uint32_t s[128];
-#pragma unroll
-            for (int c = 0; c < 128; c += 32) tmem_ld32_wait(tS[t] + lanes + c, s + c);
-            if ((j + 1) * kPrRows > least) {                      // some row of the tile does not see all of these keys
-                const int lim = mine - j * kPrRows;
-#pragma unroll
-                for (int i = 0; i < 128; ++i) s[i] = i < lim ? s[i] : 0xFF800000u;
-            }
-            float top[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) top[c] = fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 4]));
-#pragma unroll
-            for (int i = 8; i < 128; i += 8)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) top[c] = fmaxf(fmaxf(top[c], __uint_as_float(s[i + c])), __uint_as_float(s[i + 4 + c]));
-            const float rowmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            const bool grown = rowmax > m && !(rowmax * p.scale2 <= m2 + kGrow && m != -INFINITY);
-            if (__any_sync(0xffffffffu, grown)) {
-                float f = 1.f;
-                if (grown) {
-                    const float next = rowmax * p.scale2;
-                    f = m == -INFINITY ? 0.f : ex2f(m2 - next);
-                    m = rowmax;
-                    m2 = next;
-                    sum *= f;
-                }
-                if (j > 0) {
-                    ok = wait_phase(odone + 8 * t, (j - 1) & 1, abort_flag);
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < HD; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(tO[t] + lanes + c, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tmem_st32(tO[t] + lanes + c, o);
-                    }
-                }
-            }
-            const uint64_t scale = pack2(p.scale2, p.scale2), minus = pack2(-m2, -m2);
-            uint64_t part[2] = {0ull, 0ull};
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
-                uint32_t w[16];
-#pragma unroll
-                for (int i0 = 0; i0 < 16; ++i0) { const int i = hh * 16 + i0;
-                    float a, b;
-                    unpack2(fma2(pack2(__uint_as_float(s[64 * c + 2 * i]), __uint_as_float(s[64 * c + 2 * i + 1])), scale, minus), a, b);
-                    a = ex2f(a);
-                    b = ex2f(b);
-                    part[i & 1] = add2(part[i & 1], pack2(a, b));
-                    w[i0] = bf16_pair(a, b);
-                }
-                tmem_st16(tS[t] + lanes + c * 32 + hh * 16, w); }
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive((c ? pfull : phalf) + 8 * t);
-            }
-            float a, b;
-            unpack2(add2(part[0], part[1]), a, b);
-            sum += a + b;
-        }
-        // ---- the rows' results ----
-        if (ok && n > 0) ok = wait_phase(fixed, 0, abort_flag);
-        if (ok && steps > 0) ok = wait_phase(odone + 8 * t, (steps - 1) & 1, abort_flag);
-        tc_fence_after();
-        if (ok && !*(volatile int*)&s_again) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            __nv_bfloat16* out = (__nv_bfloat16*)p.a.out + ((it.row + r) * p.a.n_q + h) * p.a.head_dim;
-#pragma unroll
-            for (int c = 0; c < HD; c += 32) {
-                uint32_t o[32];
-                if (steps > 0) {
-                    tmem_ld32(tO[t] + lanes + c, o);
-                    tmem_ld_wait();
-                }
-                if (r < it.rows && t < p.tiles)
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        if (c + i >= p.a.head_dim) continue;
-                        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                        if (sum != 0.f) {
-                            auto x = [&](int e) { return __uint_as_float(o[i + e]) * inv; };
-                            v = make_uint4(bf16_pair(x(0), x(1)), bf16_pair(x(2), x(3)), bf16_pair(x(4), x(5)), bf16_pair(x(6), x(7)));
-                        }
-                        *reinterpret_cast<uint4*>(out + c + i) = v;
-                    }
-            }
-        }
-        if (ok && *(volatile int*)&s_again) prompt_rows<__nv_bfloat16>(p.a, it, h, warp, 8);
-    } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 8) {
-        // ---- copies: Q, then K and V tile by tile ----
-        bool ok = n > 0;
-        if (ok && lane == 0) {
-            mbar_expect_tx(qfull, (uint32_t)(p.tiles * TILE));
-            for (int t = 0; t < p.tiles; ++t)
-                for (int c = 0; c < Sh::blks; ++c) tma_load_3d(sq + t * TILE + c * BLK, &qmap, c * 64, h, (int)it.row + t * kPrRows, qfull);
-        }
-        const int boxes = kPrRows / p.box;
-        int s = 0;
-        uint32_t ph = 0;
-        for (int j = 0; j < n && ok; ++j) {
-            // rows of the boxes, a lane each; none behind the last key
-            int y = -1;
-            const int pos = j * kPrRows + lane * p.box;
-            if (lane < boxes && pos < it.keys) {
-                y = (int)kv_row(p.a.kv, it.b, it.row0, pos);
-                if (y < 0) s_again = 1;
-            }
-            __syncwarp();
-            const unsigned there = __ballot_sync(0xffffffffu, y >= 0);
-            const uint32_t bytes = (uint32_t)(__popc(there) * p.box * 128 * Sh::blks);
-            for (int kv = 0; kv < 2 && ok; ++kv) {
-                ok = wait_phase(empty + 8 * s, ph ^ 1u, abort_flag);
+        uint32_t c = 0;                      // steps of this tile so far (their parity is that of its barriers)
+        PromptWork x;
+        for (int w = 0; ok && next_work(w, &x); ++w) {
+            const PromptItem& it = x.it;
+            const int steps = steps_of(it, t);
+            const int mine = it.sees(r, p.a.causal), least = it.sees(t * kPrRows, p.a.causal);      // keys of this row, of the tile's first
+            float m = -INFINITY, m2 = 0.f, sum = 0.f;      // running maximum of S; scale2 times it (0: nothing seen yet)
+            for (int j = 0; j < steps; ++j) {
+                ok = wait_phase(sfull + 8 * t, (c + j) & 1, abort_flag);
                 if (!ok) break;
-                const uint32_t bar = full + 8 * s, dst = ring + s * TILE;
-                if (lane == 0) {
-                    if (bytes) mbar_expect_tx(bar, bytes);
-                    else mbar_arrive(bar);
+                tc_fence_after();
+                uint32_t s[128];
+#pragma unroll
+                for (int i = 0; i < 128; i += 32) tmem_ld32_wait(tSt + i, s + i);
+                if ((j + 1) * kPrRows > least) {           // some row of the tile does not see all of these keys
+                    const int lim = mine - j * kPrRows;
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) s[i] = i < lim ? s[i] : 0xFF800000u;
                 }
-                for (int g = 0; g < boxes; ++g) {
-                    const int row = __shfl_sync(0xffffffffu, y, g);
-                    if (lane == 0 && row >= 0)
-                        for (int c = 0; c < Sh::blks; ++c) tma_load_3d(dst + c * BLK + g * p.box * 128, kv ? &vmap : &kmap, c * 64, hkv, row, bar);
-                }
-                if (++s == NST) { s = 0; ph ^= 1u; }
-            }
-        }
-        if (!ok && n > 0) {      // copies under way are waited for (again with a limit)
-            volatile int none = 0;
-            wait_phase(qfull, 0, const_cast<volatile int*>(&none));
-            for (int i = 0; i < NST; ++i) wait_phase(full + 8 * i, ph ^ (i >= s ? 1u : 0u), const_cast<volatile int*>(&none));
-        }
-    } else if (warp == 9) {
-        // ---- MMAs ----
-        constexpr uint32_t id_s = idesc_bf16(128), id_o = idesc_bf16(HD) | (1u << 16);     // (bit 16: B with N innermost)
-        const bool leader = elect_one();
-        bool ok = n > 0;
-        int s = 0;                                            // the ring's next stage
-        uint32_t ph = 0;
-        auto wait = [&](uint32_t bar, uint32_t parity) {
-            if (ok) ok = wait_phase(bar, parity, abort_flag);
-            tc_fence_after();
-        };
-        auto step = [&]() { if (++s == NST) { s = 0; ph ^= 1u; } };
-        // low words of descriptors (in 16 bytes) and their high word; V's: the blocks of 64 columns apart
-        const uint32_t hi = (uint32_t)(smem_desc_sw128(0) >> 32), lead = (uint32_t)smem_desc_sw128(0), lead_v = (uint32_t)smem_desc_rows(0, BLK);
-        auto product_s = [&](int t, int stage) {
-            if (!ok) return;
-            const uint32_t a = lead + ((sq + t * TILE) >> 4), b = lead + ((ring + stage * TILE) >> 4);
+                float top[4];
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-                const uint32_t o = (k >> 2) * (BLK >> 4) + (k & 3) * 2;
-                if (leader) umma_ss(tS[t], a + o, b + o, hi, id_s, k > 0);
-            }
-            umma_commit_if(sfull + 8 * t, leader);
-        };
-        wait(qfull, 0);
-        wait(full + 8 * s, ph);
-        for (int t = 0; t < 2; ++t)
-            if (nt[t] > 0) product_s(t, s);
-        if (ok) umma_commit_if(empty + 8 * s, leader);
-        step();
-        for (int j = 0; j < n && ok; ++j) {
-            const int vs = s;
-            const uint32_t vph = ph;
-            step();
-            const int ks = s;
-            const uint32_t kph = ph;
-            if (j + 1 < n) step();
-            wait(full + 8 * vs, vph);
-            if (j == n - 1) wait(vfix, 0);
-            bool have_k = false;
+                for (int i = 0; i < 4; ++i) top[i] = fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 4]));
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                if (j < nt[t]) {
-                    const uint32_t b = lead_v + ((ring + vs * TILE) >> 4);
+                for (int i = 8; i < 128; i += 8)
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {       // P's first half is there sooner
-                        wait((half ? pfull : phalf) + 8 * t, j & 1);
+                    for (int u = 0; u < 4; ++u) top[u] = fmaxf(fmaxf(top[u], __uint_as_float(s[i + u])), __uint_as_float(s[i + 4 + u]));
+                const float rowmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                const bool grown = rowmax > m && !(rowmax * p.scale2 <= m2 + kGrow && m != -INFINITY);
+                if (__any_sync(0xffffffffu, grown)) {
+                    float f = 1.f;
+                    if (grown) {
+                        const float next = rowmax * p.scale2;
+                        f = m == -INFINITY ? 0.f : ex2f(m2 - next);
+                        m = rowmax;
+                        m2 = next;
+                        sum *= f;
+                    }
+                    if (j > 0) {      // (S of this step came after the P V of the last but one)
+                        ok = wait_phase(odone + 8 * t, (c + j - 1) & 1, abort_flag);
                         if (!ok) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int i = 0; i < HD; i += 16) {
+                            uint32_t o[16];
+                            tmem_ld16_wait(tOt + i, o);
 #pragma unroll
-                        for (int k = half * 4; k < half * 4 + 4; ++k) if (leader) umma_ts(tO[t], tS[t] + k * 8, b + k * (2048 >> 4), hi, id_o, j > 0 || k > 0);
+                            for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
+                            tmem_st16(tOt + i, o);
+                        }
                     }
-                    if (ok) umma_commit_if(odone + 8 * t, leader);
                 }
-                if (t == 1 && ok) umma_commit_if(empty + 8 * vs, leader);
-                if (j + 1 < nt[t]) {
-                    if (!have_k) wait(full + 8 * ks, kph);
-                    have_k = true;
-                    product_s(t, ks);
+                const uint64_t scale = pack2(p.scale2, p.scale2), minus = pack2(-m2, -m2);
+                uint64_t part[2] = {0ull, 0ull};
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    uint32_t v[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float a, b;
+                        unpack2(fma2(pack2(__uint_as_float(s[32 * g + 2 * i]), __uint_as_float(s[32 * g + 2 * i + 1])), scale, minus), a, b);
+                        a = ex2f(a);
+                        b = ex2f(b);
+                        part[i & 1] = add2(part[i & 1], pack2(a, b));
+                        v[i] = bf16_pair(a, b);
+                    }
+                    tmem_st16(tSt + 16 * g, v);
+                    if (g & 1) {
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive((g == 3 ? pfull : phalf) + 8 * t);
+                    }
                 }
-                if (t == 1 && j + 1 < n && ok) umma_commit_if(empty + 8 * ks, leader);
+                float a, b;
+                unpack2(add2(part[0], part[1]), a, b);
+                sum += a + b;
             }
-        }
-        if (!ok && n > 0) {      // products under way are waited for (with a limit) before the memory they use is given up
-            volatile int none = 0;
-            umma_commit_if(over, leader);
-            wait_phase(over, 0, const_cast<volatile int*>(&none));
-        }
-    } else if (warp == 10) {
-        // ---- V's edges ----
-        bool ok = n > 0;
-        const int seen_by_all = sees(0);
-        int s = 0;
-        uint32_t ph = 0;
-        for (int i = 0; i < 2 * n && ok; ++i) {
-            ok = wait_phase(full + 8 * s, ph, abort_flag);
+            // ---- the rows' results ----
+            c += steps;
+            if (ok) ok = wait_phase(fixed + 8 * (w & 1), (w >> 1) & 1, abort_flag);
+            if (steps > 0 && ok) ok = wait_phase(odone + 8 * t, (c - 1) & 1, abort_flag);
             if (!ok) break;
-            if (i & 1) {
-                const int j = i >> 1;
-                const uint32_t v = ring + s * TILE;
-                const int end = min(it.keys - j * kPrRows, kPrRows);
-                for (int e = end * 8 * Sh::blks + lane; e < kPrRows * 8 * Sh::blks; e += 32) {     // behind the last key: zeros
-                    const int row = e / (8 * Sh::blks), c = e - row * (8 * Sh::blks);
-                    sts128(v + (c >> 3) * BLK + row * 128 + ((c & 7) << 4), 0u, 0u, 0u, 0u);
-                }
-                if (j == n - 1) {
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(vfix);
-                }
-                // keys that some rows see and some do not
-                const int from = max(seen_by_all - j * kPrRows, 0);
-                uint32_t found = 0;
-                if (from < end) {
-#pragma unroll 8
-                    for (int e = from * 8 * Sh::blks + lane; e < end * 8 * Sh::blks; e += 32) {
-                        const int row = e / (8 * Sh::blks), c = e - row * (8 * Sh::blks);
-                        uint32_t x[4];
-                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(v + (c >> 3) * BLK + row * 128 + ((c & 7) << 4)));
+            tc_fence_after();
+            if (!s_again[w & 1]) {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                __nv_bfloat16* out = (__nv_bfloat16*)p.a.out + ((it.row + r) * p.a.n_q + x.h) * p.a.head_dim;
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) found |= ((x[u] & 0x7FFF7FFFu) + 0x00800080u) & 0x80008000u;   // exponent of ones
+                for (int i = 0; i < HD; i += 32) {
+                    uint32_t o[32];
+                    if (steps > 0) tmem_ld32_wait(tOt + i, o);
+                    if (r < it.rows && t < p.tiles)
+#pragma unroll
+                        for (int u = 0; u < 32; u += 8) {
+                            if (i + u >= p.a.head_dim) continue;
+                            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                            if (sum != 0.f) {
+                                auto y = [&](int e) { return __uint_as_float(o[u + e]) * inv; };
+                                v = make_uint4(bf16_pair(y(0), y(1)), bf16_pair(y(2), y(3)), bf16_pair(y(4), y(5)), bf16_pair(y(6), y(7)));
+                            }
+                            *reinterpret_cast<uint4*>(out + i + u) = v;
+                        }
+                }
+                tc_fence_before();       // O has been read before the next rows' P is handed on
+            } else {
+                prompt_rows<__nv_bfloat16>(p.a, it, x.h, warp, 8);
+            }
+            done_work(w);
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 8) {
+            // ---- work dealt out; copies: Q, then K and V tile by tile ----
+            const int boxes = kPrRows / p.box;
+            int s = 0, item = blockIdx.x;
+            uint32_t ph = 0, cq = 0;
+            for (int w = 0;; ++w) {
+                PromptWork x;
+                x.it = w == 0 ? first : prompt_item(p.a, p.tiles * kPrRows, item / p.a.n_q);
+                x.h = item % p.a.n_q;
+                const PromptItem& it = x.it;
+                ok = wait_phase(wempty + 8 * (w & 1), ((w >> 1) & 1) ^ 1u, abort_flag);
+                if (!ok) break;
+                if (lane == 0) {
+                    s_again[w & 1] = 0;
+                    s_work[w & 1] = x;
+                    mbar_arrive(wfull + 8 * (w & 1));
+                }
+                if (it.rows == 0) break;
+                const int n = max(steps_of(it, 0), steps_of(it, 1)), hkv = x.h / p.a.group;
+                if (n > 0) {
+                    ok = wait_phase(qempty, (cq & 1) ^ 1u, abort_flag);
+                    if (!ok) break;
+                    ++cq;
+                    if (lane == 0) {
+                        mbar_expect_tx(qfull, (uint32_t)(p.tiles * TILE));
+                        for (int t = 0; t < p.tiles; ++t)
+                            for (int c = 0; c < Sh::blks; ++c) tma_load_3d(sq + t * TILE + c * BLK, &qmap, c * 64, x.h, (int)it.row + t * kPrRows, qfull);
                     }
                 }
-                if (found) s_again = 1;
+                // rows of a tile's boxes, a lane each (-1: behind the last key, -2: no page), looked up a tile ahead
+                auto rows_at = [&](int j) {
+                    const int pos = j * kPrRows + lane * p.box;
+                    if (j >= n || lane >= boxes || pos >= it.keys) return -1;
+                    const int row = (int)kv_row(p.a.kv, it.b, it.row0, pos);
+                    return row < 0 ? -2 : row;
+                };
+                int ahead = rows_at(0);
+                for (int j = 0; j < n && ok; ++j) {
+                    const int y = ahead;
+                    ahead = rows_at(j + 1);
+                    if (y == -2) s_again[w & 1] = 1;
+                    __syncwarp();
+                    const unsigned there = __ballot_sync(0xffffffffu, y >= 0);
+                    const uint32_t bytes = (uint32_t)(__popc(there) * p.box * 128 * Sh::blks);
+                    for (int kv = 0; kv < 2; ++kv) {
+                        if (ok) ok = wait_phase(empty + 8 * s, ph ^ 1u, abort_flag);
+                        if (!ok) break;
+                        const uint32_t bar = full + 8 * s, dst = ring + s * TILE;
+                        if (lane == 0) {
+                            if (bytes) mbar_expect_tx(bar, bytes);
+                            else mbar_arrive(bar);
+                        }
+                        for (int g = 0; g < boxes; ++g) {
+                            const int row = __shfl_sync(0xffffffffu, y, g);
+                            if (lane == 0 && row >= 0)
+                                for (int c = 0; c < Sh::blks; ++c) tma_load_3d(dst + c * BLK + g * p.box * 128, kv ? &vmap : &kmap, c * 64, hkv, row, bar);
+                        }
+                        if (++s == NST) { s = 0; ph ^= 1u; }
+                    }
+                }
+                if (!ok) break;
+                // The next one, now that this one's last copies are on their way: asked for earlier, the long ones' blocks would take it from
+                // those that are done sooner (2048 rows, 32 heads: 48 -> 61 us).
+                if (lane == 0) item = atomicAdd(p.counters, 1) + (int)gridDim.x;
+                item = __shfl_sync(0xffffffffu, item, 0);
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty + 8 * s);
-            if (++s == NST) { s = 0; ph ^= 1u; }
+            if (!ok) {      // copies under way are waited for (again with a limit)
+                volatile int none = 0;
+                if (cq) wait_phase(qfull, (cq - 1) & 1, const_cast<volatile int*>(&none));
+                for (int i = 0; i < NST; ++i) wait_phase(full + 8 * i, ph ^ (i >= s ? 1u : 0u), const_cast<volatile int*>(&none));
+            }
+        } else if (warp == 9) {
+            // ---- MMAs ----
+            constexpr uint32_t id_s = idesc_bf16(128), id_o = idesc_bf16(HD) | (1u << 16);     // (bit 16: B with N innermost)
+            const bool leader = elect_one();
+            int s = 0;                                            // the ring's next stage
+            uint32_t ph = 0, c[2] = {0, 0}, cq = 0;               // steps so far; blocks of rows with any
+            auto wait = [&](uint32_t bar, uint32_t parity) {
+                if (ok) ok = wait_phase(bar, parity, abort_flag);
+                tc_fence_after();
+            };
+            auto step = [&]() { if (++s == NST) { s = 0; ph ^= 1u; } };
+            // low words of descriptors (in 16 bytes) and their high word; V's: the blocks of 64 columns apart
+            const uint32_t hi = (uint32_t)(smem_desc_sw128(0) >> 32), lead = (uint32_t)smem_desc_sw128(0), lead_v = (uint32_t)smem_desc_rows(0, BLK);
+            auto product_s = [&](int t, int stage) {
+                if (!ok) return;
+                const uint32_t a = lead + ((sq + t * TILE) >> 4), b = lead + ((ring + stage * TILE) >> 4);
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) {
+                    const uint32_t o = (k >> 2) * (BLK >> 4) + (k & 3) * 2;
+                    if (leader) umma_ss(tS[t], a + o, b + o, hi, id_s, k > 0);
+                }
+                umma_commit_if(sfull + 8 * t, leader);
+            };
+            PromptWork x;
+            for (int w = 0; ok && next_work(w, &x); ++w) {
+                const int nt[2] = {steps_of(x.it, 0), steps_of(x.it, 1)}, n = max(nt[0], nt[1]);
+                if (n > 0) {
+                    wait(qfull, cq & 1);
+                    wait(full + 8 * s, ph);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        if (nt[t] > 0) product_s(t, s);
+                    if (ok) umma_commit_if(empty + 8 * s, leader);
+                    if (ok && n == 1) umma_commit_if(qempty, leader);
+                    step();
+                }
+                for (int j = 0; j < n && ok; ++j) {
+                    const int vs = s;
+                    const uint32_t vph = ph;
+                    step();
+                    const int ks = s;
+                    const uint32_t kph = ph;
+                    if (j + 1 < n) step();
+                    wait(full + 8 * vs, vph);
+                    if (j == n - 1) wait(vfix + 8 * (w & 1), (w >> 1) & 1);
+                    bool have_k = false;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (j < nt[t]) {
+                            const uint32_t b = lead_v + ((ring + vs * TILE) >> 4);
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {       // P's first half is there sooner
+                                wait((half ? pfull : phalf) + 8 * t, (c[t] + j) & 1);
+                                if (!ok) break;
+#pragma unroll
+                                for (int k = half * 4; k < half * 4 + 4; ++k) if (leader) umma_ts(tO[t], tS[t] + k * 8, b + k * (2048 >> 4), hi, id_o, j > 0 || k > 0);
+                            }
+                            if (ok) umma_commit_if(odone + 8 * t, leader);
+                        }
+                        if (t == 1 && ok) umma_commit_if(empty + 8 * vs, leader);
+                        if (j + 1 < nt[t]) {
+                            if (!have_k) wait(full + 8 * ks, kph);
+                            have_k = true;
+                            product_s(t, ks);
+                        }
+                        if (t == 1 && j + 1 < n && ok) umma_commit_if(empty + 8 * ks, leader);
+                    }
+                    if (ok && j + 2 == n) umma_commit_if(qempty, leader);      // Q's last product is issued
+                }
+                c[0] += nt[0];
+                c[1] += nt[1];
+                cq += n > 0;
+                done_work(w);
+            }
+            if (!ok) {      // products under way are waited for (with a limit) before the memory they use is given up
+                volatile int none = 0;
+                umma_commit_if(over, leader);
+                wait_phase(over, 0, const_cast<volatile int*>(&none));
+            }
+        } else if (warp == 10) {
+            // ---- V's edges ----
+            int s = 0;
+            uint32_t ph = 0;
+            PromptWork x;
+            for (int w = 0; ok && next_work(w, &x); ++w) {
+                const PromptItem& it = x.it;
+                const int n = max(steps_of(it, 0), steps_of(it, 1)), seen_by_all = it.sees(0, p.a.causal);
+                for (int i = 0; i < 2 * n; ++i) {
+                    ok = wait_phase(full + 8 * s, ph, abort_flag);
+                    if (!ok) break;
+                    if (i & 1) {
+                        const int j = i >> 1;
+                        const uint32_t v = ring + s * TILE;
+                        const int end = min(it.keys - j * kPrRows, kPrRows);
+                        for (int e = end * 8 * Sh::blks + lane; e < kPrRows * 8 * Sh::blks; e += 32) {     // behind the last key: zeros
+                            const int row = e / (8 * Sh::blks), c = e - row * (8 * Sh::blks);
+                            sts128(v + (c >> 3) * BLK + row * 128 + ((c & 7) << 4), 0u, 0u, 0u, 0u);
+                        }
+                        if (j == n - 1) {
+                            fence_async_smem();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(vfix + 8 * (w & 1));
+                        }
+                        // keys that some rows see and some do not
+                        const int from = max(seen_by_all - j * kPrRows, 0);
+                        uint32_t found = 0;
+                        if (from < end) {
+#pragma unroll 8
+                            for (int e = from * 8 * Sh::blks + lane; e < end * 8 * Sh::blks; e += 32) {
+                                const int row = e / (8 * Sh::blks), c = e - row * (8 * Sh::blks);
+                                uint32_t y[4];
+                                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3]) : "r"(v + (c >> 3) * BLK + row * 128 + ((c & 7) << 4)));
+#pragma unroll
+                                for (int u = 0; u < 4; ++u) found |= ((y[u] & 0x7FFF7FFFu) + 0x00800080u) & 0x80008000u;   // exponent of ones
+                            }
+                        }
+                        if (found) s_again[w & 1] = 1;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(empty + 8 * s);
+                    if (++s == NST) { s = 0; ph ^= 1u; }
+                }
+                if (!ok) break;
+                if (lane == 0) {
+                    if (n == 0) mbar_arrive(vfix + 8 * (w & 1));
+                    mbar_arrive(fixed + 8 * (w & 1));
+                }
+                done_work(w);
+            }
         }
-        if (lane == 0) mbar_arrive(fixed);
-    }
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 9) tmem_dealloc(tmem, 512);
-    if (tid == 0 && s_abort) atomicExch(p.status, 2);
+    if (tid == 0) {
+        if (s_abort) atomicExch(p.status, 2);
+        if (atomicAdd(p.counters + 1, 1) == (int)gridDim.x - 1) p.counters[0] = p.counters[1] = 0;      // the last block: for the next launch
+    }
 }
 
 int32_t prompt_configure() {
@@ -404,7 +480,8 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a) {
     if (rc == RSTQ_OK) rc = rows_tensor_map(&kmap, a.k, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc == RSTQ_OK) rc = rows_tensor_map(&vmap, a.v, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc != RSTQ_OK) return rc;
-    const dim3 grid((unsigned)blocks), block(kPrThreads);
+    p.counters = ds.counters + ds.counters_len - 2;
+    const dim3 grid((unsigned)std::min<int64_t>(blocks, ds.sm_count)), block(kPrThreads);
     RSTQ_CUDA(a.head_dim <= 64 ? launch_pdl(prompt_kernel<64>, grid, block, (size_t)PromptShape<64>::smem, ds, p, qmap, kmap, vmap)
                                : launch_pdl(prompt_kernel<128>, grid, block, (size_t)PromptShape<128>::smem, ds, p, qmap, kmap, vmap));
     return RSTQ_OK;
