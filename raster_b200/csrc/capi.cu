@@ -627,7 +627,7 @@ int32_t rstq_init(const int32_t* devices, rstq_ctx** ctxp, int32_t ndev) {
             if ((r = dx_configure()) != RSTQ_OK) return r;
             if ((r = attn_configure(ds)) != RSTQ_OK) return r;
             if ((r = decode_configure(ds)) != RSTQ_OK) return r;
-            if ((r = prompt_configure()) != RSTQ_OK) return r;
+            if ((r = prompt_configure(ds)) != RSTQ_OK) return r;
             if ((r = prompt_f32_configure()) != RSTQ_OK) return r;
             if ((r = pages_configure(ds)) != RSTQ_OK) return r;
             RSTQ_CUDA(cudaStreamSynchronize(ds.stream));
@@ -671,6 +671,7 @@ int32_t rstq_shutdown(rstq_ctx* ctx) {
         if (ds.attn_scratch) cudaFree(ds.attn_scratch);
         if (ds.attn_slots) cudaFree(ds.attn_slots);
         if (ds.page_scratch) cudaFree(ds.page_scratch);
+        if (ds.prompt_slots) cudaFree(ds.prompt_slots);
         if (ds.kq_scratch) cudaFree(ds.kq_scratch);
         if (ds.f_image) cudaFree(ds.f_image);
         if (ds.bind_stage) cudaFree(ds.bind_stage);

@@ -289,9 +289,10 @@ static int32_t run_prompt(rstq_ctx* ctx, rstq_buf* q, const PromptArgs& a) {
     if (a.rows == 0) return RSTQ_OK;
     DeviceState& ds = ctx->devs[q->dev];
     int32_t rc;
+    int launches = 1;
     if (a.head_dim > 128 || a.scale <= 0.f || a.kv_rows == 0) rc = launch_attention_rows(ds, a);
-    else rc = a.dtype == RSTQ_BF16 ? launch_prompt(ds, a) : launch_prompt_f32(ds, a);
-    if (rc == RSTQ_OK) ctx->launches++;
+    else rc = a.dtype == RSTQ_BF16 ? launch_prompt(ds, a, &launches) : launch_prompt_f32(ds, a);
+    if (rc == RSTQ_OK) ctx->launches += launches;
     return rc;
 }
 

@@ -50,6 +50,12 @@ __device__ __forceinline__ void tmem_ld16_wait(uint32_t taddr, uint32_t (&r)[16]
         : "r"(taddr)
         : "memory");
 }
+// 32 bytes at once: a thread per row writes whole sectors, half the requests of 16 bytes each
+__device__ __forceinline__ void st_sector(void* p, const uint32_t (&v)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                 "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
 // pairs of f32 in one instruction
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
@@ -134,63 +140,165 @@ __device__ __forceinline__ float ex2f(float x) {
     return y;
 }
 
-// What a block works on: rows [first, first + n) of the packed q, sequence b.
+// What a block works on: rows [row, row + rows) of the packed q, of sequence b, against tiles j0 .. j1 - 1 of its keys.
 struct PromptItem {
-    int b, rows;           // sequence, rows of it in this block (0: nothing to do)
+    int b, rows;           // sequence, rows of it in this block (0: nothing left to do)
     int64_t row;           // the first one, packed
     int behind;            // rows from the first one to the sequence's end
     int keys, row0;        // keys of the sequence; packed: the first one's row
+    int j0, j1;            // tiles of keys
+    int part, parts;       // which of how many parts of the block's keys
     // keys that row r of the block sees
     __device__ __forceinline__ int sees(int r, int causal) const {
         return causal ? min(max(keys - behind + 1 + r, 0), keys) : keys;
     }
 };
-// Block `item` of those of all sequences, `per` rows each; counted from the end, so that the blocks with most keys of a
-// long sequence come first.  A warp's lanes work together and get the same answer.
-static __device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, int per, int item) {
+constexpr int kMaxParts = 16;
+// One lane's sequence cut into blocks of `per` rows, and the tiles of `tile` keys that block k sees.
+struct PromptSequence {
+    int n, keys, row0, first, blocks;
+    __device__ __forceinline__ void load(const PromptArgs& a, int b, int per) {
+        n = keys = row0 = first = 0;
+        if (b < a.seqs) {
+            int64_t f, l, r;
+            packed_range(a.cu_q, b, a.rows, &f, &l);
+            keys = (int)kv_length(a.kv, b, &r);
+            n = (int)(l - f);
+            first = (int)f;
+            row0 = (int)r;
+        }
+        blocks = (n + per - 1) / per;
+    }
+    __device__ __forceinline__ int tiles(int k, int per, int causal, int tile) const {
+        const int last = min(n, (k + 1) * per) - 1, s = causal ? min(max(keys - n + 1 + last, 0), keys) : keys;
+        return (s + tile - 1) / tile;
+    }
+};
+// parts of a block that sees w tiles, where a part should have about `share`
+__device__ __forceinline__ int prompt_parts(int w, int share) { return w > share + (share >> 2) ? min((w + share - 1) / share, kMaxParts) : 1; }
+__device__ __forceinline__ int prompt_count(const PromptSequence& q, int per, int causal, int tile, int share) {
+    if (q.blocks == 0 || prompt_parts(q.tiles(q.blocks - 1, per, causal, tile), share) == 1) return q.blocks;     // (the last sees most)
+    int c = 0;
+    for (int k = 0; k < q.blocks; ++k) c += prompt_parts(q.tiles(k, per, causal, tile), share);
+    return c;
+}
+// How many tiles of keys a part should have, half of what each of `sms` blocks of threads would have to do: no fewer than eight, and all
+// (no parts) where that makes more than `most` items of work in all.  heads: items per block of rows.
+static __device__ __forceinline__ int prompt_share(const PromptArgs& a, int per, int tile, int heads, int sms, int most, int* total) {
     const int lane = threadIdx.x & 31;
-    auto rows_of = [&](int b, int64_t* first) {
-        int64_t last;
-        *first = 0;
-        if (b >= a.seqs) return 0;
-        packed_range(a.cu_q, b, a.rows, first, &last);
-        return (int)(last - *first);
-    };
+    float all = 0.f;       // (sums of integers below 2^24, or large enough not to matter)
+    for (int b0 = 0; b0 < a.seqs; b0 += 32) {
+        PromptSequence q;
+        q.load(a, b0 + lane, per);
+        float w = q.blocks ? 0.5f * (float)q.blocks * (float)(q.tiles(0, per, a.causal, tile) + q.tiles(q.blocks - 1, per, a.causal, tile)) : 0.f;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) w += __shfl_xor_sync(0xffffffffu, w, d);
+        all += w;
+    }
+    const int share = (int)fminf(fmaxf(ceilf(all * (float)heads / (float)(2 * sms)), 8.f), 1e9f);
+    int items = 0;
+    for (int b0 = 0; b0 < a.seqs && items <= most; b0 += 32) {
+        PromptSequence q;
+        q.load(a, b0 + lane, per);
+        if (__any_sync(0xffffffffu, q.blocks > most)) items = most + 1;
+        else items += __reduce_add_sync(0xffffffffu, prompt_count(q, per, a.causal, tile, share));
+    }
+    *total = (int64_t)items * heads <= most ? items * heads : 0;
+    return *total ? share : 1 << 30;
+}
+// Block `item` of those of all sequences, `per` rows each, all of its keys; counted from the end, so that the blocks with most keys of a
+// long sequence come first.  A warp's lanes work together and get the same answer.
+static __device__ __forceinline__ PromptItem prompt_block(const PromptArgs& a, int per, int tile, int item) {
+    const int lane = threadIdx.x & 31;
     PromptItem it;
     it.rows = 0;
-    int base = 0;
     for (int b0 = (a.seqs - 1) & ~31; b0 >= 0; b0 -= 32) {
-        int64_t first;
-        const int b = b0 + 31 - lane, n = rows_of(b, &first), m = (n + per - 1) / per;
+        PromptSequence q;
+        q.load(a, b0 + 31 - lane, per);
+        int x = q.blocks;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += y;
+        }
+        const unsigned behind = __ballot_sync(0xffffffffu, x > item);
+        if (!behind) {
+            item -= __shfl_sync(0xffffffffu, x, 31);
+            if (item < 0) return it;                       // (sequences that overlap beyond counting)
+            continue;
+        }
+        const int src = __ffs((int)behind) - 1, k = __shfl_sync(0xffffffffu, x, src) - 1 - item;      // of the sequence, from its start
+        q.n = __shfl_sync(0xffffffffu, q.n, src);
+        if (k < 0 || (int64_t)k * per >= q.n) return it;
+        it.keys = q.keys = __shfl_sync(0xffffffffu, q.keys, src);
+        it.b = b0 + 31 - src;
+        it.row = __shfl_sync(0xffffffffu, q.first, src) + (int64_t)k * per;
+        it.behind = q.n - k * per;
+        it.rows = it.behind < per ? it.behind : per;
+        it.row0 = __shfl_sync(0xffffffffu, q.row0, src);
+        it.parts = 1;
+        it.part = it.j0 = 0;
+        it.j1 = q.tiles(k, per, a.causal, tile);
+        return it;
+    }
+    return it;
+}
+// Item `item` of those of all sequences: blocks of `per` rows, from the end of each sequence (those that see most keys first), in
+// parts.  A warp's lanes work together and get the same answer.
+static __device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, int per, int tile, int share, int item) {
+    const int lane = threadIdx.x & 31;
+    PromptItem it;
+    it.rows = 0;
+    for (int b0 = (a.seqs - 1) & ~31; b0 >= 0; b0 -= 32) {
+        PromptSequence q;
+        q.load(a, b0 + 31 - lane, per);
+        const int m = prompt_count(q, per, a.causal, tile, share);
         int x = m;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, x, d);
             if (lane >= d) x += y;
         }
-        const unsigned behind = __ballot_sync(0xffffffffu, base + x > item);
-        if (behind) {
-            const int src = __ffs((int)behind) - 1;
-            const int end = __shfl_sync(0xffffffffu, base + x, src), rows = __shfl_sync(0xffffffffu, n, src);
-            const int block = end - 1 - item;              // (of the sequence, from its start)
-            if (block < 0 || (int64_t)block * per >= rows) return it;     // (sequences that overlap beyond counting)
-            it.b = b0 + 31 - src;
-            it.row = __shfl_sync(0xffffffffu, (int)first, src) + (int64_t)block * per;
-            it.behind = rows - block * per;
-            it.rows = it.behind < per ? it.behind : per;
-            int64_t row0;
-            it.keys = (int)kv_length(a.kv, it.b, &row0);
-            it.row0 = (int)row0;
-            return it;
+        const unsigned behind = __ballot_sync(0xffffffffu, x > item);
+        if (!behind) {
+            item -= __shfl_sync(0xffffffffu, x, 31);
+            if (item < 0) return it;                       // (sequences that overlap beyond counting)
+            continue;
         }
-        base += __shfl_sync(0xffffffffu, x, 31);
+        const int src = __ffs((int)behind) - 1;
+        int left = item - __shfl_sync(0xffffffffu, x - m, src);      // items of this sequence before it
+        const int blocks = __shfl_sync(0xffffffffu, q.blocks, src);
+        const bool whole = __shfl_sync(0xffffffffu, m, src) == blocks;
+        q.n = __shfl_sync(0xffffffffu, q.n, src);
+        q.keys = __shfl_sync(0xffffffffu, q.keys, src);
+        int k = blocks - 1 - (whole ? left : 0), parts = 1;
+        if (!whole)
+            for (;; --k) {
+                if (k < 0) return it;
+                parts = prompt_parts(q.tiles(k, per, a.causal, tile), share);
+                if (left < parts) break;
+                left -= parts;
+            }
+        if (left < 0 || k < 0 || (int64_t)k * per >= q.n) return it;
+        const int w = q.tiles(k, per, a.causal, tile);
+        it.b = b0 + 31 - src;
+        it.row = __shfl_sync(0xffffffffu, q.first, src) + (int64_t)k * per;
+        it.behind = q.n - k * per;
+        it.rows = it.behind < per ? it.behind : per;
+        it.keys = q.keys;
+        it.row0 = __shfl_sync(0xffffffffu, q.row0, src);
+        it.parts = parts;
+        it.part = whole ? 0 : left;
+        it.j0 = (int)((int64_t)w * it.part / parts);
+        it.j1 = (int)((int64_t)w * (it.part + 1) / parts);
+        return it;
     }
     return it;
 }
 
 // The block's rows one by one, from the positions they see alone.
 template <typename T>
-__device__ __forceinline__ void prompt_rows(const PromptArgs& a, const PromptItem& it, int h, int warp, int warps) {
+__device__ __forceinline__ void prompt_rows(const PromptArgs& a, const PromptItem& it, int h, int warp, int warps) {     // (of one head)
     const int lane = threadIdx.x & 31;
     using S = RowState<T>;      // (head_dim <= 128: one piece of a lane)
     bool bad = false;

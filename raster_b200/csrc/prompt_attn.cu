@@ -32,21 +32,36 @@ struct PromptShape {
     static constexpr int smem = 1024 + (2 + stages) * tile;
 };
 
+constexpr int kPromptSlots = 512;      // items of a call whose blocks' keys are cut into parts
+
 struct PromptParams {
     PromptArgs a;
     int tiles;                       // query tiles of a block: 1 or 2
+    int pack;                        // log2 of the heads of a group that share a tile: its rows are (row of q, head), the head innermost
+    int heads;                       // items per block of rows: n_kv, or n_q without packing
+    int bound;                       // items there are at most
+    int sms, most;                   // blocks of threads; items of work up to which a block's keys may be cut into parts (0: never)
     int box;                         // rows of a box of keys
+    int sectors;                     // the rows of out begin on 32-byte boundaries, and so do their pieces of 16 columns
     float scale2;
     int* status;
+    float* part;                     // a slot per item: what a part of a block has found
+    PromptItem* list;                // ... and what the item was; their number, 0 where no block's keys are cut
+    int* listed;
     int* counters;                   // [0] items dealt out beyond the first of every block, [1] blocks that are done: zero between launches
 };
 // what a warp has to know of a block of rows
 struct PromptWork {
     PromptItem it;
-    int h;                           // query head
+    int h;                           // query head, or the packed ones' KV head
+    int item;
 };
-
+// a slot, in floats: 256 rows' sums, four columns at a time; their references; their sums of weights; whether they have to be taken again
 template <int HD>
+__host__ __device__ constexpr int prompt_slot() { return 2 * kPrRows * (HD + 2) + 32; }
+
+// PARTS: a block's keys may be cut into parts.
+template <int HD, bool PARTS>
 __global__ void __launch_bounds__(kPrThreads, 1)
 prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
               const __grid_constant__ CUtensorMap vmap) {
@@ -103,17 +118,27 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     asm volatile("griddepcontrol.wait;" ::: "memory");
     PromptItem first;                // the block's first work, looked up while tensor memory is on its way
     first.rows = 0;
-    if (warp == 8) first = prompt_item(p.a, p.tiles * kPrRows, blockIdx.x / p.a.n_q);
+    const int per = (p.tiles * kPrRows) >> p.pack;       // rows of q of a block
+    int share = 1 << 30;
+    if (warp == 8) {
+        if (PARTS) {
+            int items;
+            share = prompt_share(p.a, per, kPrRows, p.heads, p.sms, p.most, &items);
+            if (blockIdx.x == 0 && lane == 0) *p.listed = items;
+        }
+        first = PARTS ? prompt_item(p.a, per, kPrRows, share, blockIdx.x / p.heads) : prompt_block(p.a, per, kPrRows, blockIdx.x / p.heads);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = (uint32_t)uniform((int)s_tmem);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // (not before this block has its tensor memory)
     const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + HD};
-    // steps of the two tiles of a block of rows: tiles of keys that some row of theirs sees
+    // keys that row r of a block's tiles sees, and the steps of a tile: tiles of keys, of the item's, that some row of it sees
+    auto sees = [&](const PromptItem& it, int r) { return it.sees(r >> p.pack, p.a.causal); };
     auto steps_of = [&](const PromptItem& it, int t) {
-        const int last = min(it.rows, (t + 1) * kPrRows) - 1;
-        return uniform(t < p.tiles && last >= t * kPrRows ? (it.sees(last, p.a.causal) + kPrRows - 1) / kPrRows : 0);
+        const int last = min(it.rows << p.pack, (t + 1) * kPrRows) - 1;
+        return uniform(t < p.tiles && last >= t * kPrRows ? max(min(it.j1, (sees(it, last) + kPrRows - 1) / kPrRows) - it.j0, 0) : 0);
     };
     bool ok = true;
     // The next block of rows, of which `w` is the number; false: there is none.
@@ -141,7 +166,8 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         for (int w = 0; ok && next_work(w, &x); ++w) {
             const PromptItem& it = x.it;
             const int steps = steps_of(it, t);
-            const int mine = it.sees(r, p.a.causal), least = it.sees(t * kPrRows, p.a.causal);      // keys of this row, of the tile's first
+            // keys of this row, of the tile's first, from the item's first on
+            const int mine = sees(it, r) - it.j0 * kPrRows, least = sees(it, t * kPrRows) - it.j0 * kPrRows;
             float m = -INFINITY, m2 = 0.f, sum = 0.f;      // running maximum of S; scale2 times it (0: nothing seen yet)
             for (int j = 0; j < steps; ++j) {
                 ok = wait_phase(sfull + 8 * t, (c + j) & 1, abort_flag);
@@ -219,29 +245,49 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             if (steps > 0 && ok) ok = wait_phase(odone + 8 * t, (c - 1) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
-            if (!s_again[w & 1]) {
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                __nv_bfloat16* out = (__nv_bfloat16*)p.a.out + ((it.row + r) * p.a.n_q + x.h) * p.a.head_dim;
+            const bool has_row = t < p.tiles && (r >> p.pack) < it.rows;
+            const int head = p.pack ? (x.h << p.pack) + (r & ((1 << p.pack) - 1)) : x.h;
+            __nv_bfloat16* out = (__nv_bfloat16*)p.a.out + ((it.row + (r >> p.pack)) * p.a.n_q + head) * p.a.head_dim;
+            const bool again = s_again[w & 1] != 0;
+            // (a part of a block's keys: what it has found goes to its slot, for prompt_join_kernel)
+            const bool whole = !PARTS || it.parts == 1;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            float* slot = p.part + (whole ? 0 : (int64_t)x.item * prompt_slot<HD>());
+            if (!whole || !again)
 #pragma unroll
                 for (int i = 0; i < HD; i += 32) {
                     uint32_t o[32];
                     if (steps > 0) tmem_ld32_wait(tOt + i, o);
-                    if (r < it.rows && t < p.tiles)
+                    if (has_row && whole) {
 #pragma unroll
-                        for (int u = 0; u < 32; u += 8) {
+                        for (int u = 0; u < 32; u += 16) {
                             if (i + u >= p.a.head_dim) continue;
-                            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                            if (sum != 0.f) {
-                                auto y = [&](int e) { return __uint_as_float(o[u + e]) * inv; };
-                                v = make_uint4(bf16_pair(y(0), y(1)), bf16_pair(y(2), y(3)), bf16_pair(y(4), y(5)), bf16_pair(y(6), y(7)));
+                            uint32_t v[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                v[e] = sum == 0.f ? 0u : bf16_pair(__uint_as_float(o[u + 2 * e]) * inv, __uint_as_float(o[u + 2 * e + 1]) * inv);
+                            if (p.sectors) st_sector(out + i + u, v);
+                            else {
+                                *reinterpret_cast<uint4*>(out + i + u) = make_uint4(v[0], v[1], v[2], v[3]);
+                                if (i + u + 8 < p.a.head_dim) *reinterpret_cast<uint4*>(out + i + u + 8) = make_uint4(v[4], v[5], v[6], v[7]);
                             }
-                            *reinterpret_cast<uint4*>(out + i + u) = v;
                         }
+                    } else if (PARTS && has_row && steps > 0) {
+#pragma unroll
+                        for (int u = 0; u < 32; u += 4)
+                            *reinterpret_cast<uint4*>(slot + ((i + u) / 4 * 2 * kPrRows + r) * 4) = make_uint4(o[u], o[u + 1], o[u + 2], o[u + 3]);
+                    }
                 }
-                tc_fence_before();       // O has been read before the next rows' P is handed on
-            } else {
-                prompt_rows<__nv_bfloat16>(p.a, it, x.h, warp, 8);
+            if (PARTS && !whole) {
+                if (has_row) {
+                    slot[2 * kPrRows * HD + r] = m2;
+                    slot[2 * kPrRows * (HD + 1) + r] = sum;      // (0: the columns say nothing)
+                }
+                if (tid == 0) slot[2 * kPrRows * (HD + 2)] = again ? 1.f : 0.f;
             }
+            tc_fence_before();       // O has been read before the next rows' P is handed on
+            if (again && whole)
+                for (int i = 0; i < 1 << p.pack; ++i) prompt_rows<__nv_bfloat16>(p.a, it, p.pack ? (x.h << p.pack) + i : x.h, warp, 8);
             done_work(w);
         }
     } else {
@@ -251,10 +297,20 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             const int boxes = kPrRows / p.box;
             int s = 0, item = blockIdx.x;
             uint32_t ph = 0, cq = 0;
+            // The next item, asked for when the last copies of this one are on their way.  (Asked for with the item itself, the long ones'
+            // blocks would take it from those that are done sooner: 2048 rows, 32 heads 48 -> 61 us.)
+            auto claim = [&]() {
+                first.rows = 0;
+                if (p.bound <= (int)gridDim.x) return;
+                if (lane == 0) item = atomicAdd(p.counters, 1) + (int)gridDim.x;
+                item = __shfl_sync(0xffffffffu, item, 0);
+                first = PARTS ? prompt_item(p.a, per, kPrRows, share, item / p.heads) : prompt_block(p.a, per, kPrRows, item / p.heads);
+            };
             for (int w = 0;; ++w) {
                 PromptWork x;
-                x.it = w == 0 ? first : prompt_item(p.a, p.tiles * kPrRows, item / p.a.n_q);
-                x.h = item % p.a.n_q;
+                x.it = first;
+                x.h = item % p.heads;
+                x.item = item;
                 const PromptItem& it = x.it;
                 ok = wait_phase(wempty + 8 * (w & 1), ((w >> 1) & 1) ^ 1u, abort_flag);
                 if (!ok) break;
@@ -264,7 +320,16 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     mbar_arrive(wfull + 8 * (w & 1));
                 }
                 if (it.rows == 0) break;
-                const int n = max(steps_of(it, 0), steps_of(it, 1)), hkv = x.h / p.a.group;
+                if (PARTS && lane == 0 && share < 1 << 30) p.list[item] = it;
+                const int n = max(steps_of(it, 0), steps_of(it, 1)), hkv = p.pack ? x.h : x.h / p.a.group;
+                // rows of a tile's boxes, a lane each (-1: behind the last key, -2: no page), looked up a tile ahead
+                auto rows_at = [&](int j) {
+                    const int pos = (it.j0 + j) * kPrRows + lane * p.box;
+                    if (j >= n || lane >= boxes || pos >= it.keys) return -1;
+                    const int row = (int)kv_row(p.a.kv, it.b, it.row0, pos);
+                    return row < 0 ? -2 : row;
+                };
+                int ahead = rows_at(0);
                 if (n > 0) {
                     ok = wait_phase(qempty, (cq & 1) ^ 1u, abort_flag);
                     if (!ok) break;
@@ -272,17 +337,10 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     if (lane == 0) {
                         mbar_expect_tx(qfull, (uint32_t)(p.tiles * TILE));
                         for (int t = 0; t < p.tiles; ++t)
-                            for (int c = 0; c < Sh::blks; ++c) tma_load_3d(sq + t * TILE + c * BLK, &qmap, c * 64, x.h, (int)it.row + t * kPrRows, qfull);
+                            for (int c = 0; c < Sh::blks; ++c)
+                                tma_load_4d(sq + t * TILE + c * BLK, &qmap, c * 64, p.pack ? 0 : x.h % p.a.group, hkv, (int)it.row + ((t * kPrRows) >> p.pack), qfull);
                     }
                 }
-                // rows of a tile's boxes, a lane each (-1: behind the last key, -2: no page), looked up a tile ahead
-                auto rows_at = [&](int j) {
-                    const int pos = j * kPrRows + lane * p.box;
-                    if (j >= n || lane >= boxes || pos >= it.keys) return -1;
-                    const int row = (int)kv_row(p.a.kv, it.b, it.row0, pos);
-                    return row < 0 ? -2 : row;
-                };
-                int ahead = rows_at(0);
                 for (int j = 0; j < n && ok; ++j) {
                     const int y = ahead;
                     ahead = rows_at(j + 1);
@@ -307,10 +365,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     }
                 }
                 if (!ok) break;
-                // The next one, now that this one's last copies are on their way: asked for earlier, the long ones' blocks would take it from
-                // those that are done sooner (2048 rows, 32 heads: 48 -> 61 us).
-                if (lane == 0) item = atomicAdd(p.counters, 1) + (int)gridDim.x;
-                item = __shfl_sync(0xffffffffu, item, 0);
+                claim();
             }
             if (!ok) {      // copies under way are waited for (again with a limit)
                 volatile int none = 0;
@@ -403,14 +458,14 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             PromptWork x;
             for (int w = 0; ok && next_work(w, &x); ++w) {
                 const PromptItem& it = x.it;
-                const int n = max(steps_of(it, 0), steps_of(it, 1)), seen_by_all = it.sees(0, p.a.causal);
+                const int n = max(steps_of(it, 0), steps_of(it, 1)), base = it.j0 * kPrRows, seen_by_all = sees(it, 0) - base;
                 for (int i = 0; i < 2 * n; ++i) {
                     ok = wait_phase(full + 8 * s, ph, abort_flag);
                     if (!ok) break;
                     if (i & 1) {
                         const int j = i >> 1;
                         const uint32_t v = ring + s * TILE;
-                        const int end = min(it.keys - j * kPrRows, kPrRows);
+                        const int end = min(it.keys - base - j * kPrRows, kPrRows);
                         for (int e = end * 8 * Sh::blks + lane; e < kPrRows * 8 * Sh::blks; e += 32) {     // behind the last key: zeros
                             const int row = e / (8 * Sh::blks), c = e - row * (8 * Sh::blks);
                             sts128(v + (c >> 3) * BLK + row * 128 + ((c & 7) << 4), 0u, 0u, 0u, 0u);
@@ -457,33 +512,138 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     }
 }
 
-int32_t prompt_configure() {
+// The parts of a block joined, in their order: blocks of threads per item, a slice of the columns each, of which those of the first part do it.
+constexpr int kJoinSlices = 8;
+template <int HD>
+__global__ void __launch_bounds__(256, 3)
+prompt_join_kernel(const PromptParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr int SLOT = prompt_slot<HD>(), R = 2 * kPrRows;
+    const int tid = threadIdx.x, all = *p.listed * kJoinSlices;
+    for (int job = blockIdx.x; job < all; job += gridDim.x) {
+    const int item = job / kJoinSlices, slice = job - item * kJoinSlices;
+    const PromptItem it = p.list[item];
+    if (it.parts == 1 || it.part != 0) continue;
+    const int h = item % p.heads;
+    const float* from = p.part + (int64_t)item * SLOT;
+    const int64_t step = (int64_t)p.heads * SLOT;
+    bool again = false;
+#pragma unroll
+    for (int q = 0; q < kMaxParts; ++q) again |= __ldcg(from + min(q, it.parts - 1) * step + R * (HD + 2)) != 0.f;
+    if (again) {
+        if (slice == 0)
+            for (int i = 0; i < 1 << p.pack; ++i) prompt_rows<__nv_bfloat16>(p.a, it, p.pack ? (h << p.pack) + i : h, tid >> 5, 8);
+        continue;
+    }
+    // eight columns of a row per thread: rows side by side
+    const int rows = it.rows << p.pack, pieces = p.a.head_dim / 8, mine = (pieces - slice + kJoinSlices - 1) / kJoinSlices;
+    for (int e = tid; e < rows * mine; e += 256) {
+        const int x = e / rows, r = e - x * rows, i = x * kJoinSlices + slice;
+        float top = -INFINITY, total = 0.f, a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int q0 = 0; q0 < it.parts; q0 += 4) {
+            // (a load of a part that is not there is one of the last part's, with a weight of 0: loads behind a branch would wait for one another)
+            float4 u[4], v[4];
+            float f[4], s[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float* x = from + min(q0 + q, it.parts - 1) * step;
+                s[q] = __ldcg(x + R * (HD + 1) + r);
+                f[q] = __ldcg(x + R * HD + r);
+                u[q] = __ldcg(reinterpret_cast<const float4*>(x) + 2 * i * R + r);
+                v[q] = __ldcg(reinterpret_cast<const float4*>(x) + (2 * i + 1) * R + r);
+            }
+            float next = top;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                f[q] = q0 + q < it.parts && s[q] != 0.f ? f[q] : -INFINITY;
+                next = fmaxf(next, f[q]);
+            }
+            const float ref = next == -INFINITY ? 0.f : next, g = ex2f(top - ref);
+            top = next;
+            total *= g;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) a[x] *= g;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float w = ex2f(f[q] - ref);
+                if (w == 0.f) continue;
+                total = fmaf(w, s[q], total);
+                a[0] = fmaf(w, u[q].x, a[0]); a[1] = fmaf(w, u[q].y, a[1]); a[2] = fmaf(w, u[q].z, a[2]); a[3] = fmaf(w, u[q].w, a[3]);
+                a[4] = fmaf(w, v[q].x, a[4]); a[5] = fmaf(w, v[q].y, a[5]); a[6] = fmaf(w, v[q].z, a[6]); a[7] = fmaf(w, v[q].w, a[7]);
+            }
+        }
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        const int head = p.pack ? (h << p.pack) + (r & ((1 << p.pack) - 1)) : h;
+        *reinterpret_cast<uint4*>((__nv_bfloat16*)p.a.out + ((it.row + (r >> p.pack)) * p.a.n_q + head) * p.a.head_dim + 8 * i) =
+            make_uint4(bf16_pair(a[0] * inv, a[1] * inv), bf16_pair(a[2] * inv, a[3] * inv), bf16_pair(a[4] * inv, a[5] * inv), bf16_pair(a[6] * inv, a[7] * inv));
+    }
+    }
+}
+
+int32_t prompt_configure(DeviceState& ds) {
     constexpr auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    RSTQ_CUDA(cudaFuncSetAttribute(prompt_kernel<64>, attr, PromptShape<64>::smem));
-    RSTQ_CUDA(cudaFuncSetAttribute(prompt_kernel<128>, attr, PromptShape<128>::smem));
+    RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<64, false>), attr, PromptShape<64>::smem));
+    RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<64, true>), attr, PromptShape<64>::smem));
+    RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<128, false>), attr, PromptShape<128>::smem));
+    RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<128, true>), attr, PromptShape<128>::smem));
+    RSTQ_CUDA(cudaMalloc((void**)&ds.prompt_slots, (size_t)kPromptSlots * (prompt_slot<128>() * 4 + sizeof(PromptItem)) + 64));
     return RSTQ_OK;
 }
 
-int32_t launch_prompt(DeviceState& ds, const PromptArgs& a) {
+// q as [rows][n_kv][group][head_dim], in boxes of 128 rows of a tile
+static int32_t prompt_q_map(CUtensorMap* m, const PromptArgs& a, int heads) {
+    const EncodeTiledFn enc = encode_tiled_fn();
+    RSTQ_REQUIRE(enc, RSTQ_E_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[4] = {(cuuint64_t)a.head_dim, (cuuint64_t)a.group, (cuuint64_t)a.n_kv, (cuuint64_t)a.rows};
+    const cuuint64_t strides[3] = {(cuuint64_t)a.head_dim * 2, (cuuint64_t)a.group * a.head_dim * 2, (cuuint64_t)a.ldq * 2};
+    const cuuint32_t box[4] = {64u, (cuuint32_t)heads, 1u, (cuuint32_t)(kPrRows / heads)}, ones[4] = {1u, 1u, 1u, 1u};
+    const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(a.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    RSTQ_REQUIRE(r == CUDA_SUCCESS, RSTQ_E_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return RSTQ_OK;
+}
+
+int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     PromptParams p;
     p.a = a;
     p.scale2 = a.scale * 1.4426950408889634f;
     p.status = ds.status;
+    p.sectors = ((uintptr_t)a.out & 31) == 0 && a.head_dim % 16 == 0;
     p.box = a.kv.table ? std::min(1 << a.kv.shift, kPrRows) : kPrRows;
+    // Heads of a group that is a power of two share a tile: its K and V are read once for all of them, and few rows fill it.
+    p.pack = a.group > 1 && a.group <= kPrRows && (a.group & (a.group - 1)) == 0 ? log2_of(a.group) : 0;
+    p.heads = p.pack ? a.n_kv : a.n_q;
     // Two query tiles per block keep the tensor core busy; with fewer blocks than SMs one each does the rows sooner.
-    p.tiles = a.rows * a.n_q <= 2 * kPrRows * (int64_t)ds.sm_count / 2 ? 1 : 2;
-    const int per = p.tiles * kPrRows;
-    const int64_t blocks = (a.rows / per + std::min<int64_t>(a.seqs, a.rows)) * a.n_q;     // no sequence has more than this of them
+    p.tiles = a.rows * a.n_q <= kPrRows * (int64_t)ds.sm_count ? 1 : 2;
+    const int per = (p.tiles * kPrRows) >> p.pack;
+    const int64_t blocks = (a.rows / per + std::min<int64_t>(a.seqs, a.rows)) * p.heads;     // no sequence has more than this of them
     RSTQ_REQUIRE(blocks < (1ll << 31), RSTQ_E_LIMIT, "%lld thread blocks", (long long)blocks);
+    // Few blocks of rows that may see many keys (a cache, or more keys than rows): these are cut into parts, which a second launch joins.
+    const int64_t keys = a.kv.table ? (int64_t)a.kv.width << a.kv.shift : a.kv_rows > a.rows ? a.kv_rows : 0;
+    const bool parts = keys > 8 * kPrRows && (a.rows / per + std::min<int64_t>(a.seqs, a.rows)) * p.heads <= ds.sm_count;
+    p.sms = ds.sm_count;
+    p.bound = parts ? 1 << 30 : (int)blocks;
+    p.most = kPromptSlots;
+    p.part = ds.prompt_slots;
+    p.list = (PromptItem*)(ds.prompt_slots + (int64_t)kPromptSlots * prompt_slot<128>());
+    p.listed = (int*)(p.list + kPromptSlots);
     CUtensorMap qmap, kmap, vmap;
-    int32_t rc = rows_tensor_map(&qmap, a.q, a.dtype, a.rows, a.ldq, a.n_q, a.head_dim, kPrRows);
+    int32_t rc = prompt_q_map(&qmap, a, 1 << p.pack);
     if (rc == RSTQ_OK) rc = rows_tensor_map(&kmap, a.k, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc == RSTQ_OK) rc = rows_tensor_map(&vmap, a.v, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc != RSTQ_OK) return rc;
     p.counters = ds.counters + ds.counters_len - 2;
-    const dim3 grid((unsigned)std::min<int64_t>(blocks, ds.sm_count)), block(kPrThreads);
-    RSTQ_CUDA(a.head_dim <= 64 ? launch_pdl(prompt_kernel<64>, grid, block, (size_t)PromptShape<64>::smem, ds, p, qmap, kmap, vmap)
-                               : launch_pdl(prompt_kernel<128>, grid, block, (size_t)PromptShape<128>::smem, ds, p, qmap, kmap, vmap));
+    const dim3 grid((unsigned)(parts ? ds.sm_count : std::min<int64_t>(blocks, ds.sm_count)));
+    auto go = [&](auto kernel, int smem) { return launch_pdl(kernel, grid, dim3(kPrThreads), (size_t)smem, ds, p, qmap, kmap, vmap); };
+    if (a.head_dim <= 64) RSTQ_CUDA(parts ? go(prompt_kernel<64, true>, PromptShape<64>::smem) : go(prompt_kernel<64, false>, PromptShape<64>::smem));
+    else RSTQ_CUDA(parts ? go(prompt_kernel<128, true>, PromptShape<128>::smem) : go(prompt_kernel<128, false>, PromptShape<128>::smem));
+    if (parts) {
+        const dim3 join((unsigned)(12 * ds.sm_count));
+        RSTQ_CUDA(a.head_dim <= 64 ? launch_pdl(prompt_join_kernel<64>, join, dim3(256), 0, ds, p) : launch_pdl(prompt_join_kernel<128>, join, dim3(256), 0, ds, p));
+        *launches = 2;
+    } else *launches = 1;
     return RSTQ_OK;
 }
 

@@ -85,7 +85,7 @@ prompt_f32_kernel(const PromptParamsF p) {
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp == 0) {
-        const PromptItem it = prompt_item(p.a, kPfRows, blockIdx.x / p.a.n_q);
+        const PromptItem it = prompt_block(p.a, kPfRows, kPfKeys, blockIdx.x / p.a.n_q);
         if (lane == 0) s_item = it;
     }
     tc_fence_before();

@@ -406,6 +406,68 @@ def test_prompt(ctx, dtype, n_q, n_kv, d, page, lens, new, causal):
             close(got, want, tol, f"sequence {b}")
 
 
+# few rows behind many keys, which are cut into parts; groups of heads that share a tile and that do not; many blocks of rows
+LONG = [
+    ("bf16", 8, 2, 128, 32, [2500, 1100, 7, 1500], [2, 40, 7, 1], True),
+    ("bf16", 6, 2, 64, 16, [3000, 0, 1030], [5, 0, 30], True),
+    ("bf16", 2, 2, 128, 0, [1500, 200], [3, 200], True),
+    ("bf16", 16, 1, 96, 64, [1200], [20], False),
+    ("bf16", 4, 1, 128, 256, [4000], [1], True),
+    ("bf16", 8, 1, 64, 0, [700, 600, 650], None, True),
+    ("f32", 4, 1, 128, 32, [1500, 70], [3, 70], True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,n_q,n_kv,d,page,lens,new,causal", LONG)
+def test_prompt_of_few_rows_behind_many_keys(ctx, dtype, n_q, n_kv, d, page, lens, new, causal):
+    seqs, scale = prompt_case(ctx, dtype, n_q, n_kv, d, page, lens, new, causal)
+    for b, (got, q, k, v) in enumerate(seqs):
+        pick = sorted({0, len(q) // 2, len(q) - 1}) if len(q) > 64 else range(len(q))       # (the model is slow)
+        for r in pick:
+            if len(q):
+                m = len(k) - len(q) + r + 1 if causal else len(k)
+                want, tol = pm.attention(q[r:r + 1], k[:m], v[:m], scale, False, dtype)
+                close(got[r:r + 1], want, tol, f"sequence {b} row {r}")
+
+
+@pytest.mark.gpu
+def test_prompt_parts_with_values_that_are_not_numbers(ctx):
+    """Keys cut into parts: an infinity above the diagonal, in the last part, is not seen; one below it is."""
+    n_q, n_kv, d, page, n, rows = 4, 1, 64, 32, 2600, 3
+    p = Pool(ctx, [n], n_kv, d, page, "bf16")
+    v = p.bv.download().reshape(p.v.shape)
+    at = lambda pos: (p.table[0, pos // page], pos % page)  # noqa: E731
+    v[at(n - 1)][0, 5] = pm.encode(np.array([np.inf], np.float32), "bf16")[0]        # the last row's own
+    v[at(100)][0, 6] = pm.encode(np.array([-np.inf], np.float32), "bf16")[0]         # everybody's
+    p.bv.upload(v)
+    q = pm.decode(pm.encode(normal(4, rows, n_q, d), "bf16"), "bf16")
+    bq, bo, cu = ctx.array_to_buffer(pm.encode(q, "bf16")), ctx.make_buffer(rows * n_q * d, np.uint16), ctx.array_to_buffer(np.array([0, rows], np.int32))
+    ctx.paged_prompt_attention(bq, p.bk, p.bv, bo, p.bt, cu, p.bl, rows, 1, n_q, n_q, n_kv, d, page, p.n_pages, p.width, 0.125, True, L.BF16)
+    ctx.sync()
+    got = pm.decode(bo.download(), "bf16").reshape(rows, n_q, d)
+    assert np.isneginf(got[:, :, 6]).all() and np.isposinf(got[2, :, 5]).all() and np.isfinite(got[:2, :, 5]).all()
+    for r in range(rows):
+        m = n - rows + r + 1
+        want, tol = pm.attention(q[r:r + 1], p.keys[0][:m], p.values[0][:m], 0.125, False, "bf16")
+        keep = [i for i in range(d) if i not in (5, 6)]
+        close(got[r:r + 1][..., keep], want[..., keep], tol[..., keep], f"row {r}")
+    tab = p.table.copy()
+    tab[0, 40] = p.n_pages
+    p.bt.upload(tab)                                                                   # a page that is none: its positions are left out
+    ctx.paged_prompt_attention(bq, p.bk, p.bv, bo, p.bt, cu, p.bl, rows, 1, n_q, n_q, n_kv, d, page, p.n_pages, p.width, 0.125, True, L.BF16)
+    with pytest.raises(L.RstqError) as e:
+        ctx.sync()
+    assert e.value.code == L.E_RANGE
+    got = pm.decode(bo.download(), "bf16").reshape(rows, n_q, d)
+    k, w = (np.delete(x[0], np.s_[40 * page:41 * page], 0) for x in (p.keys, p.values))
+    want, tol = pm.attention(q[:1], k[:len(k) - 2], w[:len(k) - 2], 0.125, False, "bf16")
+    close(got[:1][..., keep], want[..., keep], tol[..., keep])
+    for b in (bq, bo, cu):
+        b.free()
+    p.free()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,d", [("bf16", 128), ("bf16", 64), ("bf16", 256), ("f32", 64)])
 def test_prompt_rows_do_not_see_what_comes_after_them(ctx, dtype, d):
