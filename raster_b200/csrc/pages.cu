@@ -204,15 +204,18 @@ pages_extend_kernel(const PageState s, const int32_t* __restrict__ list, const i
         const int i = i0 + threadIdx.x, k = i < n ? need(i) : 0;
         int total;
         const int at = base + block_scan(k, &total, s_warp);
-        if (i < n) {
-            const int b = list[i], len = page_len(s, b), have = pages_of(s, len);
-            for (int j = 0; j < k; ++j) {
-                const int pg = w.map[at + j];
-                s.table[(int64_t)b * s.width + have + j] = pg;
+        const int b = i < n ? list[i] : 0, len = i < n ? page_len(s, b) : 0;
+        const int64_t e0 = (int64_t)b * s.width + pages_of(s, len);
+        for (uint32_t left = __ballot_sync(0xffffffffu, k > 0); left; left &= left - 1) {     // a warp writes its sequences' entries in turn
+            const int l = __ffs((int)left) - 1, kl = __shfl_sync(0xffffffffu, k, l), al = __shfl_sync(0xffffffffu, at, l);
+            const int64_t el = __shfl_sync(0xffffffffu, e0, l);
+            for (int j = threadIdx.x & 31; j < kl; j += 32) {
+                const int pg = w.map[al + j];
+                s.table[el + j] = pg;
                 s.refs[pg] = 1;
             }
-            s.lens[b] = len + counts[i];
         }
+        if (i < n) s.lens[b] = len + counts[i];
         base += total;
     }
     say(s, kInfoOk, s.n_pages - free + (int)want, 0, 0);
@@ -230,14 +233,16 @@ pages_fork_kernel(const PageState s, const int32_t* __restrict__ src, const int3
     int bad = first_bad(n, &s_min, [&](int i) {
         return (uint32_t)src[i] >= (uint32_t)s.seqs || (uint32_t)dst[i] >= (uint32_t)s.seqs || take_bit(s_bits, dst[i]) || s.lens[dst[i]] != 0;
     });
-    if (bad == n)     // a source is nobody's destination, and its pages are pages
-        bad = first_bad(n, &s_min, [&](int i) {
-            if (has_bit(s_bits, src[i])) return true;
+    if (bad == n) {   // a source is nobody's destination, and its pages are pages (a warp per source: its loads are under way together)
+        for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {
             const int np = pages_of(s, page_len(s, src[i]));
-            for (int j = 0; j < np; ++j)
-                if ((uint32_t)s.table[(int64_t)src[i] * s.width + j] >= (uint32_t)s.n_pages) return true;
-            return false;
-        });
+            bool wrong = has_bit(s_bits, src[i]);
+            for (int j = threadIdx.x & 31; j < np; j += 32) wrong |= (uint32_t)s.table[(int64_t)src[i] * s.width + j] >= (uint32_t)s.n_pages;
+            if (wrong) atomicMin(&s_min, i);
+        }
+        __syncthreads();
+        bad = s_min;
+    }
     if (bad < n) {
         const int used = s.n_pages - list_free(s, 0, nullptr, s_warp);
         say(s, kInfoList, used, 0, bad);
@@ -284,7 +289,7 @@ pages_fork_kernel(const PageState s, const int32_t* __restrict__ src, const int3
 
 // Pages held that lie behind the first `live` ones go, in order, to the free pages among those.
 __global__ void __launch_bounds__(kPlanThreads)
-pages_compact_kernel(const PageState s, const PageScratch w) {
+pages_compact_kernel(const PageState s, int32_t* refs_out, const PageScratch w) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     __shared__ int s_warp[32];
@@ -307,13 +312,26 @@ pages_compact_kernel(const PageState s, const PageScratch w) {
         for (int j = 0; j < 4; ++j) {
             const int pg = 4 * i + j;
             if (pg < live && v[j] <= 0) w.to[ah++] = pg;
-            if (pg >= live && pg < s.n_pages && v[j] > 0) w.from[am++] = pg;
+            if (pg >= live && pg < s.n_pages) {
+                if (v[j] > 0) w.from[am++] = pg;
+                else w.map[pg] = pg;
+            }
         }
         holes += th;
         moves += tm;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < moves; i += kPlanThreads) w.map[w.from[i]] = w.to[i];
+    // the counts as they become: a page that moves takes its count along (a count of a free page stays as it is)
+    if (refs_out != s.refs) {
+        for (int i = threadIdx.x; i < s.n_pages; i += kPlanThreads) refs_out[i] = s.refs[i];
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < moves; i += kPlanThreads) {
+        const int a = w.from[i], b = w.to[i];
+        refs_out[b] = s.refs[a];
+        refs_out[a] = 0;
+        w.map[a] = b;
+    }
     if (threadIdx.x == 0) {
         w.header[0] = moves;
         w.header[1] = live;
@@ -329,7 +347,7 @@ struct CopyParams {
     int layers, n_pages, parts;     // pieces of 4 KB of a page
     // compact: the tables as they become
     PageState s;
-    int32_t *table_out, *refs_out;
+    int32_t* table_out;
     const int* map;
     const int* live;
 };
@@ -369,30 +387,9 @@ pages_copy_kernel(const CopyParams p) {
         const int64_t t0 = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
         for (int64_t e = t0; e < (int64_t)p.s.seqs * p.s.width; e += step) {
             const int b = (int)(e / p.s.width), j = (int)(e - (int64_t)b * p.s.width), pg = p.s.table[e];
-            const bool moved = j < pages_of(p.s, page_len(p.s, b)) && pg >= live && pg < p.s.n_pages && p.s.refs[pg] > 0;
-            p.table_out[e] = moved ? p.map[pg] : pg;
+            const bool held = j < pages_of(p.s, page_len(p.s, b)) && pg >= live && pg < p.s.n_pages;
+            p.table_out[e] = held ? p.map[pg] : pg;
         }
-        // (each moved pair is written by the thread of its old page alone, other pages by their own)
-    }
-}
-
-// refs as they become, after every table entry has been looked up with the old ones
-__global__ void __launch_bounds__(256)
-pages_refs_kernel(const CopyParams p) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int pairs = *p.pairs;
-    const int t0 = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
-    const int live = *p.live;
-    if (p.refs_out != p.s.refs)
-        for (int i = t0; i < p.s.n_pages; i += step) {
-            const int r = p.s.refs[i];
-            if (i < live ? r > 0 : true) p.refs_out[i] = i < live ? r : (r > 0 ? 0 : r);
-        }
-    for (int i = t0; i < pairs; i += step) {
-        const int a = p.from[i], b = p.to[i], r = p.s.refs[a];
-        p.refs_out[b] = r;
-        p.refs_out[a] = 0;
     }
 }
 
@@ -540,7 +537,7 @@ int32_t rstq_pages_compact(rstq_ctx* ctx, rstq_buf* kcache, rstq_buf* vcache, rs
     if (rc != RSTQ_OK) return rc;
     DeviceState& ds = ctx->devs[table->dev];
     const PageScratch w = page_scratch(ds);
-    RSTQ_CUDA(launch_pdl(pages_compact_kernel, dim3(1), dim3(kPlanThreads), 0, ds, s, w));
+    RSTQ_CUDA(launch_pdl(pages_compact_kernel, dim3(1), dim3(kPlanThreads), 0, ds, s, (int32_t*)refs_out->ptr, w));
     p.from = w.from;
     p.to = w.to;
     p.pairs = w.header;
@@ -548,10 +545,8 @@ int32_t rstq_pages_compact(rstq_ctx* ctx, rstq_buf* kcache, rstq_buf* vcache, rs
     p.map = w.map;
     p.s = s;
     p.table_out = (int32_t*)table_out->ptr;
-    p.refs_out = (int32_t*)refs_out->ptr;
     RSTQ_CUDA(launch_pdl(pages_copy_kernel, copy_grid(ds, p, n_pages / 2, seqs * max_pages), dim3(256), 0, ds, p));
-    RSTQ_CUDA(launch_pdl(pages_refs_kernel, dim3((unsigned)std::min<int64_t>((n_pages + 255) / 256, ds.sm_count)), dim3(256), 0, ds, p));
-    ctx->launches += 3;
+    ctx->launches += 2;
     return RSTQ_OK;
 }
 
