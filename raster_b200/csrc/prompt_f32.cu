@@ -211,6 +211,7 @@ prompt_f32_kernel(const PromptParamsF p) {
         constexpr int LPR = HD / 4, RPI = 32 / LPR, NI = 16 / RPI;      // lanes of a row; rows of a load; loads of a warp's 16 rows
         const int w = warp - 4, d = (lane % LPR) * 4, sub = lane / LPR;
         const bool in = d < p.a.head_dim;
+        const int din = in ? d : 0;
         uint32_t top = 0;             // largest magnitude seen, as bits
         auto write = [&](uint32_t base, int plane, int blk, int row, float4 x) {
             top = max(max(top, max(__float_as_uint(x.x) & 0x7FFFFFFFu, __float_as_uint(x.y) & 0x7FFFFFFFu)),
@@ -239,45 +240,69 @@ prompt_f32_kernel(const PromptParamsF p) {
             }
             return (int)row;
         };
+        // Loads are made of some row in any case, so that all of them are under way at once; `live` says which rows count (a bit each).
         auto fetch = [&](float4 (&x)[NI], const void* base, int rows) {
+            const float* from = (const float*)base + (int64_t)hkv * p.a.head_dim + din;
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                const int row = __shfl_sync(0xffffffffu, rows, i * RPI + sub);
-                x[i] = in && row >= 0 ? *reinterpret_cast<const float4*>((const float*)base + (int64_t)row * p.a.kv.ld + (int64_t)hkv * p.a.head_dim + d)
-                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+                const int row = max(__shfl_sync(0xffffffffu, rows, i * RPI + sub), 0);
+                x[i] = *reinterpret_cast<const float4*>(from + (int64_t)row * p.a.kv.ld);
             }
         };
+        auto rows_in = [&](int rows) {
+            const uint32_t there = __ballot_sync(0xffffffffu, rows >= 0) >> sub;
+            return in ? there : 0u;
+        };
+        auto only = [&](bool there, float4 x) {
+            return make_float4(there ? x.x : 0.f, there ? x.y : 0.f, there ? x.z : 0.f, there ? x.w : 0.f);
+        };
+        // K is written a tile ahead of V: with two places for S before the V of the tile before it, as the next S comes before that P V,
+        // with one behind it.
         float4 k[NI], v[NI];
-        int rows = places(0);
+        int r1 = places(0), r2 = places(1);
+        uint32_t klive = 0, vlive = 0;
         if (ok) {
-            fetch(k, p.a.k, rows);
+            fetch(k, p.a.k, r1);
+            klive = rows_in(r1);
             for (int half = 0; half < 2; ++half) {
                 float4 x[NI];
 #pragma unroll
                 for (int i = 0; i < NI; ++i) {
                     const int row = w * 32 + half * 16 + i * RPI + sub;
-                    x[i] = in && row < it.rows ? *reinterpret_cast<const float4*>((const float*)p.a.q + (it.row + row) * p.a.ldq + (int64_t)h * p.a.head_dim + d)
-                                               : make_float4(0.f, 0.f, 0.f, 0.f);
+                    x[i] = *reinterpret_cast<const float4*>((const float*)p.a.q + (it.row + min(row, it.rows - 1)) * p.a.ldq + (int64_t)h * p.a.head_dim + din);
                 }
 #pragma unroll
-                for (int i = 0; i < NI; ++i) write(sq, Sh::qplane, Sh::qblk, w * 32 + half * 16 + i * RPI + sub, x[i]);
+                for (int i = 0; i < NI; ++i) {
+                    const int row = w * 32 + half * 16 + i * RPI + sub;
+                    write(sq, Sh::qplane, Sh::qblk, row, only(in && row < it.rows, x[i]));
+                }
             }
             hand(qfull);
         }
-        for (int j = 0; j < n && ok; ++j) {
-            fetch(v, p.a.v, rows);
-            rows = places(j + 1);
+        // (the fence of a hand-over waits for loads under way: both fetches come behind both)
+        auto write_k = [&](int j) {
+            if (!ok || j >= n) return;
             ok = wait_phase(kfree, (j & 1) ^ 1u, abort_flag);
-            if (!ok) break;
+            if (!ok) return;
 #pragma unroll
-            for (int i = 0; i < NI; ++i) write(sk, Sh::kplane, Sh::kblk, w * 16 + i * RPI + sub, k[i]);
+            for (int i = 0; i < NI; ++i) write(sk, Sh::kplane, Sh::kblk, w * 16 + i * RPI + sub, only(klive >> (i * RPI) & 1, k[i]));
             hand(kfull);
-            if (j + 1 < n) fetch(k, p.a.k, rows);
-            ok = wait_phase(vfree, (j & 1) ^ 1u, abort_flag);
+        };
+        write_k(0);
+        for (int j = 0; j < n && ok; ++j) {
+            fetch(v, p.a.v, r1);
+            vlive = rows_in(r1);
+            if (j + 1 < n) fetch(k, p.a.k, r2);
+            klive = rows_in(r2);
+            r1 = r2;
+            r2 = places(j + 2);
+            if (NB == 2) write_k(j + 1);
+            if (ok) ok = wait_phase(vfree, (j & 1) ^ 1u, abort_flag);
             if (!ok) break;
 #pragma unroll
-            for (int i = 0; i < NI; ++i) write(sv, Sh::kplane, Sh::kblk, w * 16 + i * RPI + sub, v[i]);
+            for (int i = 0; i < NI; ++i) write(sv, Sh::kplane, Sh::kblk, w * 16 + i * RPI + sub, only(vlive >> (i * RPI) & 1, v[i]));
             hand(vfull);
+            if (NB == 1) write_k(j + 1);
         }
     } else {
         // ---- MMAs ----
