@@ -458,11 +458,13 @@ RSTQ_API int32_t rstq_gqa_decode_attention(rstq_ctx* ctx, rstq_buf* q, rstq_buf*
  * of the pool counts as positions that nobody sees (and are not written), as does a row whose position has no page; the
  * next rstq_sync then returns RSTQ_E_RANGE.
  * ldq, ldk, ldkv: elements from a row of q (of k and v) to the next, 0 = packed; rows start on 16-byte boundaries, so a
- * slice of a fused q|k|v matmul's result can be handed over.  Scratch is the context's: calls that could overlap on the GPU
+ * slice of a fused q|k|v matmul's result can be handed over.  No array that a call writes may lie over another one of its
+ * arrays (RSTQ_E_INVALID), but where said below.  Scratch is the context's: calls that could overlap on the GPU
  * (graphs replayed on two streams) need a context each.
  *
  *   rstq_paged_rope_append       q turned to qout [rows][n_q][head_dim]; k turned and v written to their pages, in `dtype`
- *                                (q, k, v are in_dtype).  cu may be NULL: rows == seqs, one per sequence.  qout may be q.
+ *                                (q, k, v are in_dtype).  cu may be NULL: rows == seqs, one per sequence.  qout may be q
+ *                                where q is packed and of the type stored.
  *   rstq_paged_decode_attention  one row of q per sequence against all its positions; a sequence of none gives zeros.
  *   rstq_prompt_attention        rows of packed sequences (cu_q) against packed keys and values [kv_rows][n_kv][head_dim]
  *                                (cu_k; may be cu_q); causal = 1: a row sees the keys up to its own place, the last row

@@ -107,6 +107,26 @@ __device__ __forceinline__ int row_sequence(const int32_t* cu, int seqs, int64_t
 inline bool paged_buf(const rstq_buf* b, const rstq_ctx* ctx, int64_t bytes) {
     return b && b->magic == kBufMagic && b->ctx == ctx && b->bytes >= bytes && ((uintptr_t)b->ptr & 15) == 0;
 }
+// Bytes of an array that a call reads or writes.
+struct Span {
+    const void* p;
+    int64_t n;
+};
+inline bool apart(const Span& a, const Span& b) {
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    return a.n <= 0 || b.n <= 0 || x + (uintptr_t)a.n <= y || y + (uintptr_t)b.n <= x;
+}
+// No array that is written lies over another one, read or written.
+template <size_t W, size_t R>
+inline bool apart(const Span (&written)[W], const Span (&read)[R]) {
+    for (size_t i = 0; i < W; ++i) {
+        for (size_t j = i + 1; j < W; ++j)
+            if (!apart(written[i], written[j])) return false;
+        for (size_t j = 0; j < R; ++j)
+            if (!apart(written[i], read[j])) return false;
+    }
+    return true;
+}
 inline int elem_bytes(int32_t dtype) { return dtype == RSTQ_BF16 ? 2 : 4; }
 inline int log2_of(int64_t v) {
     int s = 0;

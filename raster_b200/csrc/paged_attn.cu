@@ -191,7 +191,7 @@ int32_t rstq_paged_rope_append(rstq_ctx* ctx, rstq_buf* q, rstq_buf* k, rstq_buf
     if (rc != RSTQ_OK) return rc;
     RSTQ_REQUIRE(rows >= 0 && rows <= kMaxRows && (cu || rows == seqs), RSTQ_E_SHAPE, "rows = %lld of %lld sequences (without cu, one each)",
                  (long long)rows, (long long)seqs);
-    RSTQ_REQUIRE(theta > 0.0, RSTQ_E_SHAPE, "theta = %g", theta);
+    RSTQ_REQUIRE(theta > 0.0 && isfinite(theta), RSTQ_E_SHAPE, "theta = %g", theta);
     if (rows == 0) return RSTQ_OK;
     const int64_t qrow = n_q * head_dim, kvrow = n_kv * head_dim, ib = elem_bytes(in_dtype), ob = elem_bytes(dtype);
     if (!ldq) ldq = qrow;
@@ -206,6 +206,14 @@ int32_t rstq_paged_rope_append(rstq_ctx* ctx, rstq_buf* q, rstq_buf* k, rstq_buf
                      paged_buf(lens, ctx, seqs * 4) && (!cu || paged_buf(cu, ctx, (seqs + 1) * 4)),
                  RSTQ_E_INVALID, "invalid, unaligned or too small buffer");
     RSTQ_REQUIRE(same_device(q, k, v, qout, kcache, vcache, table, lens, cu), RSTQ_E_DEVICE, "buffers live on different devices");
+    // in place: every pair of elements is read and written by one thread, if it stays where it is
+    const bool in_place = qout->ptr == q->ptr && in_dtype == dtype && (ldq == qrow || rows == 1);
+    const Span written[] = {{qout->ptr, rows * qrow * ob}, {kcache->ptr, pool}, {vcache->ptr, pool}};
+    const Span read[] = {{k->ptr, ((rows - 1) * ldkv + kvrow) * ib}, {v->ptr, ((rows - 1) * ldkv + kvrow) * ib}, {table->ptr, seqs * max_pages * 4},
+                         {lens->ptr, seqs * 4}, {cu ? cu->ptr : nullptr, cu ? (seqs + 1) * 4 : 0}};
+    const Span qs = {q->ptr, ((rows - 1) * ldq + qrow) * ib};
+    RSTQ_REQUIRE(apart(written, read) && (in_place || apart(written[0], qs)) && apart(written[1], qs) && apart(written[2], qs), RSTQ_E_INVALID,
+                 "an array that is written lies over another one");
     DeviceState& ds = ctx->devs[q->dev];
     if ((rc = use_dev(ctx, q->dev)) != RSTQ_OK) return rc;
     AppendParams p;
@@ -246,7 +254,7 @@ static int32_t attention_args(rstq_ctx* ctx, rstq_buf* q, rstq_buf* k, rstq_buf*
     RSTQ_REQUIRE(rows >= 0 && rows <= kMaxRows && kv_rows >= 0 && kv_rows <= kMaxRows, RSTQ_E_SHAPE, "rows = %lld, kv_rows = %lld",
                  (long long)rows, (long long)kv_rows);
     RSTQ_REQUIRE(causal == 0 || causal == 1, RSTQ_E_INVALID, "causal = %d (0 or 1)", (int)causal);
-    RSTQ_REQUIRE(isfinite(scale), RSTQ_E_SHAPE, "scale = %g", scale);
+    RSTQ_REQUIRE(fabs(scale) <= 1e30, RSTQ_E_SHAPE, "scale = %g", scale);       // (log2(e) times it is a float too)
     const int64_t qrow = n_q * head_dim, kvrow = n_kv * head_dim, eb = elem_bytes(dtype);
     if (!ldq) ldq = qrow;
     if (!ldk) ldk = kvrow;
@@ -259,6 +267,10 @@ static int32_t attention_args(rstq_ctx* ctx, rstq_buf* q, rstq_buf* k, rstq_buf*
                      paged_buf(lens_or_cu, ctx, (packed ? seqs + 1 : seqs) * 4),
                  RSTQ_E_INVALID, "invalid, unaligned or too small buffer");
     RSTQ_REQUIRE(same_device(q, k, v, out, table, cu_q, lens_or_cu), RSTQ_E_DEVICE, "buffers live on different devices");
+    const Span written[] = {{out->ptr, rows * qrow * eb}};
+    const Span read[] = {{q->ptr, qb}, {k->ptr, kb}, {v->ptr, kb}, {packed ? nullptr : table->ptr, packed ? 0 : seqs * max_pages * 4},
+                         {cu_q ? cu_q->ptr : nullptr, cu_q ? (seqs + 1) * 4 : 0}, {lens_or_cu->ptr, (packed ? seqs + 1 : seqs) * 4}};
+    RSTQ_REQUIRE(apart(written, read), RSTQ_E_INVALID, "out lies over an array that is read");
     DeviceState& ds = ctx->devs[q->dev];
     const int32_t* w = (const int32_t*)lens_or_cu->ptr;
     a->q = q->ptr; a->k = k->ptr; a->v = v->ptr; a->out = out->ptr;

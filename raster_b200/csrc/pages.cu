@@ -432,25 +432,33 @@ static int32_t page_state(rstq_ctx* ctx, rstq_buf* table, rstq_buf* lens, rstq_b
                      paged_buf(info, ctx, 16),
                  RSTQ_E_INVALID, "invalid, unaligned or too small buffer");
     RSTQ_REQUIRE(same_device(table, lens, refs, info), RSTQ_E_DEVICE, "buffers live on different devices");
+    const Span written[] = {{table->ptr, seqs * max_pages * 4}, {lens->ptr, seqs * 4}, {refs->ptr, n_pages * 4}, {info->ptr, 16}}, none[] = {{nullptr, 0}};
+    RSTQ_REQUIRE(apart(written, none), RSTQ_E_INVALID, "table, lens, refs and info lie over one another");
     *s = PageState{(int32_t*)table->ptr, (int32_t*)lens->ptr, (int32_t*)refs->ptr, (int32_t*)info->ptr,
                    (int)seqs, (int)n_pages, (int)max_pages, (int)page};
     return use_dev(ctx, table->dev);
 }
-static int32_t list_args(rstq_ctx* ctx, const rstq_buf* on, rstq_buf* a, rstq_buf* b, int64_t n) {
+static int32_t list_args(rstq_ctx* ctx, const PageState& s, const rstq_buf* on, rstq_buf* a, rstq_buf* b, int64_t n) {
     RSTQ_REQUIRE(n >= 0 && n <= kListMax, RSTQ_E_LIMIT, "a list of %lld (0 .. %d)", (long long)n, kListMax);
     RSTQ_REQUIRE(paged_buf(a, ctx, n * 4) && (!b || paged_buf(b, ctx, n * 4)), RSTQ_E_INVALID, "invalid, unaligned or too small list");
     RSTQ_REQUIRE(same_device(on, a, b), RSTQ_E_DEVICE, "buffers live on different devices");
+    const Span written[] = {{s.table, (int64_t)s.seqs * s.width * 4}, {s.lens, s.seqs * 4ll}, {s.refs, s.n_pages * 4ll}, {s.info, 16}};
+    const Span read[] = {{a->ptr, n * 4}, {b ? b->ptr : nullptr, b ? n * 4 : 0}};
+    RSTQ_REQUIRE(apart(written, read), RSTQ_E_INVALID, "a list lies over what the call writes");
     return RSTQ_OK;
 }
-// the pools' part: layers x n_pages pages of page_bytes, K and V
+// the pools' part: layers x n_pages pages of page_bytes, K and V; `others`: the call's other arrays
+template <size_t N>
 static int32_t pool_args(rstq_ctx* ctx, const rstq_buf* on, rstq_buf* k, rstq_buf* v, int64_t layers, int64_t n_pages, int64_t page_bytes,
-                         CopyParams* p) {
+                         const Span (&others)[N], CopyParams* p) {
     RSTQ_REQUIRE(layers >= 1 && layers <= 4096 && page_bytes >= 16 && page_bytes <= (1ll << 30), RSTQ_E_SHAPE, "layers = %lld, bytes of a page = %lld",
                  (long long)layers, (long long)page_bytes);
     RSTQ_REQUIRE(page_bytes % 16 == 0, RSTQ_E_ALIGN, "%lld bytes of a page: not a multiple of 16", (long long)page_bytes);
     RSTQ_REQUIRE(paged_buf(k, ctx, layers * n_pages * page_bytes) && paged_buf(v, ctx, layers * n_pages * page_bytes), RSTQ_E_INVALID,
                  "invalid, unaligned or too small pool");
     RSTQ_REQUIRE(same_device(on, k, v), RSTQ_E_DEVICE, "buffers live on different devices");
+    const Span written[] = {{k->ptr, layers * n_pages * page_bytes}, {v->ptr, layers * n_pages * page_bytes}};
+    RSTQ_REQUIRE(apart(written, others), RSTQ_E_INVALID, "a pool lies over another array");
     *p = CopyParams{};
     p->k = (uint8_t*)k->ptr;
     p->v = (uint8_t*)v->ptr;
@@ -472,7 +480,7 @@ int32_t rstq_pages_free(rstq_ctx* ctx, rstq_buf* table, rstq_buf* lens, rstq_buf
                         int64_t seqs, int64_t n_pages, int64_t max_pages, int64_t page) {
     PageState s;
     int32_t rc = page_state(ctx, table, lens, refs, info, seqs, n_pages, max_pages, page, &s);
-    if (rc == RSTQ_OK) rc = list_args(ctx, table, list, nullptr, n);
+    if (rc == RSTQ_OK) rc = list_args(ctx, s, table, list, nullptr, n);
     if (rc != RSTQ_OK) return rc;
     DeviceState& ds = ctx->devs[table->dev];
     RSTQ_CUDA(launch_pdl(pages_free_kernel, dim3(1), dim3(kPlanThreads), 0, ds, s, (const int32_t*)list->ptr, (int)n));
@@ -486,7 +494,7 @@ int32_t rstq_pages_extend(rstq_ctx* ctx, rstq_buf* table, rstq_buf* lens, rstq_b
     int32_t rc = page_state(ctx, table, lens, refs, info, seqs, n_pages, max_pages, page, &s);
     if (rc == RSTQ_OK) {
         RSTQ_REQUIRE(counts, RSTQ_E_INVALID, "null list");
-        rc = list_args(ctx, table, list, counts, n);
+        rc = list_args(ctx, s, table, list, counts, n);
     }
     if (rc != RSTQ_OK) return rc;
     DeviceState& ds = ctx->devs[table->dev];
@@ -505,9 +513,13 @@ int32_t rstq_pages_fork(rstq_ctx* ctx, rstq_buf* kcache, rstq_buf* vcache, rstq_
     if (rc == RSTQ_OK) {
         RSTQ_REQUIRE(dst, RSTQ_E_INVALID, "null list");
         RSTQ_REQUIRE(row_bytes >= 1 && row_bytes <= (1ll << 30), RSTQ_E_SHAPE, "row_bytes = %lld", (long long)row_bytes);
-        rc = list_args(ctx, table, src, dst, n);
+        rc = list_args(ctx, s, table, src, dst, n);
     }
-    if (rc == RSTQ_OK) rc = pool_args(ctx, table, kcache, vcache, layers, n_pages, page * row_bytes, &p);
+    if (rc == RSTQ_OK) {
+        const Span others[] = {{s.table, (int64_t)s.seqs * s.width * 4}, {s.lens, s.seqs * 4ll}, {s.refs, s.n_pages * 4ll}, {s.info, 16},
+                               {src->ptr, n * 4}, {dst->ptr, n * 4}};
+        rc = pool_args(ctx, table, kcache, vcache, layers, n_pages, page * row_bytes, others, &p);
+    }
     if (rc != RSTQ_OK) return rc;
     DeviceState& ds = ctx->devs[table->dev];
     const PageScratch w = page_scratch(ds);
@@ -532,7 +544,14 @@ int32_t rstq_pages_compact(rstq_ctx* ctx, rstq_buf* kcache, rstq_buf* vcache, rs
         RSTQ_REQUIRE(paged_buf(table_out, ctx, seqs * max_pages * 4) && paged_buf(refs_out, ctx, n_pages * 4), RSTQ_E_INVALID,
                      "invalid, unaligned or too small buffer");
         RSTQ_REQUIRE(same_device(table, table_out, refs_out), RSTQ_E_DEVICE, "buffers live on different devices");
-        rc = pool_args(ctx, table, kcache, vcache, layers, n_pages, page * row_bytes, &p);
+        // in place, or somewhere else
+        const int64_t tb = (int64_t)s.seqs * s.width * 4, rb = s.n_pages * 4ll;
+        const Span to = {table_out->ptr, tb}, ro = {refs_out->ptr, rb};
+        const Span others[] = {{s.table, tb}, {s.lens, s.seqs * 4ll}, {s.refs, rb}, {s.info, 16}, to, ro};
+        RSTQ_REQUIRE((to.p == s.table || apart(to, others[0])) && apart(to, others[1]) && apart(to, others[2]) && apart(to, others[3]) &&
+                         apart(to, ro) && (ro.p == s.refs || apart(ro, others[2])) && apart(ro, others[0]) && apart(ro, others[1]) && apart(ro, others[3]),
+                     RSTQ_E_INVALID, "table_out or refs_out lies over another array");
+        rc = pool_args(ctx, table, kcache, vcache, layers, n_pages, page * row_bytes, others, &p);
     }
     if (rc != RSTQ_OK) return rc;
     DeviceState& ds = ctx->devs[table->dev];
@@ -556,8 +575,13 @@ int32_t rstq_pages_copy(rstq_ctx* ctx, rstq_buf* kcache, rstq_buf* vcache, rstq_
     RSTQ_REQUIRE(n_pages >= 1 && n_pages <= kMaxPages, RSTQ_E_LIMIT, "n_pages = %lld (1 .. %lld)", (long long)n_pages, (long long)kMaxPages);
     RSTQ_REQUIRE(dst && paged_buf(info, ctx, 16), RSTQ_E_INVALID, "invalid, unaligned or too small buffer");
     CopyParams p;
-    int32_t rc = list_args(ctx, info, src, dst, n);
-    if (rc == RSTQ_OK) rc = pool_args(ctx, info, kcache, vcache, layers, n_pages, page_bytes, &p);
+    PageState s{};
+    s.info = (int32_t*)info->ptr;
+    int32_t rc = list_args(ctx, s, info, src, dst, n);
+    if (rc == RSTQ_OK) {
+        const Span others[] = {{info->ptr, 16}, {src->ptr, n * 4}, {dst->ptr, n * 4}};
+        rc = pool_args(ctx, info, kcache, vcache, layers, n_pages, page_bytes, others, &p);
+    }
     if (rc == RSTQ_OK) rc = use_dev(ctx, info->dev);
     if (rc != RSTQ_OK) return rc;
     DeviceState& ds = ctx->devs[info->dev];

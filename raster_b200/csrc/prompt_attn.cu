@@ -588,7 +588,9 @@ int32_t prompt_configure(DeviceState& ds) {
     RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<64, true>), attr, PromptShape<64>::smem));
     RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<128, false>), attr, PromptShape<128>::smem));
     RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<128, true>), attr, PromptShape<128>::smem));
-    RSTQ_CUDA(cudaMalloc((void**)&ds.prompt_slots, (size_t)kPromptSlots * (prompt_slot<128>() * 4 + sizeof(PromptItem)) + 64));
+    const size_t slots = (size_t)kPromptSlots * (prompt_slot<128>() * 4 + sizeof(PromptItem));
+    RSTQ_CUDA(cudaMalloc((void**)&ds.prompt_slots, slots + 64));
+    RSTQ_CUDA(cudaMemsetAsync((char*)ds.prompt_slots + slots, 0, 64, ds.stream));
     return RSTQ_OK;
 }
 
@@ -634,7 +636,7 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     if (rc == RSTQ_OK) rc = rows_tensor_map(&kmap, a.k, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc == RSTQ_OK) rc = rows_tensor_map(&vmap, a.v, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc != RSTQ_OK) return rc;
-    p.counters = ds.counters + ds.counters_len - 2;
+    p.counters = p.listed + 4;
     const dim3 grid((unsigned)(parts ? ds.sm_count : std::min<int64_t>(blocks, ds.sm_count)));
     auto go = [&](auto kernel, int smem) { return launch_pdl(kernel, grid, dim3(kPrThreads), (size_t)smem, ds, p, qmap, kmap, vmap); };
     if (a.head_dim <= 64) RSTQ_CUDA(parts ? go(prompt_kernel<64, true>, PromptShape<64>::smem) : go(prompt_kernel<64, false>, PromptShape<64>::smem));
