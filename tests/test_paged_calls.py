@@ -302,3 +302,76 @@ def test_long_sequences_and_long_lists(ctx):
     c.free([8, 9] + many)
     assert c.m.used() == 0
     c.close()
+
+
+# ---- offsets beyond 32 bits -------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [128, 256])
+def test_a_pool_of_more_than_2_32_elements(ctx, d):
+    """Rows written to, read from and moved out of the last pages of a pool whose elements no 32-bit offset reaches."""
+    n_q, n_kv, page, theta, scale = 16, 1024 // d, 256, 1e4, d ** -0.5
+    size = page * n_kv * d
+    n_pages, lens = (1 << 32) // size + 6, [300, 513]                  # two pages and three, of the last six
+    table = np.array([[n_pages - 1, n_pages - 5, -1], [n_pages - 2, n_pages - 6, n_pages - 3]], np.int32)
+    rows = sum(lens)
+    bk, bv = ctx.make_buffer(n_pages * size, np.uint16), ctx.make_buffer(n_pages * size, np.uint16)
+    at = lambda b, i: ctx.wrap_buffer(b.device_ptr + 2 * size * i, size, np.uint16)  # noqa: E731
+    for i in range(n_pages - 6, n_pages):
+        for b in (bk, bv):
+            w = at(b, i)
+            w.fill_bytes(0xFF)
+            w.free()
+    q, k, v = (normal(s, rows, h, d) for s, h in ((1, n_q), (2, n_kv), (3, n_kv)))
+    up = ctx.array_to_buffer
+    bq, bkn, bvn, bt, bl = up(q), up(k), up(v), up(table), up(np.array(lens, np.int32))
+    cu = np.cumsum([0] + lens).astype(np.int32)
+    bcu, bqt, bo = up(cu), ctx.make_buffer(rows * n_q * d, np.uint16), ctx.make_buffer(rows * n_q * d, np.uint16)
+    ctx.paged_rope_append(bq, bkn, bvn, bqt, bk, bv, bt, bl, bcu, rows, 2, n_q, n_kv, d, page, n_pages, 3, theta, L.F32, L.BF16)
+    ctx.sync()
+
+    def pages(pool, tab):
+        out = []
+        for b, n in enumerate(lens):
+            parts = []
+            for j in range(-(-n // page)):
+                w = at(pool, int(tab[b, j]))
+                parts.append(pm.from_bf16(w.download()).reshape(page, n_kv, d))
+                w.free()
+            out.append(np.concatenate(parts)[:n])
+        return out
+    kk, vv = pages(bk, table), pages(bv, table)
+    for b, n in enumerate(lens):
+        assert np.array_equal(vv[b], pm.from_bf16(pm.to_bf16(v[cu[b]:cu[b + 1]])))
+        for i in (0, n // 2, n - 1):       # (rounded once; the angle's sine and cosine to 2^-22 of a row's largest)
+            want = pm.rope(k[cu[b] + i], i, theta)
+            assert (np.abs(kk[b][i] - want) <= pm.HALF["bf16"] * np.abs(want) + 2.0 ** -20 * np.abs(k[cu[b] + i]).max()).all()
+    qt = pm.from_bf16(bqt.download()).reshape(rows, n_q, d)
+    heads = (n_q, n_q // n_kv, n_kv, d, page, n_pages, 3, scale)
+
+    def check(got, b, r):
+        m = r + 1
+        want, tol = pm.attention(qt[cu[b] + r][None], kk[b][:m], vv[b][:m], scale, False, "bf16")
+        close(got[None], want, tol, f"sequence {b} row {r}")
+    ctx.paged_prompt_attention(bqt, bk, bv, bo, bt, bcu, bl, rows, 2, *heads, True, L.BF16)
+    ctx.sync()
+    got = pm.from_bf16(bo.download()).reshape(rows, n_q, d)
+    for b, n in enumerate(lens):
+        for r in (0, 255, 256, n - 1):
+            check(got[cu[b] + r], b, r)
+    last = up(pm.to_bf16(qt[cu[1:] - 1]))
+    ctx.paged_decode_attention(last, bk, bv, bo, bt, bl, 2, *heads, L.BF16)
+    ctx.sync()
+    got = pm.from_bf16(bo.download(n=2 * n_q * d)).reshape(2, n_q, d)
+    for b, n in enumerate(lens):
+        check(got[b], b, n - 1)
+    # to the first pages
+    refs = np.zeros(n_pages, np.int32)
+    refs[table[table >= 0]] = 1
+    br, bi = up(refs), ctx.make_buffer(4, np.int32)
+    ctx.pages_compact(bk, bv, bt, bl, br, bt, br, bi, 2, n_pages, 3, page, 1, n_kv * d * 2)
+    ctx.sync()
+    moved = bt.download().reshape(2, 3)
+    assert bi.download().tolist() == [0, 5, 5, 0] and sorted(moved[table >= 0]) == list(range(5))
+    assert all(np.array_equal(a, b) for a, b in zip(kk + vv, pages(bk, moved) + pages(bv, moved)))
+    for b in (bk, bv, bq, bkn, bvn, bt, bl, bcu, bqt, bo, last, br, bi):
+        b.free()
