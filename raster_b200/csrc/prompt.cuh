@@ -153,7 +153,7 @@ struct PromptItem {
         return causal ? min(max(keys - behind + 1 + r, 0), keys) : keys;
     }
 };
-constexpr int kMaxParts = 16;
+constexpr int kMaxParts = 16, kPartRounds = 3;
 // One lane's sequence cut into blocks of `per` rows, and the tiles of `tile` keys that block k sees.
 struct PromptSequence {
     int n, keys, row0, first, blocks;
@@ -182,29 +182,54 @@ __device__ __forceinline__ int prompt_count(const PromptSequence& q, int per, in
     for (int k = 0; k < q.blocks; ++k) c += prompt_parts(q.tiles(k, per, causal, tile), share);
     return c;
 }
-// How many tiles of keys a part should have, half of what each of `sms` blocks of threads would have to do: no fewer than eight, and all
-// (no parts) where that makes more than `most` items of work in all.  heads: items per block of rows.
-static __device__ __forceinline__ int prompt_share(const PromptArgs& a, int per, int tile, int heads, int sms, int most, int* total) {
+// Items of all sequences with parts of about `share` tiles; more than `most`: that they are more.
+static __device__ __forceinline__ int prompt_items(const PromptArgs& a, int per, int tile, int share, int most) {
     const int lane = threadIdx.x & 31;
-    float all = 0.f;       // (sums of integers below 2^24, or large enough not to matter)
-    for (int b0 = 0; b0 < a.seqs; b0 += 32) {
-        PromptSequence q;
-        q.load(a, b0 + lane, per);
-        float w = q.blocks ? 0.5f * (float)q.blocks * (float)(q.tiles(0, per, a.causal, tile) + q.tiles(q.blocks - 1, per, a.causal, tile)) : 0.f;
-#pragma unroll
-        for (int d = 16; d; d >>= 1) w += __shfl_xor_sync(0xffffffffu, w, d);
-        all += w;
-    }
-    const int share = (int)fminf(fmaxf(ceilf(all * (float)heads / (float)(2 * sms)), 8.f), 1e9f);
     int items = 0;
     for (int b0 = 0; b0 < a.seqs && items <= most; b0 += 32) {
         PromptSequence q;
         q.load(a, b0 + lane, per);
-        if (__any_sync(0xffffffffu, q.blocks > most)) items = most + 1;
-        else items += __reduce_add_sync(0xffffffffu, prompt_count(q, per, a.causal, tile, share));
+        if (__any_sync(0xffffffffu, q.blocks > most)) return most + 1;
+        items += __reduce_add_sync(0xffffffffu, prompt_count(q, per, a.causal, tile, share));
     }
-    *total = (int64_t)items * heads <= most ? items * heads : 0;
-    return *total ? share : 1 << 30;
+    return items;
+}
+// How many tiles of keys a part should have; all (no parts, *total = 0) where that is sooner done.  `sms` blocks of threads take the items in
+// rounds: for one, two and three of them the shortest parts that do not need another, and of these and of whole blocks what takes the
+// fewest tiles one after the other.  An item costs about two tiles beside its own, the joining launch three; parts of fewer than four tiles are not made.  heads: items per block of rows.
+static __device__ __forceinline__ int prompt_share(const PromptArgs& a, int per, int tile, int heads, int sms, int* total) {
+    const int lane = threadIdx.x & 31;
+    float all = 0.f;       // (sums of integers below 2^24, or large enough not to matter)
+    int longest = 0, blocks = 0;
+    for (int b0 = 0; b0 < a.seqs; b0 += 32) {
+        PromptSequence q;
+        q.load(a, b0 + lane, per);
+        const int last = q.blocks ? q.tiles(q.blocks - 1, per, a.causal, tile) : 0;
+        float w = q.blocks ? 0.5f * (float)q.blocks * (float)(q.tiles(0, per, a.causal, tile) + last) : 0.f;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) w += __shfl_xor_sync(0xffffffffu, w, d);
+        all += w;
+        longest = max(longest, __reduce_max_sync(0xffffffffu, last));
+        blocks = min(blocks + __reduce_add_sync(0xffffffffu, min(q.blocks, 1 << 20)), 1 << 25);
+    }
+    int best = 1 << 30, items = 0;
+    int64_t cost = ((int64_t)blocks * heads + sms - 1) / sms * (longest + 2);
+    for (int rounds = 1; rounds <= kPartRounds; ++rounds) {
+        const int most = rounds * sms / heads;
+        int share = (int)fminf(fmaxf(ceilf(all * (float)heads / (float)(rounds * sms)), 4.f), 1e6f);
+        for (int tries = 0; tries < 6; ++tries, share += (share >> 3) + 1) {
+            const int64_t now = (int64_t)rounds * (share + 2) + 3;
+            if (now >= cost) break;
+            const int n = prompt_items(a, per, tile, share, most);
+            if (n > most) continue;
+            cost = now;
+            best = share;
+            items = n * heads;
+            break;
+        }
+    }
+    *total = items;
+    return best;
 }
 // Block `item` of those of all sequences, `per` rows each, all of its keys; counted from the end, so that the blocks with most keys of a
 // long sequence come first.  A warp's lanes work together and get the same answer.

@@ -40,7 +40,7 @@ struct PromptParams {
     int pack;                        // log2 of the heads of a group that share a tile: its rows are (row of q, head), the head innermost
     int heads;                       // items per block of rows: n_kv, or n_q without packing
     int bound;                       // items there are at most
-    int sms, most;                   // blocks of threads; items of work up to which a block's keys may be cut into parts (0: never)
+    int sms;                         // blocks of threads that take the items of a call whose blocks' keys may be cut into parts
     int box;                         // rows of a box of keys
     int sectors;                     // the rows of out begin on 32-byte boundaries, and so do their pieces of 16 columns
     float scale2;
@@ -123,7 +123,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     if (warp == 8) {
         if (PARTS) {
             int items;
-            share = prompt_share(p.a, per, kPrRows, p.heads, p.sms, p.most, &items);
+            share = prompt_share(p.a, per, kPrRows, p.heads, p.sms, &items);
             if (blockIdx.x == 0 && lane == 0) *p.listed = items;
         }
         first = PARTS ? prompt_item(p.a, per, kPrRows, share, blockIdx.x / p.heads) : prompt_block(p.a, per, kPrRows, blockIdx.x / p.heads);
@@ -619,15 +619,17 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     p.heads = p.pack ? a.n_kv : a.n_q;
     // Two query tiles per block keep the tensor core busy; with fewer blocks than SMs one each does the rows sooner.
     p.tiles = a.rows * a.n_q <= kPrRows * (int64_t)ds.sm_count ? 1 : 2;
-    const int per = (p.tiles * kPrRows) >> p.pack;
-    const int64_t blocks = (a.rows / per + std::min<int64_t>(a.seqs, a.rows)) * p.heads;     // no sequence has more than this of them
-    RSTQ_REQUIRE(blocks < (1ll << 31), RSTQ_E_LIMIT, "%lld thread blocks", (long long)blocks);
     // Few blocks of rows that may see many keys (a cache, or more keys than rows): these are cut into parts, which a second launch joins.
-    const int64_t keys = a.kv.table ? (int64_t)a.kv.width << a.kv.shift : a.kv_rows > a.rows ? a.kv_rows : 0;
-    const bool parts = keys > 8 * kPrRows && (a.rows / per + std::min<int64_t>(a.seqs, a.rows)) * p.heads <= ds.sm_count;
-    p.sms = ds.sm_count;
+    // (A sequence's rows of more than a tile then take two as well: there is no lack of parts.)
+    const int64_t keys = a.kv.table ? (int64_t)a.kv.width << a.kv.shift : a.kv_rows > a.rows ? a.kv_rows : 0, some = std::min<int64_t>(a.seqs, a.rows);
+    const int tiles = a.rows << p.pack > kPrRows * some ? 2 : 1;
+    const bool parts = keys > 8 * kPrRows && (a.rows / ((tiles * kPrRows) >> p.pack) + some) * p.heads <= ds.sm_count;
+    if (parts) p.tiles = tiles;
+    const int per = (p.tiles * kPrRows) >> p.pack;
+    const int64_t blocks = (a.rows / per + some) * p.heads;     // no sequence has more than this of them
+    RSTQ_REQUIRE(blocks < (1ll << 31), RSTQ_E_LIMIT, "%lld thread blocks", (long long)blocks);
+    p.sms = std::min(ds.sm_count, kPromptSlots / kPartRounds);
     p.bound = parts ? 1 << 30 : (int)blocks;
-    p.most = kPromptSlots;
     p.part = ds.prompt_slots;
     p.list = (PromptItem*)(ds.prompt_slots + (int64_t)kPromptSlots * prompt_slot<128>());
     p.listed = (int*)(p.list + kPromptSlots);
@@ -637,7 +639,7 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     if (rc == RSTQ_OK) rc = rows_tensor_map(&vmap, a.v, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc != RSTQ_OK) return rc;
     p.counters = p.listed + 4;
-    const dim3 grid((unsigned)(parts ? ds.sm_count : std::min<int64_t>(blocks, ds.sm_count)));
+    const dim3 grid((unsigned)(parts ? p.sms : std::min<int64_t>(blocks, ds.sm_count)));
     auto go = [&](auto kernel, int smem) { return launch_pdl(kernel, grid, dim3(kPrThreads), (size_t)smem, ds, p, qmap, kmap, vmap); };
     if (a.head_dim <= 64) RSTQ_CUDA(parts ? go(prompt_kernel<64, true>, PromptShape<64>::smem) : go(prompt_kernel<64, false>, PromptShape<64>::smem));
     else RSTQ_CUDA(parts ? go(prompt_kernel<128, true>, PromptShape<128>::smem) : go(prompt_kernel<128, false>, PromptShape<128>::smem));
