@@ -10,8 +10,11 @@
 //
 // A block has 128 query rows of one sequence and head.  Four warps fetch K and V, a tile of 64 keys at a time and one ahead in
 // registers, split them and write the terms to shared memory, swizzled as the tensor core wants them (zeros behind the last key);
-// four warps are the softmax, a thread per row, P's three terms over S in tensor memory; one thread issues.  With head_dim above 64 there
-// are two places for S and P, and the next tile's S is formed while this one's exponentials are; up to 64 two blocks share an SM.
+// four warps are the softmax, a thread per row, P's three terms over S in tensor memory; one thread issues.  There are two places for S and
+// P, and the next tile's S is formed while this one's exponentials are.  (Of 64 columns two blocks with one place each would fit an SM: two
+// sequences of 1000 rows 63 us, against 46.)  A step of 64 keys takes 1.7 us with 64 columns, 3.7 with 128, of which the MMAs are 1 and 2
+// (an MMA of S is bound by reading Q and K from shared memory, 48 cycles): the rest is the way from S through the softmax to P V and, with
+// 128, V's terms, which wait for the last product with V.  1024 rows of 16 heads: 37 and 67 us.
 // An infinity or NaN has no such terms: a block that meets one (in keys or values its rows may not even see) computes its rows one by one
 // (attend_row), and so does one whose table names no page.
 #include <algorithm>
@@ -21,12 +24,11 @@
 namespace rstq {
 
 constexpr int kPfThreads = 288;      // softmax, split, MMA
-constexpr int kPfRows = 128, kPfKeys = 64;
+constexpr int kPfRows = 128, kPfKeys = 64, kPfPlaces = 2;      // places for S in tensor memory
 template <int HD>
 struct PromptShapeF {
     static constexpr int blks = HD / 64, qblk = kPfRows * 128, kblk = kPfKeys * 128;     // 64 columns of a term
     static constexpr int qplane = blks * qblk, kplane = blks * kblk;
-    static constexpr int bufs = HD == 128 ? 2 : 1, cols = HD == 128 ? 512 : 256;          // places for S; tensor memory
     static constexpr int smem = 1024 + 3 * (qplane + 2 * kplane);
 };
 
@@ -39,16 +41,15 @@ struct PromptParamsF {
 // The next eight bits of a pair of values, as bf16 pair; the values become what is left.
 __device__ __forceinline__ uint32_t next_term(float& a, float& b) {
     const uint32_t w = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-    a -= __uint_as_float(w << 16);
-    b -= __uint_as_float(w & 0xFFFF0000u);
+    unpack2(fma2(pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)), pack2(-1.f, -1.f), pack2(a, b)), a, b);
     return w;
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kPfThreads, PromptShapeF<HD>::bufs == 1 ? 2 : 1)
+__global__ void __launch_bounds__(kPfThreads, 1)
 prompt_f32_kernel(const PromptParamsF p) {
     using Sh = PromptShapeF<HD>;
-    constexpr int NB = Sh::bufs;
+    constexpr int NB = kPfPlaces;
     extern __shared__ uint8_t s_raw0[];
     uint8_t* s_raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw0) + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) uint64_t s_bar[11];
@@ -80,7 +81,7 @@ prompt_f32_kernel(const PromptParamsF p) {
         fence_async_smem();
     }
     if (warp == 8) {
-        tmem_alloc(smem_u32(&s_tmem), Sh::cols);
+        tmem_alloc(smem_u32(&s_tmem), 512);
         tmem_relinquish();
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -119,7 +120,8 @@ prompt_f32_kernel(const PromptParamsF p) {
                 tmem_ld16(tS + 64 + c, b);
                 tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[c + i] = __uint_as_float(a[i]) + __uint_as_float(b[i]);
+                for (int i = 0; i < 16; i += 2)
+                    unpack2(add2(pack2(__uint_as_float(a[i]), __uint_as_float(a[i + 1])), pack2(__uint_as_float(b[i]), __uint_as_float(b[i + 1]))), s[c + i], s[c + i + 1]);
             }
             if ((j + 1) * kPfKeys > least) {
                 const int lim = mine - j * kPfKeys;
@@ -155,15 +157,18 @@ prompt_f32_kernel(const PromptParamsF p) {
                     }
                 }
             }
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
+            uint64_t part[2] = {0ull, 0ull};
+            const uint64_t scale = pack2(p.scale2, p.scale2), minus = pack2(-m2, -m2);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 uint32_t w[3][16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    float a = ex2f(fmaf(s[c * 32 + 2 * i], p.scale2, -m2)), b = ex2f(fmaf(s[c * 32 + 2 * i + 1], p.scale2, -m2));
-                    part[i & 1] += a;
-                    part[2 + (i & 1)] += b;
+                    float a, b;
+                    unpack2(fma2(pack2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), scale, minus), a, b);
+                    a = ex2f(a);
+                    b = ex2f(b);
+                    part[i & 1] = add2(part[i & 1], pack2(a, b));
                     w[0][i] = next_term(a, b);
                     w[1][i] = next_term(a, b);
                     w[2][i] = next_term(a, b);
@@ -171,12 +176,14 @@ prompt_f32_kernel(const PromptParamsF p) {
 #pragma unroll
                 for (int x = 0; x < 3; ++x) tmem_st16(tS + x * 32 + c * 16, w[x]);
             }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            float a, b;
+            unpack2(add2(part[0], part[1]), a, b);
+            sum += a + b;
             tmem_st_wait();
             tc_fence_before();
-            // Two places: S of the last tile came before the last P V but one was done.  That is waited for here, while the last one cannot
+            // S of the last tile came before the last P V but one was done.  That is waited for here, while the last one cannot
             // be done yet: afterwards a parity would not tell the two apart.
-            if (NB == 2 && j == n - 1 && j > 0) ok = wait_phase(odone, (j - 1) & 1, abort_flag);
+            if (j == n - 1 && j > 0) ok = wait_phase(odone, (j - 1) & 1, abort_flag);
             __syncwarp();
             if (lane == 0) mbar_arrive(pfull + 8 * buf);
         }
@@ -256,8 +263,7 @@ prompt_f32_kernel(const PromptParamsF p) {
         auto only = [&](bool there, float4 x) {
             return make_float4(there ? x.x : 0.f, there ? x.y : 0.f, there ? x.z : 0.f, there ? x.w : 0.f);
         };
-        // K is written a tile ahead of V: with two places for S before the V of the tile before it, as the next S comes before that P V,
-        // with one behind it.
+        // K is written a tile ahead of V: the next S comes before this tile's P V
         float4 k[NI], v[NI];
         int r1 = places(0), r2 = places(1);
         uint32_t klive = 0, vlive = 0;
@@ -296,13 +302,12 @@ prompt_f32_kernel(const PromptParamsF p) {
             klive = rows_in(r2);
             r1 = r2;
             r2 = places(j + 2);
-            if (NB == 2) write_k(j + 1);
+            write_k(j + 1);
             if (ok) ok = wait_phase(vfree, (j & 1) ^ 1u, abort_flag);
             if (!ok) break;
 #pragma unroll
             for (int i = 0; i < NI; ++i) write(sv, Sh::kplane, Sh::kblk, w * 16 + i * RPI + sub, only(vlive >> (i * RPI) & 1, v[i]));
             hand(vfull);
-            if (NB == 1) write_k(j + 1);
         }
     } else {
         // ---- MMAs ----
@@ -335,7 +340,7 @@ prompt_f32_kernel(const PromptParamsF p) {
         if (n > 0) product_s(0);
         for (int j = 0; j < n && ok; ++j) {
             const uint32_t tP = tmem + (j % NB) * 128;
-            if (NB == 2 && j + 1 < n) product_s(j + 1);
+            if (j + 1 < n) product_s(j + 1);
             wait(vfull, j & 1);
             wait(pfull + 8 * (j % NB), (j / NB) & 1);
             if (!ok) break;
@@ -347,7 +352,6 @@ prompt_f32_kernel(const PromptParamsF p) {
                             j > 0 || x > 1 || k > 0);
             umma_commit_if(odone, leader);
             umma_commit_if(vfree, leader);
-            if (NB == 1 && j + 1 < n) product_s(j + 1);
         }
         if (!ok && n > 0) {      // products under way are waited for (with a limit) before the memory they use is given up
             volatile int none = 0;
@@ -357,7 +361,7 @@ prompt_f32_kernel(const PromptParamsF p) {
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) tmem_dealloc(tmem, Sh::cols);
+    if (warp == 8) tmem_dealloc(tmem, 512);
     if (tid == 0 && s_abort) atomicExch(p.status, 2);
 }
 
