@@ -2,7 +2,8 @@
 //
 //   out[i] = sum_j p_ij V[j] / sum_j p_ij,   p_ij = exp(scale q_i.K_j - m_i),   j <= i + (keys - rows) of its sequence
 //
-// A thread block has 256 query rows of one sequence and head as two tiles of 128, and walks the sequence's keys in tiles of 128:
+// A block of rows is two query tiles of 128 (row, head) pairs of one sequence: 256 rows of a head, or 256 / group rows of all heads of a
+// group that is a power of two, which then read K and V once and fill the tiles with few rows.  Its keys go by in tiles of 128:
 //
 //   S = Q K^T   (tcgen05, Q and K from shared memory, S in tensor memory)
 //   P = exp2(scale2 S - m)   (a warpgroup per query tile, a thread per row: S from tensor memory, P back over it in bf16)
@@ -12,12 +13,25 @@
 // only when it grows by more than 2^8: until then P is up to 256 and O need not be rescaled (sums are f32; P's relative rounding
 // does not depend on its size), so O is read and written back for a few tiles at the start of a row and hardly ever after.
 // P is rounded to bf16, the type of V (2^-9 rms of each weight, no more than the result's own rounding); its sum is taken before that.
+// P is handed to the tensor core in halves, as soon as each is written.
 //
-// K and V come by TMA through one ring, a box of 128 packed rows or one per page.  Keys a row does not see get -inf before the
-// maximum.  V's rows behind a sequence's end (another sequence's, a stale page's) are zeroed in shared memory before the product, for
-// 0 * NaN is NaN; what lies above the diagonal cannot be zeroed, it belongs to other rows: a warp looks through those few tiles, and where
-// it finds an infinity or NaN the block's rows are computed again one by one, from the positions they see alone (attend_row).
+// K and V come by TMA through one ring, a box of 128 packed rows or one per page (the table is read a tile ahead).  Keys a row does not see
+// get -inf before the maximum.  V's rows behind a sequence's end (another sequence's, a stale page's) are zeroed in shared memory before the
+// product, for 0 * NaN is NaN; what lies above the diagonal cannot be zeroed, it belongs to other rows: a warp looks through those few tiles,
+// and where it finds an infinity or NaN the block's rows are computed again one by one, from the positions they see alone (attend_row).
 // So are those of a block whose table names no page.
+//
+// A thread block stays on its SM and takes the next block of rows, those with most keys of a sequence first, when its copies for this one are
+// out (a counter): the next rows' Q, K and V are on their way during the last products.  Few blocks of rows that see many keys are cut
+// into parts along the keys (prompt_share); a part leaves its sums, maximum and weight in a slot, and a second launch joins them in order, so
+// that results do not depend on who was first.
+//
+// What it takes.  A step (256 rows, 128 keys, head_dim 128) takes 1.9 us, of which the MMAs are 1.05 and the exponentials, on the
+// SM's 16 special-function lanes, as much: the chain S, maximum, exponentials, P V, next S of each tile does not close any tighter in 512
+// columns of tensor memory, two places for S per tile would need 768.  8192 rows, 32 heads over 8: 436 us, 1260 TFLOP/s (510 in a row, at
+// the power limit: 1080); 4096 rows 122 us; 8192 of 64 columns 380 us.  Beside the steps a block of rows costs 2.6 us, mostly its stores,
+// and a launch 5 to 7 us until the first S.  512 rows behind 16000 keys 158 us (in parts; 255 with one query tile per block), 2 rows 32 us.
+// A polynomial in place of a part of the exponentials was slower, so were 64 keys per tile with two places for S.
 #include <algorithm>
 
 #include "prompt.cuh"
