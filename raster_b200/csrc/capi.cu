@@ -670,6 +670,7 @@ int32_t rstq_shutdown(rstq_ctx* ctx) {
         if (ds.gemm_scratch) cudaFree(ds.gemm_scratch);
         if (ds.attn_scratch) cudaFree(ds.attn_scratch);
         if (ds.attn_slots) cudaFree(ds.attn_slots);
+        if (ds.seq_starts) cudaFree(ds.seq_starts);
         if (ds.page_scratch) cudaFree(ds.page_scratch);
         if (ds.prompt_slots) cudaFree(ds.prompt_slots);
         if (ds.kq_scratch) cudaFree(ds.kq_scratch);

@@ -106,6 +106,7 @@ struct DeviceState {
     int attn_clusters[9] = {};     // ... and how many clusters of 2 .. 8 of its thread blocks the device holds at once,
     int attn_narrow_clusters[9] = {};   // or of its blocks of a quarter of the warps
     float* prompt_slots = nullptr; // prompt attention: what parts of a block's keys have found
+    int64_t* seq_starts = nullptr; // attention of many sequences: where the work of each begins
     void* page_scratch = nullptr;  // paged caches: lists of pages between the launches of one call
     void* pinned = nullptr;        // host staging for the host-array entry points
     int64_t pinned_bytes = 0;
@@ -356,7 +357,7 @@ int32_t gemm_configure(DeviceState& ds);
 // attn.cu
 int32_t attn_configure(DeviceState& ds);  // scratch, shared-memory attributes and cluster counts, once per device
 // paged_decode.cu
-int32_t decode_configure(DeviceState& ds);  // shared-memory attributes, once per device
+int32_t decode_configure(DeviceState& ds);  // scratch, shared-memory attributes, once per device
 // prompt_attn.cu
 int32_t prompt_configure(DeviceState& ds);      // scratch, shared-memory attributes, once per device
 int32_t prompt_f32_configure();

@@ -131,6 +131,58 @@ paged_rope_append_kernel(const AppendParams p, const int per_block) {
     }
 }
 
+// ---- many sequences ------------------------------------------------------------------------------
+// One block: a thread per sequence of 1024 at a time, sums over warps and then over the block.
+constexpr int kSumThreads = 1024;
+__global__ void __launch_bounds__(kSumThreads)
+sums_kernel(const PromptArgs a, const int per, const int extra, int64_t* __restrict__ start) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    __shared__ int64_t s_warp[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t base = 0;
+    for (int b0 = 0; b0 < a.seqs; b0 += kSumThreads) {
+        const int b = b0 + threadIdx.x;
+        int64_t v = 0;
+        if (b < a.seqs) {
+            int64_t first, last;
+            if (a.cu_q) {
+                packed_range(a.cu_q, b, a.rows, &first, &last);
+                v = (last - first + per - 1) / per;
+            } else {
+                const int64_t len = kv_length(a.kv, b, &first);
+                v = len > 0 ? (len + per - 1) / per + extra : 0;
+            }
+        }
+        int64_t x = v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += y;
+        }
+        if (lane == 31) s_warp[warp] = x;
+        __syncthreads();
+        if (warp == 0) {
+            int64_t w = s_warp[lane];
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t y = __shfl_up_sync(0xffffffffu, w, d);
+                if (lane >= d) w += y;
+            }
+            s_warp[lane] = w;
+        }
+        __syncthreads();
+        if (b < a.seqs) start[b] = base + x - v + (warp ? s_warp[warp - 1] : 0);
+        base += s_warp[31];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) start[a.seqs] = base;
+}
+int32_t launch_sums(DeviceState& ds, const PromptArgs& a, int per, int extra) {
+    RSTQ_CUDA(launch_pdl(sums_kernel, dim3(1), dim3(kSumThreads), 0, ds, a, per, extra, ds.seq_starts));
+    return RSTQ_OK;
+}
+
 // ---- attention, any shape -----------------------------------------------------------------------
 // One query row and head per thread block: its four warps take four positions in turn (attend_row), and their states are joined
 // through shared memory.  For what the tiled kernels do not take: head_dim above 128, a scale that is not positive (they find the maximum
@@ -303,6 +355,7 @@ static int32_t attention_args(rstq_ctx* ctx, rstq_buf* q, rstq_buf* k, rstq_buf*
     a->rows = rows; a->ldq = ldq;
     a->seqs = (int)seqs; a->n_q = (int)n_q; a->group = (int)group; a->n_kv = (int)n_kv; a->head_dim = (int)head_dim;
     a->scale = (float)scale; a->causal = causal; a->dtype = dtype; a->kv_rows = kv_rows;
+    a->start = nullptr;
     return use_dev(ctx, q->dev);
 }
 
@@ -314,10 +367,10 @@ int32_t rstq_paged_decode_attention(rstq_ctx* ctx, rstq_buf* q, rstq_buf* kcache
                                 page, n_pages, max_pages, ldq, 0, scale, 0, dtype, false, &a);
     if (rc != RSTQ_OK) return rc;
     DeviceState& ds = ctx->devs[q->dev];
-    rc = head_dim <= 128 ? launch_paged_decode(ds, a) : launch_attention_rows(ds, a);
-    if (rc != RSTQ_OK) return rc;
-    ctx->launches++;
-    return RSTQ_OK;
+    int launches = 1;
+    rc = head_dim <= 128 ? launch_paged_decode(ds, a, &launches) : launch_attention_rows(ds, a);
+    if (rc == RSTQ_OK) ctx->launches += launches;
+    return rc;
 }
 
 static int32_t run_prompt(rstq_ctx* ctx, rstq_buf* q, const PromptArgs& a) {
@@ -326,7 +379,7 @@ static int32_t run_prompt(rstq_ctx* ctx, rstq_buf* q, const PromptArgs& a) {
     int32_t rc;
     int launches = 1;
     if (a.head_dim > 128 || a.scale <= 0.f || a.kv_rows == 0) rc = launch_attention_rows(ds, a);
-    else rc = a.dtype == RSTQ_BF16 ? launch_prompt(ds, a, &launches) : launch_prompt_f32(ds, a);
+    else rc = a.dtype == RSTQ_BF16 ? launch_prompt(ds, a, &launches) : launch_prompt_f32(ds, a, &launches);
     if (rc == RSTQ_OK) ctx->launches += launches;
     return rc;
 }

@@ -52,6 +52,7 @@ struct DecodeParams {
     int* counters;                                    // [blocks], zero between launches
     int* status;
     int box;                                          // rows of a box: min(page, tile)
+    const int64_t* start;                             // units of a head before each sequence; null: few sequences
 };
 template <typename T>
 __host__ __device__ constexpr int dec_tile() { return sizeof(T) == 2 ? 64 : 32; }
@@ -102,6 +103,7 @@ __device__ __forceinline__ void bar_consumers() { asm volatile("bar.sync 1, 128;
 // What the end of a (sequence, head) costs a block, in tiles: its warps' states are joined and the next one's queries taken.  (0, 1, 2, 3:
 // 16 sequences of 300 13.9, 12.9, 11.9, 12.9 us, of 4000 49.3, 48.5, 47.8, 48.9; four in f32 of 1300 35.8, 35.3, 34.9, 35.3.)
 constexpr int kDecEnd = 2;
+constexpr int kDecSums = 256;                         // sequences above which launch_sums adds the lengths up (1000 of 100: 115 -> 107 us)
 constexpr float kRest = 7.8886091e-31f;      // 2^-100
 
 // Where a block's range of units lies.  Units of sequence b: for each of H heads its tiles, and kDecEnd for what the end of a part costs.  All lanes of a warp hold the same,
@@ -150,6 +152,26 @@ __device__ __forceinline__ void dec_past(const DecodeParams& p, int H, Walk* w, 
 template <int TILE, typename F>
 __device__ __forceinline__ int64_t dec_find(const DecodeParams& p, int H, Walk* w, F range) {
     const int lane = threadIdx.x & 31;
+    int64_t first, last;
+    if (p.start) {
+        const int64_t total = p.start[p.seqs] * H;
+        range(total, &first, &last);
+        w->left = last - first;
+        if (w->left <= 0) return total;
+        w->b = find_start(p.start, p.seqs, first / H);
+        // (the first unit of sequence b is start[b] * H, so b is the last one with start[b] <= first / H)
+        w->first = w->b & ~31;
+        w->lens = dec_len(p, w->first + lane);
+        w->len = __shfl_sync(0xffffffffu, w->lens, w->b - w->first);
+        const int units = dec_units<TILE>(w->len);
+        w->nt = units - kDecEnd;
+        const int64_t in = first - p.start[w->b] * H;
+        w->h = units > 0 ? (int)(in / units) : 0;
+        w->t = (int)(in - (int64_t)w->h * units);
+        if (units == 0 || w->h >= H) w->left = 0;      // (cannot be, unless a length changed meanwhile)
+        else dec_past<TILE>(p, H, w, 0);
+        return total;
+    }
     const int head = dec_len(p, lane);
     int64_t total = dec_units<TILE>(head);
     for (int b0 = 32; b0 < p.seqs; b0 += 128) {
@@ -162,7 +184,6 @@ __device__ __forceinline__ int64_t dec_find(const DecodeParams& p, int H, Walk* 
 #pragma unroll
     for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
     total *= H;
-    int64_t first, last;
     range(total, &first, &last);
     w->left = last - first;
     if (w->left <= 0) return total;
@@ -735,7 +756,7 @@ int32_t decode_configure(DeviceState& ds) {
     RSTQ_CUDA(set(paged_decode_kernel<float, 128, 1>, dec_smem<128>()));
     RSTQ_CUDA(set(paged_decode_kernel<float, 128, 4>, dec_smem<128>()));
     RSTQ_CUDA(set(paged_decode_kernel<float, 128, 8>, dec_smem<128>()));
-    (void)ds;
+    RSTQ_CUDA(cudaMalloc((void**)&ds.seq_starts, (size_t)(kMaxSeqs + 1) * 8));
     return RSTQ_OK;
 }
 
@@ -753,7 +774,7 @@ int32_t rows_tensor_map(CUtensorMap* m, const void* base, int32_t dtype, int64_t
     return RSTQ_OK;
 }
 
-int32_t launch_paged_decode(DeviceState& ds, const PromptArgs& a) {
+int32_t launch_paged_decode(DeviceState& ds, const PromptArgs& a, int* launches) {
     DecodeParams p;
     p.q = a.q; p.k = a.k; p.v = a.v; p.out = a.out;
     p.kv = a.kv;
@@ -774,6 +795,13 @@ int32_t launch_paged_decode(DeviceState& ds, const PromptArgs& a) {
     const int64_t blocks = 2 * (int64_t)ds.sm_count;
     static_assert(2 * dec_slot<128>() >= 2 * dec_slot<64>(), "slots");
     RSTQ_REQUIRE(2 * blocks * dec_slot<128>() * 4 <= ds.partials_bytes && blocks <= ds.counters_len, RSTQ_E_LIMIT, "%lld thread blocks", (long long)blocks);
+    *launches = 1;
+    p.start = nullptr;
+    if (a.seqs > kDecSums) {
+        if ((rc = launch_sums(ds, a, tile, kDecEnd)) != RSTQ_OK) return rc;
+        p.start = ds.seq_starts;
+        ++*launches;
+    }
     const int g = std::min(a.group, per);
     const size_t smem = (size_t)(a.head_dim <= 64 ? dec_smem<64>() : dec_smem<128>());
     auto go = [&](auto kernel) { return launch_pdl(kernel, dim3((unsigned)blocks), dim3(kDecThreads), smem, ds, p, kmap, vmap); };

@@ -237,6 +237,25 @@ static __device__ __forceinline__ PromptItem prompt_block(const PromptArgs& a, i
     const int lane = threadIdx.x & 31;
     PromptItem it;
     it.rows = 0;
+    if (a.start) {
+        const int64_t at = a.start[a.seqs] - 1 - item;
+        if (at < 0) return it;
+        const int b = find_start(a.start, a.seqs, at);
+        PromptSequence q;
+        q.load(a, b, per);
+        const int k = (int)(at - a.start[b]);
+        if ((int64_t)k * per >= q.n) return it;
+        it.b = b;
+        it.keys = q.keys;
+        it.row = q.first + (int64_t)k * per;
+        it.behind = q.n - k * per;
+        it.rows = it.behind < per ? it.behind : per;
+        it.row0 = q.row0;
+        it.parts = 1;
+        it.part = it.j0 = 0;
+        it.j1 = q.tiles(k, per, a.causal, tile);
+        return it;
+    }
     for (int b0 = (a.seqs - 1) & ~31; b0 >= 0; b0 -= 32) {
         PromptSequence q;
         q.load(a, b0 + 31 - lane, per);

@@ -653,6 +653,12 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     if (rc == RSTQ_OK) rc = rows_tensor_map(&vmap, a.v, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc != RSTQ_OK) return rc;
     p.counters = p.listed + 4;
+    *launches = parts ? 2 : 1;
+    if (!parts && a.seqs > kSumSeqs) {
+        if ((rc = launch_sums(ds, a, per, 0)) != RSTQ_OK) return rc;
+        p.a.start = ds.seq_starts;
+        ++*launches;
+    }
     const dim3 grid((unsigned)(parts ? p.sms : std::min<int64_t>(blocks, ds.sm_count)));
     auto go = [&](auto kernel, int smem) { return launch_pdl(kernel, grid, dim3(kPrThreads), (size_t)smem, ds, p, qmap, kmap, vmap); };
     if (a.head_dim <= 64) RSTQ_CUDA(parts ? go(prompt_kernel<64, true>, PromptShape<64>::smem) : go(prompt_kernel<64, false>, PromptShape<64>::smem));
@@ -660,8 +666,7 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     if (parts) {
         const dim3 join((unsigned)(12 * ds.sm_count));
         RSTQ_CUDA(a.head_dim <= 64 ? launch_pdl(prompt_join_kernel<64>, join, dim3(256), 0, ds, p) : launch_pdl(prompt_join_kernel<128>, join, dim3(256), 0, ds, p));
-        *launches = 2;
-    } else *launches = 1;
+    }
     return RSTQ_OK;
 }
 

@@ -372,13 +372,20 @@ int32_t prompt_f32_configure() {
     return RSTQ_OK;
 }
 
-int32_t launch_prompt_f32(DeviceState& ds, const PromptArgs& a) {
+int32_t launch_prompt_f32(DeviceState& ds, const PromptArgs& a, int* launches) {
     PromptParamsF p;
     p.a = a;
     p.scale2 = a.scale * 1.4426950408889634f;
     p.status = ds.status;
     const int64_t blocks = (a.rows / kPfRows + std::min<int64_t>(a.seqs, a.rows)) * a.n_q;
     RSTQ_REQUIRE(blocks < (1ll << 31), RSTQ_E_LIMIT, "%lld thread blocks", (long long)blocks);
+    *launches = 1;
+    if (a.seqs > kSumSeqs) {
+        const int32_t rc = launch_sums(ds, a, kPfRows, 0);
+        if (rc != RSTQ_OK) return rc;
+        p.a.start = ds.seq_starts;
+        ++*launches;
+    }
     const dim3 grid((unsigned)blocks), block(kPfThreads);
     RSTQ_CUDA(a.head_dim <= 64 ? launch_pdl(prompt_f32_kernel<64>, grid, block, (size_t)PromptShapeF<64>::smem, ds, p)
                                : launch_pdl(prompt_f32_kernel<128>, grid, block, (size_t)PromptShapeF<128>::smem, ds, p));

@@ -375,3 +375,48 @@ def test_a_pool_of_more_than_2_32_elements(ctx, d):
     assert all(np.array_equal(a, b) for a, b in zip(kk + vv, pages(bk, moved) + pages(bv, moved)))
     for b in (bk, bv, bq, bkn, bvn, bt, bl, bcu, bqt, bo, last, br, bi):
         b.free()
+
+
+# ---- many sequences -----------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,seqs", [("bf16", 65), ("bf16", 128), ("bf16", 129), ("bf16", 700), ("f32", 129), ("f32", 1100)])
+def test_prompts_of_many_sequences(ctx, dtype, seqs):
+    """Empty ones among them, at the ends too; some of several blocks of rows."""
+    n_q, n_kv, d, page = 4, 2, 64, 16
+    rng = np.random.default_rng(seqs)
+    lens = [int(x) for x in rng.integers(0, 40, seqs)]
+    for i in (seqs // 3, seqs // 2):
+        lens[i] = 300 + i
+    new = [int(rng.integers(0, n + 1)) for n in lens]
+    new[seqs // 3] = lens[seqs // 3]
+    for i in (0, seqs // 5, seqs - 1):
+        new[i] = 0
+    lens[seqs - 1] = 0
+    x = Prompts(ctx, dtype, n_q, n_kv, d, page, lens, new, seed=seqs)
+    x.call()
+    ctx.sync()
+    x.check()
+    x.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,seqs", [("bf16", 256), ("bf16", 257), ("bf16", 3000), ("f32", 300)])
+def test_decode_of_many_sequences(ctx, dtype, seqs):
+    n_q, n_kv, d, page = 4, 2, 64, 16
+    rng = np.random.default_rng(seqs)
+    lens = [int(x) for x in rng.integers(0, 30, seqs)]
+    lens[0] = lens[seqs // 2] = lens[seqs - 1] = 0
+    lens[seqs // 3] = 900
+    p = Pool(ctx, lens, n_kv, d, page, dtype, seed=seqs)
+    q = pm.decode(pm.encode(normal(seqs, seqs, n_q, d), dtype), dtype)
+    bq, bo = ctx.array_to_buffer(pm.encode(q, dtype)), ctx.make_buffer(seqs * n_q * d, NP[dtype])
+    bo.fill_bytes(0xFF)
+    ctx.paged_decode_attention(bq, p.bk, p.bv, bo, p.bt, p.bl, seqs, n_q, 2, n_kv, d, page, p.n_pages, p.width, 0.125, DT[dtype])
+    ctx.sync()
+    got = pm.decode(bo.download(), dtype).reshape(seqs, n_q, d)
+    for b in range(seqs):
+        want, tol = pm.attention(q[b:b + 1], p.keys[b], p.values[b], 0.125, False, dtype)
+        close(got[b:b + 1], want, tol, f"sequence {b} of {lens[b]}")
+    bq.free()
+    bo.free()
+    p.free()
