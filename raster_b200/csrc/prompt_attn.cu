@@ -2,8 +2,9 @@
 //
 //   out[i] = sum_j p_ij V[j] / sum_j p_ij,   p_ij = exp(scale q_i.K_j - m_i),   j <= i + (keys - rows) of its sequence
 //
-// A block of rows is two query tiles of 128 (row, head) pairs of one sequence: 256 rows of a head, or 256 / group rows of all heads of a
-// group that is a power of two, which then read K and V once and fill the tiles with few rows.  Its keys go by in tiles of 128:
+// A block of rows is two query tiles of 128 (row, head) pairs of one sequence: 256 rows of a head, or 128 / group rows per tile of all heads of
+// a group, which then read K and V once, fill the tiles with few rows and see less beyond the diagonal (12 prompts of 28 heads over 4: 90 -> 77
+// us; 20 rows each behind 200 caches 527 -> 92).  Its keys go by in tiles of 128:
 //
 //   S = Q K^T   (tcgen05, Q and K from shared memory, S in tensor memory)
 //   P = exp2(scale2 S - m)   (a warpgroup per query tile, a thread per row: S from tensor memory, P back over it in bf16)
@@ -51,7 +52,7 @@ constexpr int kPromptSlots = 512;      // items of a call whose blocks' keys are
 struct PromptParams {
     PromptArgs a;
     int tiles;                       // query tiles of a block: 1 or 2
-    int pack;                        // log2 of the heads of a group that share a tile: its rows are (row of q, head), the head innermost
+    int pack, rpt;                   // heads of a group that share a tile (1: none), rows of q of a tile: its rows are (row of q, head), the head innermost
     int heads;                       // items per block of rows: n_kv, or n_q without packing
     int bound;                       // items there are at most
     int sms;                         // blocks of threads that take the items of a call whose blocks' keys may be cut into parts
@@ -120,6 +121,9 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
     }
+    for (int e = p.rpt * p.pack * 8 + tid; e < kPrRows * 8; e += kPrThreads)      // rows of Q's tiles that no copy fills
+        for (int c = 0; c < 2 * Sh::blks; ++c) sts128(sq + c * BLK + e * 16, 0u, 0u, 0u, 0u);
+    fence_async_smem();
     if (warp == 9) {
         tmem_alloc(smem_u32(&s_tmem), 512);
         tmem_relinquish();
@@ -132,7 +136,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     asm volatile("griddepcontrol.wait;" ::: "memory");
     PromptItem first;                // the block's first work, looked up while tensor memory is on its way
     first.rows = 0;
-    const int per = (p.tiles * kPrRows) >> p.pack;       // rows of q of a block
+    const int per = p.tiles * p.rpt;                     // rows of q of a block
     int share = 1 << 30;
     if (warp == 8) {
         if (PARTS) {
@@ -148,11 +152,11 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     const uint32_t tmem = (uint32_t)uniform((int)s_tmem);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // (not before this block has its tensor memory)
     const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + HD};
-    // keys that row r of a block's tiles sees, and the steps of a tile: tiles of keys, of the item's, that some row of it sees
-    auto sees = [&](const PromptItem& it, int r) { return it.sees(r >> p.pack, p.a.causal); };
+    // keys that row r of a block sees, and the steps of a tile: tiles of keys, of the item's, that some row of it sees
+    auto sees = [&](const PromptItem& it, int r) { return it.sees(r, p.a.causal); };
     auto steps_of = [&](const PromptItem& it, int t) {
-        const int last = min(it.rows << p.pack, (t + 1) * kPrRows) - 1;
-        return uniform(t < p.tiles && last >= t * kPrRows ? max(min(it.j1, (sees(it, last) + kPrRows - 1) / kPrRows) - it.j0, 0) : 0);
+        const int last = min(it.rows, (t + 1) * p.rpt) - 1;
+        return uniform(t < p.tiles && last >= t * p.rpt ? max(min(it.j1, (sees(it, last) + kPrRows - 1) / kPrRows) - it.j0, 0) : 0);
     };
     bool ok = true;
     // The next block of rows, of which `w` is the number; false: there is none.
@@ -174,14 +178,14 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int t = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tSt = tS[0] + t * 128 + lanes, tOt = tO[0] + t * HD + lanes;
-        const int r = t * kPrRows + (warp & 3) * 32 + lane;
+        const int rt = (warp & 3) * 32 + lane, slot_row = t * kPrRows + rt, r = t * p.rpt + rt / p.pack, mine_of = rt % p.pack;      // row of the block, head
         uint32_t c = 0;                      // steps of this tile so far (their parity is that of its barriers)
         PromptWork x;
         for (int w = 0; ok && next_work(w, &x); ++w) {
             const PromptItem& it = x.it;
             const int steps = steps_of(it, t);
             // keys of this row, of the tile's first, from the item's first on
-            const int mine = sees(it, r) - it.j0 * kPrRows, least = sees(it, t * kPrRows) - it.j0 * kPrRows;
+            const int mine = sees(it, r) - it.j0 * kPrRows, least = sees(it, t * p.rpt) - it.j0 * kPrRows;
             float m = -INFINITY, m2 = 0.f, sum = 0.f;      // running maximum of S; scale2 times it (0: nothing seen yet)
             for (int j = 0; j < steps; ++j) {
                 ok = wait_phase(sfull + 8 * t, (c + j) & 1, abort_flag);
@@ -259,9 +263,8 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             if (steps > 0 && ok) ok = wait_phase(odone + 8 * t, (c - 1) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
-            const bool has_row = t < p.tiles && (r >> p.pack) < it.rows;
-            const int head = p.pack ? (x.h << p.pack) + (r & ((1 << p.pack) - 1)) : x.h;
-            __nv_bfloat16* out = (__nv_bfloat16*)p.a.out + ((it.row + (r >> p.pack)) * p.a.n_q + head) * p.a.head_dim;
+            const bool has_row = t < p.tiles && rt < p.rpt * p.pack && r < it.rows;
+            __nv_bfloat16* out = (__nv_bfloat16*)p.a.out + ((it.row + r) * p.a.n_q + x.h * p.pack + mine_of) * p.a.head_dim;
             const bool again = s_again[w & 1] != 0;
             // (a part of a block's keys: what it has found goes to its slot, for prompt_join_kernel)
             const bool whole = !PARTS || it.parts == 1;
@@ -289,19 +292,19 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     } else if (PARTS && has_row && steps > 0) {
 #pragma unroll
                         for (int u = 0; u < 32; u += 4)
-                            *reinterpret_cast<uint4*>(slot + ((i + u) / 4 * 2 * kPrRows + r) * 4) = make_uint4(o[u], o[u + 1], o[u + 2], o[u + 3]);
+                            *reinterpret_cast<uint4*>(slot + ((i + u) / 4 * 2 * kPrRows + slot_row) * 4) = make_uint4(o[u], o[u + 1], o[u + 2], o[u + 3]);
                     }
                 }
             if (PARTS && !whole) {
                 if (has_row) {
-                    slot[2 * kPrRows * HD + r] = m2;
-                    slot[2 * kPrRows * (HD + 1) + r] = sum;      // (0: the columns say nothing)
+                    slot[2 * kPrRows * HD + slot_row] = m2;
+                    slot[2 * kPrRows * (HD + 1) + slot_row] = sum;      // (0: the columns say nothing)
                 }
                 if (tid == 0) slot[2 * kPrRows * (HD + 2)] = again ? 1.f : 0.f;
             }
             tc_fence_before();       // O has been read before the next rows' P is handed on
             if (again && whole)
-                for (int i = 0; i < 1 << p.pack; ++i) prompt_rows<__nv_bfloat16>(p.a, it, p.pack ? (x.h << p.pack) + i : x.h, warp, 8);
+                for (int i = 0; i < p.pack; ++i) prompt_rows<__nv_bfloat16>(p.a, it, x.h * p.pack + i, warp, 8);
             done_work(w);
         }
     } else {
@@ -335,7 +338,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 }
                 if (it.rows == 0) break;
                 if (PARTS && lane == 0 && share < 1 << 30) p.list[item] = it;
-                const int n = max(steps_of(it, 0), steps_of(it, 1)), hkv = p.pack ? x.h : x.h / p.a.group;
+                const int n = max(steps_of(it, 0), steps_of(it, 1)), hkv = p.pack > 1 ? x.h : x.h / p.a.group;
                 // rows of a tile's boxes, a lane each (-1: behind the last key, -2: no page), looked up a tile ahead
                 auto rows_at = [&](int j) {
                     const int pos = (it.j0 + j) * kPrRows + lane * p.box;
@@ -349,10 +352,10 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     if (!ok) break;
                     ++cq;
                     if (lane == 0) {
-                        mbar_expect_tx(qfull, (uint32_t)(p.tiles * TILE));
+                        mbar_expect_tx(qfull, (uint32_t)(p.tiles * p.rpt * p.pack * HD * 2));
                         for (int t = 0; t < p.tiles; ++t)
                             for (int c = 0; c < Sh::blks; ++c)
-                                tma_load_4d(sq + t * TILE + c * BLK, &qmap, c * 64, p.pack ? 0 : x.h % p.a.group, hkv, (int)it.row + ((t * kPrRows) >> p.pack), qfull);
+                                tma_load_4d(sq + t * TILE + c * BLK, &qmap, c * 64, p.pack > 1 ? 0 : x.h % p.a.group, hkv, (int)it.row + t * p.rpt, qfull);
                     }
                 }
                 for (int j = 0; j < n && ok; ++j) {
@@ -547,13 +550,14 @@ prompt_join_kernel(const PromptParams p) {
     for (int q = 0; q < kMaxParts; ++q) again |= __ldcg(from + min(q, it.parts - 1) * step + R * (HD + 2)) != 0.f;
     if (again) {
         if (slice == 0)
-            for (int i = 0; i < 1 << p.pack; ++i) prompt_rows<__nv_bfloat16>(p.a, it, p.pack ? (h << p.pack) + i : h, tid >> 5, 8);
+            for (int i = 0; i < p.pack; ++i) prompt_rows<__nv_bfloat16>(p.a, it, h * p.pack + i, tid >> 5, 8);
         continue;
     }
     // eight columns of a row per thread: rows side by side
-    const int rows = it.rows << p.pack, pieces = p.a.head_dim / 8, mine = (pieces - slice + kJoinSlices - 1) / kJoinSlices;
+    const int rows = it.rows * p.pack, pieces = p.a.head_dim / 8, mine = (pieces - slice + kJoinSlices - 1) / kJoinSlices;
     for (int e = tid; e < rows * mine; e += 256) {
-        const int x = e / rows, r = e - x * rows, i = x * kJoinSlices + slice;
+        const int x = e / rows, y = e - x * rows, i = x * kJoinSlices + slice, row = y / p.pack, t = row / p.rpt;
+        const int r = t * (kPrRows - p.rpt * p.pack) + y;      // (the tile's rows that hold none left out)
         float top = -INFINITY, total = 0.f, a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int q0 = 0; q0 < it.parts; q0 += 4) {
@@ -589,8 +593,7 @@ prompt_join_kernel(const PromptParams p) {
             }
         }
         const float inv = total == 0.f ? 0.f : 1.f / total;
-        const int head = p.pack ? (h << p.pack) + (r & ((1 << p.pack) - 1)) : h;
-        *reinterpret_cast<uint4*>((__nv_bfloat16*)p.a.out + ((it.row + (r >> p.pack)) * p.a.n_q + head) * p.a.head_dim + 8 * i) =
+        *reinterpret_cast<uint4*>((__nv_bfloat16*)p.a.out + ((it.row + row) * p.a.n_q + h * p.pack + y - row * p.pack) * p.a.head_dim + 8 * i) =
             make_uint4(bf16_pair(a[0] * inv, a[1] * inv), bf16_pair(a[2] * inv, a[3] * inv), bf16_pair(a[4] * inv, a[5] * inv), bf16_pair(a[6] * inv, a[7] * inv));
     }
     }
@@ -608,13 +611,13 @@ int32_t prompt_configure(DeviceState& ds) {
     return RSTQ_OK;
 }
 
-// q as [rows][n_kv][group][head_dim], in boxes of 128 rows of a tile
-static int32_t prompt_q_map(CUtensorMap* m, const PromptArgs& a, int heads) {
+// q as [rows][n_kv][group][head_dim], in boxes of a tile's rows
+static int32_t prompt_q_map(CUtensorMap* m, const PromptArgs& a, int heads, int rows) {
     const EncodeTiledFn enc = encode_tiled_fn();
     RSTQ_REQUIRE(enc, RSTQ_E_CUDA, "cuTensorMapEncodeTiled is not available");
     const cuuint64_t dims[4] = {(cuuint64_t)a.head_dim, (cuuint64_t)a.group, (cuuint64_t)a.n_kv, (cuuint64_t)a.rows};
     const cuuint64_t strides[3] = {(cuuint64_t)a.head_dim * 2, (cuuint64_t)a.group * a.head_dim * 2, (cuuint64_t)a.ldq * 2};
-    const cuuint32_t box[4] = {64u, (cuuint32_t)heads, 1u, (cuuint32_t)(kPrRows / heads)}, ones[4] = {1u, 1u, 1u, 1u};
+    const cuuint32_t box[4] = {64u, (cuuint32_t)heads, 1u, (cuuint32_t)rows}, ones[4] = {1u, 1u, 1u, 1u};
     const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(a.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     RSTQ_REQUIRE(r == CUDA_SUCCESS, RSTQ_E_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
@@ -628,18 +631,20 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     p.status = ds.status;
     p.sectors = ((uintptr_t)a.out & 31) == 0 && a.head_dim % 16 == 0;
     p.box = a.kv.table ? std::min(1 << a.kv.shift, kPrRows) : kPrRows;
-    // Heads of a group that is a power of two share a tile: its K and V are read once for all of them, and few rows fill it.
-    p.pack = a.group > 1 && a.group <= kPrRows && (a.group & (a.group - 1)) == 0 ? log2_of(a.group) : 0;
-    p.heads = p.pack ? a.n_kv : a.n_q;
+    // A group's heads share a tile where they fill seven eighths of its rows: its K and V are read once for all of them, few rows fill it, and
+    // less of a prompt's tiles lies above the diagonal.
+    p.pack = kPrRows / a.group * a.group >= kPrRows / 8 * 7 ? a.group : 1;
+    p.rpt = kPrRows / p.pack;
+    p.heads = a.n_q / p.pack;
     // Two query tiles per block keep the tensor core busy; with fewer blocks than SMs one each does the rows sooner.
     p.tiles = a.rows * a.n_q <= kPrRows * (int64_t)ds.sm_count ? 1 : 2;
     // Few blocks of rows that may see many keys (a cache, or more keys than rows): these are cut into parts, which a second launch joins.
     // (A sequence's rows of more than a tile then take two as well: there is no lack of parts.)
     const int64_t keys = a.kv.table ? (int64_t)a.kv.width << a.kv.shift : a.kv_rows > a.rows ? a.kv_rows : 0, some = std::min<int64_t>(a.seqs, a.rows);
-    const int tiles = a.rows << p.pack > kPrRows * some ? 2 : 1;
-    const bool parts = keys > 8 * kPrRows && (a.rows / ((tiles * kPrRows) >> p.pack) + some) * p.heads <= ds.sm_count;
+    const int tiles = a.rows > p.rpt * some ? 2 : 1;
+    const bool parts = keys > 8 * kPrRows && (a.rows / (tiles * p.rpt) + some) * p.heads <= ds.sm_count;
     if (parts) p.tiles = tiles;
-    const int per = (p.tiles * kPrRows) >> p.pack;
+    const int per = p.tiles * p.rpt;
     const int64_t blocks = (a.rows / per + some) * p.heads;     // no sequence has more than this of them
     RSTQ_REQUIRE(blocks < (1ll << 31), RSTQ_E_LIMIT, "%lld thread blocks", (long long)blocks);
     p.sms = std::min(ds.sm_count, kPromptSlots / kPartRounds);
@@ -648,7 +653,7 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     p.list = (PromptItem*)(ds.prompt_slots + (int64_t)kPromptSlots * prompt_slot<128>());
     p.listed = (int*)(p.list + kPromptSlots);
     CUtensorMap qmap, kmap, vmap;
-    int32_t rc = prompt_q_map(&qmap, a, 1 << p.pack);
+    int32_t rc = prompt_q_map(&qmap, a, p.pack, p.rpt);
     if (rc == RSTQ_OK) rc = rows_tensor_map(&kmap, a.k, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc == RSTQ_OK) rc = rows_tensor_map(&vmap, a.v, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc != RSTQ_OK) return rc;

@@ -420,3 +420,23 @@ def test_decode_of_many_sequences(ctx, dtype, seqs):
     bq.free()
     bo.free()
     p.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q,n_kv,d,page,lens,new", [
+    (14, 2, 128, 16, [200, 37, 19, 18, 0, 1], [200, 37, 19, 2, 0, 1]),         # 18 rows of 7 heads in a tile, two rows of it empty
+    (10, 2, 64, 32, [130, 52], [130, 26]),
+    (12, 1, 96, 16, [60, 21], [60, 11]),
+    (9, 1, 128, 64, [1500, 800], [30, 29]),                                    # keys in parts
+    (7, 1, 64, 16, [1200, 2000, 40], [2, 100, 40]),
+    (43, 1, 64, 16, [40], [9]),                                                # a group that would leave a third of a tile empty
+    (64, 1, 128, 16, [70, 5], [5, 3]),
+    (128, 1, 64, 16, [30], [4]),
+    (130, 1, 64, 16, [30], [3]),
+])
+def test_groups_that_share_a_tile(ctx, n_q, n_kv, d, page, lens, new):
+    x = Prompts(ctx, "bf16", n_q, n_kv, d, page, lens, new, seed=n_q)
+    x.call()
+    ctx.sync()
+    x.check()
+    x.free()
