@@ -6,6 +6,9 @@
 
 namespace rstq {
 
+// Heads of a group that share a query tile of 128 rows, (row of q, head) with the head innermost: all of them where they fill seven eighths of it.
+inline int prompt_pack(int group) { return 128 / group * group >= 112 ? group : 1; }
+
 constexpr float kGrow = 8.f;         // log2 of how far a row's largest weight may go beyond 1
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {

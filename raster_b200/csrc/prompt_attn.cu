@@ -631,9 +631,7 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     p.status = ds.status;
     p.sectors = ((uintptr_t)a.out & 31) == 0 && a.head_dim % 16 == 0;
     p.box = a.kv.table ? std::min(1 << a.kv.shift, kPrRows) : kPrRows;
-    // A group's heads share a tile where they fill seven eighths of its rows: its K and V are read once for all of them, few rows fill it, and
-    // less of a prompt's tiles lies above the diagonal.
-    p.pack = kPrRows / a.group * a.group >= kPrRows / 8 * 7 ? a.group : 1;
+    p.pack = prompt_pack(a.group);
     p.rpt = kPrRows / p.pack;
     p.heads = a.n_q / p.pack;
     // Two query tiles per block keep the tensor core busy; with fewer blocks than SMs one each does the rows sooner.

@@ -8,7 +8,7 @@
 // another: the tensor core's additions lose a little each, and so only every sixth counts (1000 keys: 3e-7 of the result,
 // against 2e-6 with one sum).  f32 FMAs would be bound by 72 TFLOP/s of the whole device, the six MMAs by a sixth of bf16's rate.
 //
-// A block has 128 query rows of one sequence and head.  Four warps fetch K and V, a tile of 64 keys at a time and one ahead in
+// A block has a tile of 128 (row, head) pairs of one sequence: rows of a head, or rows of all heads of a group as in prompt_attn.cu.  Four warps fetch K and V, a tile of 64 keys at a time and one ahead in
 // registers, split them and write the terms to shared memory, swizzled as the tensor core wants them (zeros behind the last key);
 // four warps are the softmax, a thread per row, P's three terms over S in tensor memory; one thread issues.  There are two places for S and
 // P, and the next tile's S is formed while this one's exponentials are.  (Of 64 columns two blocks with one place each would fit an SM: two
@@ -34,6 +34,8 @@ struct PromptShapeF {
 
 struct PromptParamsF {
     PromptArgs a;
+    int pack, rpt, heads;            // heads of a group that share a tile (1: none), rows of q of a tile, blocks per rows of a tile
+    int over_pack;                   // 2^16 / pack, rounded up: x / pack = x * over_pack >> 16 for x < 128 (off by less than 128 / 2^16 < 1 / pack)
     float scale2;
     int* status;
 };
@@ -63,7 +65,7 @@ prompt_f32_kernel(const PromptParamsF p) {
     const uint32_t qfull = smem_u32(s_bar), kfull = qfull + 8, kfree = qfull + 16, vfull = qfull + 24, vfree = qfull + 32, sfull = qfull + 40,
                    pfull = qfull + 56, odone = qfull + 72, over = qfull + 80;
     volatile int* abort_flag = &s_abort;
-    const int h = blockIdx.x % p.a.n_q, hkv = h / p.a.group;
+    const int h = blockIdx.x % p.heads, hkv = p.pack > 1 ? h : h / p.a.group;      // query head, or the packed ones' KV head
     if (tid == 0) {
         s_abort = s_again = 0;
         mbar_init(qfull, 4);
@@ -86,7 +88,7 @@ prompt_f32_kernel(const PromptParamsF p) {
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp == 0) {
-        const PromptItem it = prompt_block(p.a, kPfRows, kPfKeys, blockIdx.x / p.a.n_q);
+        const PromptItem it = prompt_block(p.a, p.rpt, kPfKeys, blockIdx.x / p.heads);
         if (lane == 0) s_item = it;
     }
     tc_fence_before();
@@ -103,7 +105,7 @@ prompt_f32_kernel(const PromptParamsF p) {
     if (warp < 4) {
         // ---- softmax: a thread per row ----
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-        const int r = warp * 32 + lane, mine = sees(r), least = sees(0);
+        const int rt = warp * 32 + lane, r = rt * p.over_pack >> 16, head = h * p.pack + rt - r * p.pack, mine = sees(r), least = sees(0);
         float m = -INFINITY, m2 = 0.f, sum = 0.f;
         bool ok = true;
         for (int j = 0; j < n; ++j) {
@@ -192,7 +194,8 @@ prompt_f32_kernel(const PromptParamsF p) {
         // (s_again is set before the terms it is about are handed on, and the last product came after all of them)
         if (ok && !*(volatile int*)&s_again) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            float* out = (float*)p.a.out + ((it.row + r) * p.a.n_q + h) * p.a.head_dim;
+            const bool has_row = rt < p.rpt * p.pack && r < it.rows;
+            float* out = (float*)p.a.out + ((it.row + r) * p.a.n_q + head) * p.a.head_dim;
 #pragma unroll
             for (int c = 0; c < HD; c += 16) {
                 uint32_t a[16], b[16];
@@ -201,7 +204,7 @@ prompt_f32_kernel(const PromptParamsF p) {
                     tmem_ld16(tO + lanes + HD + c, b);
                     tmem_ld_wait();
                 }
-                if (r < it.rows)
+                if (has_row)
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
                         if (c + i >= p.a.head_dim) continue;
@@ -212,7 +215,8 @@ prompt_f32_kernel(const PromptParamsF p) {
                     }
             }
         }
-        if (ok && *(volatile int*)&s_again) prompt_rows<float>(p.a, it, h, warp, 4);
+        if (ok && *(volatile int*)&s_again)
+            for (int i = 0; i < p.pack; ++i) prompt_rows<float>(p.a, it, h * p.pack + i, warp, 4);
     } else if (warp < 8) {
         // ---- split ----
         constexpr int LPR = HD / 4, RPI = 32 / LPR, NI = 16 / RPI;      // lanes of a row; rows of a load; loads of a warp's 16 rows
@@ -274,13 +278,13 @@ prompt_f32_kernel(const PromptParamsF p) {
                 float4 x[NI];
 #pragma unroll
                 for (int i = 0; i < NI; ++i) {
-                    const int row = w * 32 + half * 16 + i * RPI + sub;
-                    x[i] = *reinterpret_cast<const float4*>((const float*)p.a.q + (it.row + min(row, it.rows - 1)) * p.a.ldq + (int64_t)h * p.a.head_dim + din);
+                    const int rt = w * 32 + half * 16 + i * RPI + sub, row = rt * p.over_pack >> 16, head = h * p.pack + rt - row * p.pack;
+                    x[i] = *reinterpret_cast<const float4*>((const float*)p.a.q + (it.row + min(row, it.rows - 1)) * p.a.ldq + (int64_t)head * p.a.head_dim + din);
                 }
 #pragma unroll
                 for (int i = 0; i < NI; ++i) {
-                    const int row = w * 32 + half * 16 + i * RPI + sub;
-                    write(sq, Sh::qplane, Sh::qblk, row, only(in && row < it.rows, x[i]));
+                    const int rt = w * 32 + half * 16 + i * RPI + sub;
+                    write(sq, Sh::qplane, Sh::qblk, rt, only(in && rt < it.rows * p.pack, x[i]));
                 }
             }
             hand(qfull);
@@ -377,11 +381,15 @@ int32_t launch_prompt_f32(DeviceState& ds, const PromptArgs& a, int* launches) {
     p.a = a;
     p.scale2 = a.scale * 1.4426950408889634f;
     p.status = ds.status;
-    const int64_t blocks = (a.rows / kPfRows + std::min<int64_t>(a.seqs, a.rows)) * a.n_q;
+    p.pack = prompt_pack(a.group);
+    p.rpt = kPfRows / p.pack;
+    p.heads = a.n_q / p.pack;
+    p.over_pack = (65536 + p.pack - 1) / p.pack;
+    const int64_t blocks = (a.rows / p.rpt + std::min<int64_t>(a.seqs, a.rows)) * p.heads;
     RSTQ_REQUIRE(blocks < (1ll << 31), RSTQ_E_LIMIT, "%lld thread blocks", (long long)blocks);
     *launches = 1;
     if (a.seqs > kSumSeqs) {
-        const int32_t rc = launch_sums(ds, a, kPfRows, 0);
+        const int32_t rc = launch_sums(ds, a, p.rpt, 0);
         if (rc != RSTQ_OK) return rc;
         p.a.start = ds.seq_starts;
         ++*launches;

@@ -423,6 +423,7 @@ def test_decode_of_many_sequences(ctx, dtype, seqs):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("n_q,n_kv,d,page,lens,new", [
     (14, 2, 128, 16, [200, 37, 19, 18, 0, 1], [200, 37, 19, 2, 0, 1]),         # 18 rows of 7 heads in a tile, two rows of it empty
     (10, 2, 64, 32, [130, 52], [130, 26]),
@@ -434,8 +435,8 @@ def test_decode_of_many_sequences(ctx, dtype, seqs):
     (128, 1, 64, 16, [30], [4]),
     (130, 1, 64, 16, [30], [3]),
 ])
-def test_groups_that_share_a_tile(ctx, n_q, n_kv, d, page, lens, new):
-    x = Prompts(ctx, "bf16", n_q, n_kv, d, page, lens, new, seed=n_q)
+def test_groups_that_share_a_tile(ctx, dtype, n_q, n_kv, d, page, lens, new):
+    x = Prompts(ctx, dtype, n_q, n_kv, d, page, lens, new, seed=n_q)
     x.call()
     ctx.sync()
     x.check()
