@@ -6,6 +6,28 @@
 
 namespace rstq {
 
+// ---- keys cut into parts ----
+// What a part of a block of rows has found goes to its slot; a second launch joins the parts in their order.  (prompt_attn.cu)
+constexpr int kPromptSlots = 512;      // items of a call whose blocks' keys are cut into parts
+// a slot, in floats: up to 256 rows' sums, four columns at a time; their references; their sums of weights; whether they have to be taken again
+template <int HD>
+__host__ __device__ constexpr int prompt_slot() { return 256 * (HD + 2) + 32; }
+struct PromptItem;
+struct PromptJoin {
+    PromptArgs a;
+    int pack, rpt, heads;            // as the kernel that leaves the parts has them
+    float* part;                     // a slot per item
+    PromptItem* list;                // what each item was; their number, 0 where no block's keys are cut
+    int* listed;
+};
+PromptJoin prompt_join(DeviceState& ds, const PromptArgs& a, int pack, int rpt, int heads);
+int32_t launch_prompt_join(DeviceState& ds, const PromptJoin& j);
+// A call's rows may see more than `most` keys: a cache, or more keys than rows.
+inline bool prompt_may_part(const PromptArgs& a, int most) {
+    const int64_t keys = a.kv.table ? (int64_t)a.kv.width << a.kv.shift : a.kv_rows > a.rows ? a.kv_rows : 0;
+    return keys > most;
+}
+
 // Heads of a group that share a query tile of 128 rows, (row of q, head) with the head innermost: all of them where they fill seven eighths of it.
 inline int prompt_pack(int group) { return 128 / group * group >= 112 ? group : 1; }
 
@@ -157,6 +179,7 @@ struct PromptItem {
     }
 };
 constexpr int kMaxParts = 16, kPartRounds = 3;
+inline int prompt_sms(const DeviceState& ds) { return ds.sm_count < kPromptSlots / kPartRounds ? ds.sm_count : kPromptSlots / kPartRounds; }
 // One lane's sequence cut into blocks of `per` rows, and the tiles of `tile` keys that block k sees.
 struct PromptSequence {
     int n, keys, row0, first, blocks;
@@ -199,8 +222,9 @@ static __device__ __forceinline__ int prompt_items(const PromptArgs& a, int per,
 }
 // How many tiles of keys a part should have; all (no parts, *total = 0) where that is sooner done.  `sms` blocks of threads take the items in
 // rounds: for one, two and three of them the shortest parts that do not need another, and of these and of whole blocks what takes the
-// fewest tiles one after the other.  An item costs about two tiles beside its own, the joining launch three; parts of fewer than four tiles are not made.  heads: items per block of rows.
-static __device__ __forceinline__ int prompt_share(const PromptArgs& a, int per, int tile, int heads, int sms, int* total) {
+// fewest tiles one after the other.  item, join: what an item costs beside its tiles and what the joining launch does, in tiles.  Parts of
+// fewer than four tiles are not made.  heads: items per block of rows.
+static __device__ __forceinline__ int prompt_share(const PromptArgs& a, int per, int tile, int heads, int sms, int item, int join, int* total) {
     const int lane = threadIdx.x & 31;
     float all = 0.f;       // (sums of integers below 2^24, or large enough not to matter)
     int longest = 0, blocks = 0;
@@ -216,12 +240,12 @@ static __device__ __forceinline__ int prompt_share(const PromptArgs& a, int per,
         blocks = min(blocks + __reduce_add_sync(0xffffffffu, min(q.blocks, 1 << 20)), 1 << 25);
     }
     int best = 1 << 30, items = 0;
-    int64_t cost = ((int64_t)blocks * heads + sms - 1) / sms * (longest + 2);
+    int64_t cost = ((int64_t)blocks * heads + sms - 1) / sms * (longest + item);
     for (int rounds = 1; rounds <= kPartRounds; ++rounds) {
         const int most = rounds * sms / heads;
         int share = (int)fminf(fmaxf(ceilf(all * (float)heads / (float)(rounds * sms)), 4.f), 1e6f);
         for (int tries = 0; tries < 6; ++tries, share += (share >> 3) + 1) {
-            const int64_t now = (int64_t)rounds * (share + 2) + 3;
+            const int64_t now = (int64_t)rounds * (share + item) + join;
             if (now >= cost) break;
             const int n = prompt_items(a, per, tile, share, most);
             if (n > most) continue;

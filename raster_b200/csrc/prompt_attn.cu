@@ -47,8 +47,6 @@ struct PromptShape {
     static constexpr int smem = 1024 + (2 + stages) * tile;
 };
 
-constexpr int kPromptSlots = 512;      // items of a call whose blocks' keys are cut into parts
-
 struct PromptParams {
     PromptArgs a;
     int tiles;                       // query tiles of a block: 1 or 2
@@ -60,9 +58,7 @@ struct PromptParams {
     int sectors;                     // the rows of out begin on 32-byte boundaries, and so do their pieces of 16 columns
     float scale2;
     int* status;
-    float* part;                     // a slot per item: what a part of a block has found
-    PromptItem* list;                // ... and what the item was; their number, 0 where no block's keys are cut
-    int* listed;
+    PromptJoin join;                 // where the parts of a block's keys go
     int* counters;                   // [0] items dealt out beyond the first of every block, [1] blocks that are done: zero between launches
 };
 // what a warp has to know of a block of rows
@@ -71,10 +67,6 @@ struct PromptWork {
     int h;                           // query head, or the packed ones' KV head
     int item;
 };
-// a slot, in floats: 256 rows' sums, four columns at a time; their references; their sums of weights; whether they have to be taken again
-template <int HD>
-__host__ __device__ constexpr int prompt_slot() { return 2 * kPrRows * (HD + 2) + 32; }
-
 // PARTS: a block's keys may be cut into parts.
 template <int HD, bool PARTS>
 __global__ void __launch_bounds__(kPrThreads, 1)
@@ -141,8 +133,8 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     if (warp == 8) {
         if (PARTS) {
             int items;
-            share = prompt_share(p.a, per, kPrRows, p.heads, p.sms, &items);
-            if (blockIdx.x == 0 && lane == 0) *p.listed = items;
+            share = prompt_share(p.a, per, kPrRows, p.heads, p.sms, 2, 3, &items);      // (a step 2 us)
+            if (blockIdx.x == 0 && lane == 0) *p.join.listed = items;
         }
         first = PARTS ? prompt_item(p.a, per, kPrRows, share, blockIdx.x / p.heads) : prompt_block(p.a, per, kPrRows, blockIdx.x / p.heads);
     }
@@ -269,7 +261,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             // (a part of a block's keys: what it has found goes to its slot, for prompt_join_kernel)
             const bool whole = !PARTS || it.parts == 1;
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            float* slot = p.part + (whole ? 0 : (int64_t)x.item * prompt_slot<HD>());
+            float* slot = p.join.part + (whole ? 0 : (int64_t)x.item * prompt_slot<HD>());
             if (!whole || !again)
 #pragma unroll
                 for (int i = 0; i < HD; i += 32) {
@@ -337,7 +329,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     mbar_arrive(wfull + 8 * (w & 1));
                 }
                 if (it.rows == 0) break;
-                if (PARTS && lane == 0 && share < 1 << 30) p.list[item] = it;
+                if (PARTS && lane == 0 && share < 1 << 30) p.join.list[item] = it;
                 const int n = max(steps_of(it, 0), steps_of(it, 1)), hkv = p.pack > 1 ? x.h : x.h / p.a.group;
                 // rows of a tile's boxes, a lane each (-1: behind the last key, -2: no page), looked up a tile ahead
                 auto rows_at = [&](int j) {
@@ -531,12 +523,13 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
 
 // The parts of a block joined, in their order: blocks of threads per item, a slice of the columns each, of which those of the first part do it.
 constexpr int kJoinSlices = 8;
-template <int HD>
+// R: rows of a block.
+template <typename T, int HD, int R>
 __global__ void __launch_bounds__(256, 3)
-prompt_join_kernel(const PromptParams p) {
+prompt_join_kernel(const PromptJoin p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    constexpr int SLOT = prompt_slot<HD>(), R = 2 * kPrRows;
+    constexpr int SLOT = prompt_slot<HD>();
     const int tid = threadIdx.x, all = *p.listed * kJoinSlices;
     for (int job = blockIdx.x; job < all; job += gridDim.x) {
     const int item = job / kJoinSlices, slice = job - item * kJoinSlices;
@@ -550,14 +543,14 @@ prompt_join_kernel(const PromptParams p) {
     for (int q = 0; q < kMaxParts; ++q) again |= __ldcg(from + min(q, it.parts - 1) * step + R * (HD + 2)) != 0.f;
     if (again) {
         if (slice == 0)
-            for (int i = 0; i < p.pack; ++i) prompt_rows<__nv_bfloat16>(p.a, it, h * p.pack + i, tid >> 5, 8);
+            for (int i = 0; i < p.pack; ++i) prompt_rows<T>(p.a, it, h * p.pack + i, tid >> 5, 8);
         continue;
     }
     // eight columns of a row per thread: rows side by side
     const int rows = it.rows * p.pack, pieces = p.a.head_dim / 8, mine = (pieces - slice + kJoinSlices - 1) / kJoinSlices;
     for (int e = tid; e < rows * mine; e += 256) {
         const int x = e / rows, y = e - x * rows, i = x * kJoinSlices + slice, row = y / p.pack, t = row / p.rpt;
-        const int r = t * (kPrRows - p.rpt * p.pack) + y;      // (the tile's rows that hold none left out)
+        const int r = t * (128 - p.rpt * p.pack) + y;      // (the tile's rows that hold none left out)
         float top = -INFINITY, total = 0.f, a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int q0 = 0; q0 < it.parts; q0 += 4) {
@@ -593,10 +586,35 @@ prompt_join_kernel(const PromptParams p) {
             }
         }
         const float inv = total == 0.f ? 0.f : 1.f / total;
-        *reinterpret_cast<uint4*>((__nv_bfloat16*)p.a.out + ((it.row + row) * p.a.n_q + h * p.pack + y - row * p.pack) * p.a.head_dim + 8 * i) =
-            make_uint4(bf16_pair(a[0] * inv, a[1] * inv), bf16_pair(a[2] * inv, a[3] * inv), bf16_pair(a[4] * inv, a[5] * inv), bf16_pair(a[6] * inv, a[7] * inv));
+        T* out = (T*)p.a.out + ((it.row + row) * p.a.n_q + h * p.pack + y - row * p.pack) * p.a.head_dim + 8 * i;
+        if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<uint4*>(out) = make_uint4(bf16_pair(a[0] * inv, a[1] * inv), bf16_pair(a[2] * inv, a[3] * inv), bf16_pair(a[4] * inv, a[5] * inv),
+                                                        bf16_pair(a[6] * inv, a[7] * inv));
+        else {
+            store4(out, make_float4(a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv));
+            store4(out + 4, make_float4(a[4] * inv, a[5] * inv, a[6] * inv, a[7] * inv));
+        }
     }
     }
+}
+
+PromptJoin prompt_join(DeviceState& ds, const PromptArgs& a, int pack, int rpt, int heads) {
+    PromptJoin j;
+    j.a = a;
+    j.pack = pack;
+    j.rpt = rpt;
+    j.heads = heads;
+    j.part = ds.prompt_slots;
+    j.list = (PromptItem*)(ds.prompt_slots + (int64_t)kPromptSlots * prompt_slot<128>());
+    j.listed = (int*)(j.list + kPromptSlots);
+    return j;
+}
+int32_t launch_prompt_join(DeviceState& ds, const PromptJoin& j) {
+    const dim3 grid((unsigned)(12 * ds.sm_count));
+    auto go = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(256), 0, ds, j); };
+    if (j.a.dtype == RSTQ_BF16) RSTQ_CUDA(j.a.head_dim <= 64 ? go(prompt_join_kernel<__nv_bfloat16, 64, 256>) : go(prompt_join_kernel<__nv_bfloat16, 128, 256>));
+    else RSTQ_CUDA(j.a.head_dim <= 64 ? go(prompt_join_kernel<float, 64, 128>) : go(prompt_join_kernel<float, 128, 128>));
+    return RSTQ_OK;
 }
 
 int32_t prompt_configure(DeviceState& ds) {
@@ -636,26 +654,24 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     p.heads = a.n_q / p.pack;
     // Two query tiles per block keep the tensor core busy; with fewer blocks than SMs one each does the rows sooner.
     p.tiles = a.rows * a.n_q <= kPrRows * (int64_t)ds.sm_count ? 1 : 2;
-    // Few blocks of rows that may see many keys (a cache, or more keys than rows): these are cut into parts, which a second launch joins.
-    // (A sequence's rows of more than a tile then take two as well: there is no lack of parts.)
-    const int64_t keys = a.kv.table ? (int64_t)a.kv.width << a.kv.shift : a.kv_rows > a.rows ? a.kv_rows : 0, some = std::min<int64_t>(a.seqs, a.rows);
+    // Few blocks of rows that may see many keys are cut into parts, which a second launch joins.  (A sequence's rows of more than a tile then
+    // take two as well: there is no lack of parts.)
+    const int64_t some = std::min<int64_t>(a.seqs, a.rows);
     const int tiles = a.rows > p.rpt * some ? 2 : 1;
-    const bool parts = keys > 8 * kPrRows && (a.rows / (tiles * p.rpt) + some) * p.heads <= ds.sm_count;
+    const bool parts = prompt_may_part(a, 1024) && (a.rows / (tiles * p.rpt) + some) * p.heads <= ds.sm_count;
     if (parts) p.tiles = tiles;
     const int per = p.tiles * p.rpt;
     const int64_t blocks = (a.rows / per + some) * p.heads;     // no sequence has more than this of them
     RSTQ_REQUIRE(blocks < (1ll << 31), RSTQ_E_LIMIT, "%lld thread blocks", (long long)blocks);
-    p.sms = std::min(ds.sm_count, kPromptSlots / kPartRounds);
+    p.sms = prompt_sms(ds);
     p.bound = parts ? 1 << 30 : (int)blocks;
-    p.part = ds.prompt_slots;
-    p.list = (PromptItem*)(ds.prompt_slots + (int64_t)kPromptSlots * prompt_slot<128>());
-    p.listed = (int*)(p.list + kPromptSlots);
+    p.join = prompt_join(ds, a, p.pack, p.rpt, p.heads);
     CUtensorMap qmap, kmap, vmap;
     int32_t rc = prompt_q_map(&qmap, a, p.pack, p.rpt);
     if (rc == RSTQ_OK) rc = rows_tensor_map(&kmap, a.k, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc == RSTQ_OK) rc = rows_tensor_map(&vmap, a.v, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc != RSTQ_OK) return rc;
-    p.counters = p.listed + 4;
+    p.counters = p.join.listed + 4;
     *launches = parts ? 2 : 1;
     if (!parts && a.seqs > kSumSeqs) {
         if ((rc = launch_sums(ds, a, per, 0)) != RSTQ_OK) return rc;
@@ -666,11 +682,7 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     auto go = [&](auto kernel, int smem) { return launch_pdl(kernel, grid, dim3(kPrThreads), (size_t)smem, ds, p, qmap, kmap, vmap); };
     if (a.head_dim <= 64) RSTQ_CUDA(parts ? go(prompt_kernel<64, true>, PromptShape<64>::smem) : go(prompt_kernel<64, false>, PromptShape<64>::smem));
     else RSTQ_CUDA(parts ? go(prompt_kernel<128, true>, PromptShape<128>::smem) : go(prompt_kernel<128, false>, PromptShape<128>::smem));
-    if (parts) {
-        const dim3 join((unsigned)(12 * ds.sm_count));
-        RSTQ_CUDA(a.head_dim <= 64 ? launch_pdl(prompt_join_kernel<64>, join, dim3(256), 0, ds, p) : launch_pdl(prompt_join_kernel<128>, join, dim3(256), 0, ds, p));
-    }
-    return RSTQ_OK;
+    return parts ? launch_prompt_join(ds, p.join) : RSTQ_OK;
 }
 
 }  // namespace rstq

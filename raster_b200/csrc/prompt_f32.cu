@@ -15,6 +15,9 @@
 // sequences of 1000 rows 63 us, against 46.)  A step of 64 keys takes 1.7 us with 64 columns, 3.7 with 128, of which the MMAs are 1 and 2
 // (an MMA of S is bound by reading Q and K from shared memory, 48 cycles): the rest is the way from S through the softmax to P V and, with
 // 128, V's terms, which wait for the last product with V.  1024 rows of 16 heads: 37 and 67 us.
+// Few blocks that see many keys are cut into parts as in prompt_attn.cu: 2 rows behind 4000 keys of 8 heads of 128 212 -> 45 us, 300 of 64 columns
+// 129 -> 50.
+//
 // An infinity or NaN has no such terms: a block that meets one (in keys or values its rows may not even see) computes its rows one by one
 // (attend_row), and so does one whose table names no page.
 #include <algorithm>
@@ -38,6 +41,8 @@ struct PromptParamsF {
     int over_pack;                   // 2^16 / pack, rounded up: x / pack = x * over_pack >> 16 for x < 128 (off by less than 128 / 2^16 < 1 / pack)
     float scale2;
     int* status;
+    int sms;                         // blocks that run at once
+    PromptJoin join;                 // where the parts of a block's keys go
 };
 
 // The next eight bits of a pair of values, as bf16 pair; the values become what is left.
@@ -47,7 +52,8 @@ __device__ __forceinline__ uint32_t next_term(float& a, float& b) {
     return w;
 }
 
-template <int HD>
+// PARTS: a block's keys may be cut into parts.
+template <int HD, bool PARTS>
 __global__ void __launch_bounds__(kPfThreads, 1)
 prompt_f32_kernel(const PromptParamsF p) {
     using Sh = PromptShapeF<HD>;
@@ -88,7 +94,16 @@ prompt_f32_kernel(const PromptParamsF p) {
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp == 0) {
-        const PromptItem it = prompt_block(p.a, p.rpt, kPfKeys, blockIdx.x / p.heads);
+        PromptItem it;
+        if (PARTS) {
+            int items;
+            const int share = prompt_share(p.a, p.rpt, kPfKeys, p.heads, p.sms, HD == 64 ? 5 : 3, HD == 64 ? 8 : 4, &items);      // (a block's begin and end 8 us)
+            it = prompt_item(p.a, p.rpt, kPfKeys, share, blockIdx.x / p.heads);
+            if (lane == 0) {
+                if (blockIdx.x == 0) *p.join.listed = items;
+                if ((int)blockIdx.x < items) p.join.list[blockIdx.x] = it;
+            }
+        } else it = prompt_block(p.a, p.rpt, kPfKeys, blockIdx.x / p.heads);
         if (lane == 0) s_item = it;
     }
     tc_fence_before();
@@ -97,9 +112,10 @@ prompt_f32_kernel(const PromptParamsF p) {
     const uint32_t tmem = (uint32_t)uniform((int)s_tmem);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // (not before this block has its tensor memory)
     const PromptItem it = s_item;
-    const int see0 = p.a.causal ? it.keys - it.behind + 1 : it.keys, grow = p.a.causal;      // row r sees the first see0 + r keys
-    auto sees = [&](int r) { return min(max(see0 + grow * r, 0), it.keys); };
-    const int n = uniform(it.rows > 0 ? (sees(it.rows - 1) + kPfKeys - 1) / kPfKeys : 0);
+    const int key0 = PARTS && it.rows > 0 ? it.j0 * kPfKeys : 0;      // the part's first key
+    auto sees = [&](int r) { return it.sees(r, p.a.causal) - key0; };     // keys that row r sees, from there
+    const int n = uniform(it.rows > 0 ? it.j1 - (PARTS ? it.j0 : 0) : 0);      // (the last row's tiles)
+    const bool whole = !PARTS || it.rows == 0 || it.parts == 1;
     const uint32_t tO = tmem + NB * 128;
 
     if (warp < 4) {
@@ -192,7 +208,28 @@ prompt_f32_kernel(const PromptParamsF p) {
         if (ok && n > 0) ok = wait_phase(odone, (n - 1) & 1, abort_flag);
         tc_fence_after();
         // (s_again is set before the terms it is about are handed on, and the last product came after all of them)
-        if (ok && !*(volatile int*)&s_again) {
+        const bool again = *(volatile int*)&s_again;
+        if (ok && !whole) {
+            // a part: sums, reference and sum of weights to its slot
+            float* slot = p.join.part + (int64_t)blockIdx.x * prompt_slot<HD>();
+            if (rt < p.rpt * p.pack && r < it.rows) {
+                slot[kPfRows * HD + rt] = m2;
+                slot[kPfRows * (HD + 1) + rt] = sum;
+            }
+            if (tid == 0) slot[kPfRows * (HD + 2)] = again ? 1.f : 0.f;
+#pragma unroll
+            for (int c = 0; c < HD; c += 16) {
+                uint32_t a[16], b[16];
+                tmem_ld16(tO + lanes + c, a);
+                tmem_ld16(tO + lanes + HD + c, b);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    auto x = [&](int e) { return __uint_as_float(a[i + e]) + __uint_as_float(b[i + e]); };
+                    store4(slot + ((c + i) / 4 * kPfRows + rt) * 4, make_float4(x(0), x(1), x(2), x(3)));
+                }
+            }
+        } else if (ok && !again) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const bool has_row = rt < p.rpt * p.pack && r < it.rows;
             float* out = (float*)p.a.out + ((it.row + r) * p.a.n_q + head) * p.a.head_dim;
@@ -215,7 +252,7 @@ prompt_f32_kernel(const PromptParamsF p) {
                     }
             }
         }
-        if (ok && *(volatile int*)&s_again)
+        if (ok && whole && again)
             for (int i = 0; i < p.pack; ++i) prompt_rows<float>(p.a, it, h * p.pack + i, warp, 4);
     } else if (warp < 8) {
         // ---- split ----
@@ -243,7 +280,7 @@ prompt_f32_kernel(const PromptParamsF p) {
         bool ok = n > 0;
         // this warp's 16 rows of a tile of K and V: their places, a lane each
         auto places = [&](int j) {
-            const int pos = j * kPfKeys + w * 16 + (lane & 15);
+            const int pos = key0 + j * kPfKeys + w * 16 + (lane & 15);
             int64_t row = -1;
             if (j < n && pos < it.keys) {
                 row = kv_row(p.a.kv, it.b, it.row0, pos);
@@ -371,8 +408,10 @@ prompt_f32_kernel(const PromptParamsF p) {
 
 int32_t prompt_f32_configure() {
     constexpr auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    RSTQ_CUDA(cudaFuncSetAttribute(prompt_f32_kernel<64>, attr, PromptShapeF<64>::smem));
-    RSTQ_CUDA(cudaFuncSetAttribute(prompt_f32_kernel<128>, attr, PromptShapeF<128>::smem));
+    RSTQ_CUDA(cudaFuncSetAttribute((prompt_f32_kernel<64, false>), attr, PromptShapeF<64>::smem));
+    RSTQ_CUDA(cudaFuncSetAttribute((prompt_f32_kernel<64, true>), attr, PromptShapeF<64>::smem));
+    RSTQ_CUDA(cudaFuncSetAttribute((prompt_f32_kernel<128, false>), attr, PromptShapeF<128>::smem));
+    RSTQ_CUDA(cudaFuncSetAttribute((prompt_f32_kernel<128, true>), attr, PromptShapeF<128>::smem));
     return RSTQ_OK;
 }
 
@@ -387,17 +426,21 @@ int32_t launch_prompt_f32(DeviceState& ds, const PromptArgs& a, int* launches) {
     p.over_pack = (65536 + p.pack - 1) / p.pack;
     const int64_t blocks = (a.rows / p.rpt + std::min<int64_t>(a.seqs, a.rows)) * p.heads;
     RSTQ_REQUIRE(blocks < (1ll << 31), RSTQ_E_LIMIT, "%lld thread blocks", (long long)blocks);
-    *launches = 1;
-    if (a.seqs > kSumSeqs) {
+    p.sms = prompt_sms(ds);
+    p.join = prompt_join(ds, a, p.pack, p.rpt, p.heads);
+    const bool parts = prompt_may_part(a, 768) && blocks <= p.sms;
+    *launches = parts ? 2 : 1;
+    if (!parts && a.seqs > kSumSeqs) {
         const int32_t rc = launch_sums(ds, a, p.rpt, 0);
         if (rc != RSTQ_OK) return rc;
         p.a.start = ds.seq_starts;
         ++*launches;
     }
-    const dim3 grid((unsigned)blocks), block(kPfThreads);
-    RSTQ_CUDA(a.head_dim <= 64 ? launch_pdl(prompt_f32_kernel<64>, grid, block, (size_t)PromptShapeF<64>::smem, ds, p)
-                               : launch_pdl(prompt_f32_kernel<128>, grid, block, (size_t)PromptShapeF<128>::smem, ds, p));
-    return RSTQ_OK;
+    const dim3 grid((unsigned)(parts ? kPartRounds * p.sms : blocks));
+    auto go = [&](auto kernel, int smem) { return launch_pdl(kernel, grid, dim3(kPfThreads), (size_t)smem, ds, p); };
+    if (a.head_dim <= 64) RSTQ_CUDA(parts ? go(prompt_f32_kernel<64, true>, PromptShapeF<64>::smem) : go(prompt_f32_kernel<64, false>, PromptShapeF<64>::smem));
+    else RSTQ_CUDA(parts ? go(prompt_f32_kernel<128, true>, PromptShapeF<128>::smem) : go(prompt_f32_kernel<128, false>, PromptShapeF<128>::smem));
+    return parts ? launch_prompt_join(ds, p.join) : RSTQ_OK;
 }
 
 }  // namespace rstq

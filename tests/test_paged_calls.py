@@ -60,6 +60,7 @@ class Prompts:
 CALLS = [("bf16", 8, 2, 128, 32, [300, 257, 40], [300, 130, 1]),
          ("bf16", 8, 2, 64, 16, [2600, 900, 1300], [3, 40, 2]),
          ("f32", 4, 2, 64, 16, [200, 130], [70, 130]),
+         ("f32", 8, 2, 128, 32, [1500, 700, 900], [3, 60, 2]),
          ("bf16", 2, 1, 256, 16, [90, 33], [20, 33])]
 
 
@@ -89,10 +90,11 @@ def test_a_prompt_call_in_a_graph(ctx, dtype, n_q, n_kv, d, page, lens, new):
 
 
 @pytest.mark.gpu
-def test_two_contexts_at_once():
+@pytest.mark.parametrize("case", [1, 3])
+def test_two_contexts_at_once(case):
     """Each with scratch of its own: calls under way together give what each gives alone."""
     both = [Context(("cuda:0",)) for _ in range(2)]
-    work = [Prompts(c, *CALLS[1], seed=s) for s, c in enumerate(both)]
+    work = [Prompts(c, *CALLS[case], seed=s) for s, c in enumerate(both)]
     alone = []
     for x in work:
         x.call()
@@ -158,7 +160,7 @@ def test_prompts_with_a_page_that_is_none(ctx, dtype, n_q, n_kv, d, page, lens, 
 
 @pytest.mark.gpu
 def test_launches_are_counted(ctx):
-    for case, launches in ((CALLS[0], 1), (CALLS[1], 2), (CALLS[2], 1), (CALLS[3], 1)):
+    for case, launches in ((CALLS[0], 1), (CALLS[1], 2), (CALLS[2], 1), (CALLS[3], 2), (CALLS[4], 1)):
         x = Prompts(ctx, *case)
         n = ctx.launch_count()
         x.call()
@@ -378,6 +380,44 @@ def test_a_pool_of_more_than_2_32_elements(ctx, d):
 
 
 # ---- many sequences -----------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,n_q,n_kv,d,page,lens,new", [
+    ("f32", 8, 2, 128, 32, [2500, 1100, 7, 1500], [2, 40, 7, 1]),
+    ("f32", 6, 2, 64, 16, [3000, 0, 1030], [5, 0, 30]),
+    ("f32", 2, 2, 96, 16, [1500, 200], [130, 3]),
+    ("f32", 4, 1, 128, 256, [4000], [1]),
+])
+def test_few_rows_behind_many_keys_in_f32(ctx, dtype, n_q, n_kv, d, page, lens, new):
+    x = Prompts(ctx, dtype, n_q, n_kv, d, page, lens, new)
+    x.call()
+    ctx.sync()
+    x.check()
+    x.free()
+
+
+@pytest.mark.gpu
+def test_parts_in_f32_with_values_that_are_not_numbers(ctx):
+    """An infinity that only the last row sees, one that all see, and nothing of the first in the others."""
+    n_q, d, page, n, rows = 4, 64, 32, 2600, 3
+    x = Prompts(ctx, "f32", n_q, 1, d, page, [n], [rows])
+    p = x.pool
+    v = p.v.copy()
+    at = lambda pos: (p.table[0, pos // page], pos % page)  # noqa: E731
+    v[at(n - 1)][0, 5] = np.inf
+    v[at(100)][0, 6] = -np.inf
+    p.bv.upload(v)
+    x.call()
+    ctx.sync()
+    got = x.raw().reshape(rows, n_q, d)
+    assert np.isneginf(got[:, :, 6]).all() and np.isposinf(got[2, :, 5]).all() and np.isfinite(got[:2, :, 5]).all()
+    keep = [i for i in range(d) if i not in (5, 6)]
+    for r in range(rows):
+        m = n - rows + r + 1
+        want, tol = pm.attention(x.q[r:r + 1], p.keys[0][:m], p.values[0][:m], x.scale, False, "f32")
+        close(got[r:r + 1][..., keep], want[..., keep], tol[..., keep], f"row {r}")
+    x.free()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,seqs", [("bf16", 65), ("bf16", 128), ("bf16", 129), ("bf16", 700), ("f32", 129), ("f32", 1100)])
 def test_prompts_of_many_sequences(ctx, dtype, seqs):
