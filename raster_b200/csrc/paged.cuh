@@ -274,7 +274,7 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches);
 int32_t launch_prompt_f32(DeviceState& ds, const PromptArgs& a, int* launches);
 // paged_attn.cu: any head_dim and length, a warp per position
 int32_t launch_attention_rows(DeviceState& ds, const PromptArgs& a);
-// paged_decode.cu: one row per sequence, paged, head_dim <= 128
+// paged_decode.cu: one row per sequence, paged
 int32_t launch_paged_decode(DeviceState& ds, const PromptArgs& a, int* launches);
 
 }  // namespace rstq

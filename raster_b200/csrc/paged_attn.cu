@@ -368,7 +368,7 @@ int32_t rstq_paged_decode_attention(rstq_ctx* ctx, rstq_buf* q, rstq_buf* kcache
     if (rc != RSTQ_OK) return rc;
     DeviceState& ds = ctx->devs[q->dev];
     int launches = 1;
-    rc = head_dim <= 128 ? launch_paged_decode(ds, a, &launches) : launch_attention_rows(ds, a);
+    rc = launch_paged_decode(ds, a, &launches);
     if (rc == RSTQ_OK) ctx->launches += launches;
     return rc;
 }

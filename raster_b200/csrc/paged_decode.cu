@@ -1,4 +1,4 @@
-// Attention of one new token per sequence over a paged cache, head_dim up to 128.
+// Attention of one new token per sequence over a paged cache.
 //
 //   out[b, h] = sum_j p_j V[b, j] / sum_j p_j,   p_j = exp(scale q.K[b, j] - m),   j < lens[b]
 //
@@ -34,13 +34,18 @@ namespace rstq {
 
 constexpr int kDecWarps = 4;                          // consumers; one more warp copies
 constexpr int kDecThreads = (kDecWarps + 1) * 32;
-constexpr int kDecRing = 80 * 1024;
-constexpr int kDecQ = 7 * 1024;                       // queries of the parts to come
+// Blocks per SM; bytes of the ring; bytes for the queries of the parts to come.  (Above 128 columns five stages and the sums take a whole SM.)
+template <int HD>
+__host__ __device__ constexpr int dec_blocks() { return HD > 128 ? 1 : 2; }
+template <int HD>
+__host__ __device__ constexpr int dec_ring() { return (HD > 128 ? 160 : 80) * 1024; }
+template <int HD>
+__host__ __device__ constexpr int dec_q() { return (HD > 128 ? 16 : 7) * 1024; }
 // the warps' sums, [warp][eight heads][HD + 4]: four floats of padding and a warp's stores meet no bank twice
 template <int HD>
 __host__ __device__ constexpr int dec_slab() { return 8 * (HD + 4); }
 template <int HD>
-__host__ __device__ constexpr int dec_smem() { return 1024 + kDecRing + kDecQ + kDecWarps * dec_slab<HD>() * 4; }
+__host__ __device__ constexpr int dec_smem() { return 1024 + dec_ring<HD>() + dec_q<HD>() + kDecWarps * dec_slab<HD>() * 4; }
 
 struct DecodeParams {
     const void *q, *k, *v;
@@ -221,12 +226,12 @@ __device__ __forceinline__ int64_t dec_find(const DecodeParams& p, int H, Walk* 
 }
 // GH: query heads served at once (bf16: 8 or 16; f32: what the group needs)
 template <typename T, int HD, int GH>
-__global__ void __launch_bounds__(kDecThreads, 2)
+__global__ void __launch_bounds__(kDecThreads, dec_blocks<HD>())
 paged_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-    constexpr int TILE = dec_tile<T>(), G16 = TILE / 16, STAGE = dec_stage<T, HD>(), NST = kDecRing / STAGE;
+    constexpr int TILE = dec_tile<T>(), G16 = TILE / 16, STAGE = dec_stage<T, HD>(), NST = dec_ring<HD>() / STAGE;
     constexpr int ES = (int)sizeof(T), BLKS = HD * ES / 128, BLK = TILE * 128;      // a tile's rows in pieces of 128 bytes: BLKS blocks
     constexpr bool BF = ES == 2;
-    constexpr int SLOT = dec_slot<HD>(), SLAB = dec_slab<HD>(), QB = GH * HD * ES, NQ = kDecQ / QB >= 4 ? 4 : kDecQ / QB;
+    constexpr int SLOT = dec_slot<HD>(), SLAB = dec_slab<HD>(), QB = GH * HD * ES, NQ = dec_q<HD>() / QB >= 4 ? 4 : dec_q<HD>() / QB;
     constexpr int PER = dec_heads<T>();               // query heads of a pass
     static_assert(NST >= 4 && NQ >= 1 && GH <= PER, "ring");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -239,8 +244,8 @@ paged_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap km
     __shared__ int4 s_open[2];                        // pairs of which the range has a part and not the whole: sequence, head, blocks
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t ring = smem_u32(s_raw), full = smem_u32(s_bar), empty = full + 8 * NST, qfull = empty + 8 * NST, qempty = qfull + 8 * NQ;
-    const uint32_t s_q = ring + kDecRing;
-    float* s_slab = reinterpret_cast<float*>(s_raw + kDecRing + kDecQ);
+    const uint32_t s_q = ring + dec_ring<HD>();
+    float* s_slab = reinterpret_cast<float*>(s_raw + dec_ring<HD>() + dec_q<HD>());
     volatile int* abort_flag = &s_abort;
     if (tid == 0) {
         s_abort = 0;
@@ -268,7 +273,9 @@ paged_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap km
     Walk w;
     w.left = 0;
     const int64_t total = dec_find<TILE>(p, H, &w, [&](int64_t n, int64_t* a, int64_t* e) {
-        if (blocks > n) blocks = (int)n;              // every range has a unit at least
+        // Ranges of two units at least: of one, every third would be the end of a pair and no tile.  (1, 2, 4: 8 sequences of 500 to 4000 of one
+        // KV head 33, 24, 22 us, four f32 of 64 7.9, 6.2, 6.0, one of 300 9.2, 9.6, 11.7.)
+        if (blocks > n / 2) blocks = n >= 2 ? (int)(n / 2) : n > 0;
         const int c = blockIdx.x;
         if (c < blocks) {                             // floor(c n / blocks)
             const int64_t each = n >> 32 ? n / blocks : (int64_t)((uint32_t)n / (uint32_t)blocks);
@@ -381,9 +388,10 @@ paged_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap km
         const int hkv = p.gz == 1 ? pass : pass / p.gz, g0 = (pass - hkv * p.gz) * PER;
         const float i = sum == 0.f ? 0.f : 1.f / sum;
         T* out = (T*)p.out + ((int64_t)b * p.n_q + hkv * p.group + g0 + h) * p.head_dim + d0;
-        if (h < min(p.group - g0, PER) && d0 < p.head_dim)     // (head_dim is a multiple of 8, of d0's step)
+        if (h < min(p.group - g0, PER))
 #pragma unroll
-            for (int e = 0; e < E; e += 4) store4(out + e, make_float4(v[e] * i, v[e + 1] * i, v[e + 2] * i, v[e + 3] * i));
+            for (int e = 0; e < E; e += 4)
+                if (d0 + e < p.head_dim) store4(out + e, make_float4(v[e] * i, v[e + 1] * i, v[e + 2] * i, v[e + 3] * i));
     };
     while (w.left > 0) {
         const int hkv = p.gz == 1 ? w.h : w.h / p.gz, g0 = (w.h - hkv * p.gz) * PER;
@@ -595,8 +603,13 @@ paged_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap km
                     }
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        float vv[4];
-                        if constexpr (VE == 4) {
+                        float vv[VE];
+                        if constexpr (VE == 8) {
+                            const uint32_t a = vb + (lane >> 2) * BLK + j * 128;
+                            const float4 x = lds128(a + ((((lane & 3) * 2) ^ j) << 4)), y = lds128(a + ((((lane & 3) * 2 + 1) ^ j) << 4));
+                            vv[0] = x.x; vv[1] = x.y; vv[2] = x.z; vv[3] = x.w;
+                            vv[4] = y.x; vv[5] = y.y; vv[6] = y.z; vv[7] = y.w;
+                        } else if constexpr (VE == 4) {
                             const float4 x = lds128(vb + (lane >> 3) * BLK + j * 128 + (((lane & 7) ^ j) << 4));
                             vv[0] = x.x; vv[1] = x.y; vv[2] = x.z; vv[3] = x.w;
                         } else {
@@ -753,14 +766,19 @@ int32_t decode_configure(DeviceState& ds) {
     auto set = [&](auto kernel, int smem) { return cudaFuncSetAttribute(kernel, attr, smem); };
     RSTQ_CUDA(set(paged_decode_kernel<__nv_bfloat16, 64, 8>, dec_smem<64>()));
     RSTQ_CUDA(set(paged_decode_kernel<__nv_bfloat16, 64, 16>, dec_smem<64>()));
-    RSTQ_CUDA(set(paged_decode_kernel<__nv_bfloat16, 128, 8>, dec_smem<128>()));
-    RSTQ_CUDA(set(paged_decode_kernel<__nv_bfloat16, 128, 16>, dec_smem<128>()));
     RSTQ_CUDA(set(paged_decode_kernel<float, 64, 1>, dec_smem<64>()));
     RSTQ_CUDA(set(paged_decode_kernel<float, 64, 4>, dec_smem<64>()));
     RSTQ_CUDA(set(paged_decode_kernel<float, 64, 8>, dec_smem<64>()));
+    RSTQ_CUDA(set(paged_decode_kernel<__nv_bfloat16, 128, 8>, dec_smem<128>()));
+    RSTQ_CUDA(set(paged_decode_kernel<__nv_bfloat16, 128, 16>, dec_smem<128>()));
     RSTQ_CUDA(set(paged_decode_kernel<float, 128, 1>, dec_smem<128>()));
     RSTQ_CUDA(set(paged_decode_kernel<float, 128, 4>, dec_smem<128>()));
     RSTQ_CUDA(set(paged_decode_kernel<float, 128, 8>, dec_smem<128>()));
+    RSTQ_CUDA(set(paged_decode_kernel<__nv_bfloat16, 256, 8>, dec_smem<256>()));
+    RSTQ_CUDA(set(paged_decode_kernel<__nv_bfloat16, 256, 16>, dec_smem<256>()));
+    RSTQ_CUDA(set(paged_decode_kernel<float, 256, 1>, dec_smem<256>()));
+    RSTQ_CUDA(set(paged_decode_kernel<float, 256, 4>, dec_smem<256>()));
+    RSTQ_CUDA(set(paged_decode_kernel<float, 256, 8>, dec_smem<256>()));
     RSTQ_CUDA(cudaMalloc((void**)&ds.seq_starts, (size_t)(kMaxSeqs + 1) * 8));
     return RSTQ_OK;
 }
@@ -797,9 +815,9 @@ int32_t launch_paged_decode(DeviceState& ds, const PromptArgs& a, int* launches)
     int32_t rc = rows_tensor_map(&kmap, a.k, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc == RSTQ_OK) rc = rows_tensor_map(&vmap, a.v, a.dtype, a.kv_rows, a.kv.ld, a.n_kv, a.head_dim, p.box);
     if (rc != RSTQ_OK) return rc;
-    const int64_t blocks = 2 * (int64_t)ds.sm_count;
-    static_assert(2 * dec_slot<128>() >= 2 * dec_slot<64>(), "slots");
-    RSTQ_REQUIRE(2 * blocks * dec_slot<128>() * 4 <= ds.partials_bytes && blocks <= ds.counters_len, RSTQ_E_LIMIT, "%lld thread blocks", (long long)blocks);
+    const int64_t blocks = (a.head_dim > 128 ? dec_blocks<256>() : dec_blocks<128>()) * (int64_t)ds.sm_count;
+    const int64_t slot = a.head_dim > 128 ? dec_slot<256>() : dec_slot<128>();
+    RSTQ_REQUIRE(2 * blocks * slot * 4 <= ds.partials_bytes && blocks <= ds.counters_len, RSTQ_E_LIMIT, "%lld thread blocks", (long long)blocks);
     *launches = 1;
     p.start = nullptr;
     if (a.seqs > kDecSums) {
@@ -808,17 +826,17 @@ int32_t launch_paged_decode(DeviceState& ds, const PromptArgs& a, int* launches)
         ++*launches;
     }
     const int g = std::min(a.group, per);
-    const size_t smem = (size_t)(a.head_dim <= 64 ? dec_smem<64>() : dec_smem<128>());
-    auto go = [&](auto kernel) { return launch_pdl(kernel, dim3((unsigned)blocks), dim3(kDecThreads), smem, ds, p, kmap, vmap); };
-    cudaError_t e;
-    if (a.dtype == RSTQ_BF16) {
-        if (a.head_dim <= 64) e = g <= 8 ? go(paged_decode_kernel<__nv_bfloat16, 64, 8>) : go(paged_decode_kernel<__nv_bfloat16, 64, 16>);
-        else e = g <= 8 ? go(paged_decode_kernel<__nv_bfloat16, 128, 8>) : go(paged_decode_kernel<__nv_bfloat16, 128, 16>);
-    } else if (a.head_dim <= 64) {
-        e = g == 1 ? go(paged_decode_kernel<float, 64, 1>) : g <= 4 ? go(paged_decode_kernel<float, 64, 4>) : go(paged_decode_kernel<float, 64, 8>);
-    } else {
-        e = g == 1 ? go(paged_decode_kernel<float, 128, 1>) : g <= 4 ? go(paged_decode_kernel<float, 128, 4>) : go(paged_decode_kernel<float, 128, 8>);
-    }
+    auto go = [&](auto kernel, int smem) { return launch_pdl(kernel, dim3((unsigned)blocks), dim3(kDecThreads), (size_t)smem, ds, p, kmap, vmap); };
+    auto sized = [&](auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        using B = __nv_bfloat16;
+        if (a.dtype == RSTQ_BF16) return g <= 8 ? go(paged_decode_kernel<B, HD, 8>, dec_smem<HD>()) : go(paged_decode_kernel<B, HD, 16>, dec_smem<HD>());
+        return g == 1   ? go(paged_decode_kernel<float, HD, 1>, dec_smem<HD>())
+               : g <= 4 ? go(paged_decode_kernel<float, HD, 4>, dec_smem<HD>())
+                        : go(paged_decode_kernel<float, HD, 8>, dec_smem<HD>());
+    };
+    const cudaError_t e = a.head_dim <= 64 ? sized(std::integral_constant<int, 64>()) : a.head_dim <= 128 ? sized(std::integral_constant<int, 128>())
+                                                                                                        : sized(std::integral_constant<int, 256>());
     RSTQ_CUDA(e);
     return RSTQ_OK;
 }

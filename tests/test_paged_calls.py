@@ -481,3 +481,34 @@ def test_groups_that_share_a_tile(ctx, dtype, n_q, n_kv, d, page, lens, new):
     ctx.sync()
     x.check()
     x.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n_q,n_kv,d,page,lens", [
+    (8, 2, 256, 16, [1, 15, 16, 17, 0, 63, 64, 65, 300]),
+    (16, 1, 256, 64, [1500, 2, 700]),
+    (20, 1, 192, 32, [260, 33]),                # more heads in the group than a block serves at once
+    (4, 4, 136, 16, [200, 31, 129]),
+    (3, 1, 248, 128, [500]),
+    (2, 2, 144, 256, [2000, 255, 257]),
+])
+def test_decode_of_wide_heads(ctx, dtype, n_q, n_kv, d, page, lens):
+    p = Pool(ctx, lens, n_kv, d, page, dtype, seed=d)
+    step = n_q * d + 8
+    full = pm.encode(normal(d, len(lens), step), dtype)
+    q = pm.decode(full, dtype)[:, :n_q * d].reshape(len(lens), n_q, d)
+    bq, bo = ctx.array_to_buffer(full), ctx.make_buffer((len(lens) + 1) * n_q * d, NP[dtype])
+    bo.fill_bytes(0x5A)
+    ctx.paged_decode_attention(bq, p.bk, p.bv, bo, p.bt, p.bl, len(lens), n_q, n_q // n_kv, n_kv, d, page, p.n_pages, p.width, d ** -0.5,
+                               DT[dtype], ldq=step)
+    ctx.sync()
+    raw = bo.download().reshape(-1, n_q, d)
+    assert (raw[-1].view(np.uint8) == 0x5A).all()
+    got = pm.decode(raw[:-1], dtype)
+    for b, n in enumerate(lens):
+        want, tol = pm.attention(q[b:b + 1], p.keys[b], p.values[b], d ** -0.5, False, dtype)
+        close(got[b:b + 1], want, tol, f"sequence {b} of {n}")
+    bq.free()
+    bo.free()
+    p.free()
