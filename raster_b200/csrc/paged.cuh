@@ -269,7 +269,7 @@ int32_t launch_sums(DeviceState& ds, const PromptArgs& a, int per, int extra);
 
 // A pool (or packed rows) as [rows][heads][head_dim], read in boxes of 128 bytes x `box` rows of one head.
 int32_t rows_tensor_map(CUtensorMap* m, const void* base, int32_t dtype, int64_t rows, int64_t ld, int heads, int head_dim, int box);
-// prompt_attn.cu, prompt_f32.cu: head_dim <= 128, scale > 0, keys to read.  (*launches: how many)
+// prompt_attn.cu (bf16), prompt_f32.cu (head_dim <= 128): scale > 0, keys to read.  (*launches: how many)
 int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches);
 int32_t launch_prompt_f32(DeviceState& ds, const PromptArgs& a, int* launches);
 // paged_attn.cu: any head_dim and length, a warp per position

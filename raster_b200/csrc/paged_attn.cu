@@ -185,7 +185,7 @@ int32_t launch_sums(DeviceState& ds, const PromptArgs& a, int per, int extra) {
 
 // ---- attention, any shape -----------------------------------------------------------------------
 // One query row and head per thread block: its four warps take four positions in turn (attend_row), and their states are joined
-// through shared memory.  For what the tiled kernels do not take: head_dim above 128, a scale that is not positive (they find the maximum
+// through shared memory.  For what the tiled kernels do not take: f32 prompts of head_dim above 128 (three terms of Q alone would fill shared memory), a scale that is not positive (they find the maximum
 // before they scale), no keys at all.  Bound by L2: every row reads its keys and values itself.
 constexpr int kRowWarps = 4;
 template <typename T>
@@ -378,7 +378,7 @@ static int32_t run_prompt(rstq_ctx* ctx, rstq_buf* q, const PromptArgs& a) {
     DeviceState& ds = ctx->devs[q->dev];
     int32_t rc;
     int launches = 1;
-    if (a.head_dim > 128 || a.scale <= 0.f || a.kv_rows == 0) rc = launch_attention_rows(ds, a);
+    if ((a.head_dim > 128 && a.dtype == RSTQ_F32) || a.scale <= 0.f || a.kv_rows == 0) rc = launch_attention_rows(ds, a);
     else rc = a.dtype == RSTQ_BF16 ? launch_prompt(ds, a, &launches) : launch_prompt_f32(ds, a, &launches);
     if (rc == RSTQ_OK) ctx->launches += launches;
     return rc;

@@ -371,7 +371,7 @@ static __device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, in
 template <typename T>
 __device__ __forceinline__ void prompt_rows(const PromptArgs& a, const PromptItem& it, int h, int warp, int warps) {     // (of one head)
     const int lane = threadIdx.x & 31;
-    using S = RowState<T>;      // (head_dim <= 128: one piece of a lane)
+    using S = RowState<T>;      // (f32: head_dim <= 128; one piece of a lane)
     bool bad = false;
     for (int r = warp; r < it.rows; r += warps) {
         S st;

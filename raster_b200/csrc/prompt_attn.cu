@@ -1,4 +1,4 @@
-// Causal attention of whole prompts, bf16, head_dim up to 128, on the tcgen05 tensor cores.
+// Causal attention of whole prompts, bf16, on the tcgen05 tensor cores.
 //
 //   out[i] = sum_j p_ij V[j] / sum_j p_ij,   p_ij = exp(scale q_i.K_j - m_i),   j <= i + (keys - rows) of its sequence
 //
@@ -43,8 +43,9 @@ constexpr int kPrThreads = 384;      // two warpgroups of softmax; copies, MMAs,
 constexpr int kPrRows = 128;         // rows of a query tile, keys of a tile
 template <int HD>
 struct PromptShape {
-    static constexpr int blks = HD / 64, tile = kPrRows * HD * 2, stages = HD == 128 ? 5 : 8;
-    static constexpr int smem = 1024 + (2 + stages) * tile;
+    // (of 256 columns one query tile: K and V of a step and Q take 192 KB, S and O 384 columns of tensor memory)
+    static constexpr int blks = HD / 64, tile = kPrRows * HD * 2, stages = HD == 256 ? 2 : HD == 128 ? 5 : 8, queries = HD == 256 ? 1 : 2;
+    static constexpr int smem = 1024 + (queries + stages) * tile;
 };
 
 struct PromptParams {
@@ -82,7 +83,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     __shared__ volatile int s_again[2];
     __shared__ PromptWork s_work[2];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;      // (the same in all lanes, for the compiler too)
-    const uint32_t sq = smem_u32(s_raw), ring = sq + 2 * TILE;
+    const uint32_t sq = smem_u32(s_raw), ring = sq + Sh::queries * TILE;
     // full / empty: a stage of the ring (empty: by the MMAs that read it and by the warp at V's edges); qfull / qempty; sfull[t]: S of a
     // tile is there; phalf[t], pfull[t]: half of P is, all of it, and O has its scale; odone[t]: P V is added; vfix[2]: the last V's edge is
     // zeroed; fixed[2]: no V of these rows will be looked at any more; wfull[2] / wempty[2]: what to work on (all six by the number of the block
@@ -114,7 +115,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         fence_async_smem();
     }
     for (int e = p.rpt * p.pack * 8 + tid; e < kPrRows * 8; e += kPrThreads)      // rows of Q's tiles that no copy fills
-        for (int c = 0; c < 2 * Sh::blks; ++c) sts128(sq + c * BLK + e * 16, 0u, 0u, 0u, 0u);
+        for (int c = 0; c < Sh::queries * Sh::blks; ++c) sts128(sq + c * BLK + e * 16, 0u, 0u, 0u, 0u);
     fence_async_smem();
     if (warp == 9) {
         tmem_alloc(smem_u32(&s_tmem), 512);
@@ -623,6 +624,7 @@ int32_t prompt_configure(DeviceState& ds) {
     RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<64, true>), attr, PromptShape<64>::smem));
     RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<128, false>), attr, PromptShape<128>::smem));
     RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<128, true>), attr, PromptShape<128>::smem));
+    RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<256, false>), attr, PromptShape<256>::smem));
     const size_t slots = (size_t)kPromptSlots * (prompt_slot<128>() * 4 + sizeof(PromptItem));
     RSTQ_CUDA(cudaMalloc((void**)&ds.prompt_slots, slots + 64));
     RSTQ_CUDA(cudaMemsetAsync((char*)ds.prompt_slots + slots, 0, 64, ds.stream));
@@ -653,12 +655,12 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     p.rpt = kPrRows / p.pack;
     p.heads = a.n_q / p.pack;
     // Two query tiles per block keep the tensor core busy; with fewer blocks than SMs one each does the rows sooner.
-    p.tiles = a.rows * a.n_q <= kPrRows * (int64_t)ds.sm_count ? 1 : 2;
+    p.tiles = a.head_dim > 128 || a.rows * a.n_q <= kPrRows * (int64_t)ds.sm_count ? 1 : 2;
     // Few blocks of rows that may see many keys are cut into parts, which a second launch joins.  (A sequence's rows of more than a tile then
     // take two as well: there is no lack of parts.)
     const int64_t some = std::min<int64_t>(a.seqs, a.rows);
     const int tiles = a.rows > p.rpt * some ? 2 : 1;
-    const bool parts = prompt_may_part(a, 1024) && (a.rows / (tiles * p.rpt) + some) * p.heads <= ds.sm_count;
+    const bool parts = a.head_dim <= 128 && prompt_may_part(a, 1024) && (a.rows / (tiles * p.rpt) + some) * p.heads <= ds.sm_count;
     if (parts) p.tiles = tiles;
     const int per = p.tiles * p.rpt;
     const int64_t blocks = (a.rows / per + some) * p.heads;     // no sequence has more than this of them
@@ -681,7 +683,8 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     const dim3 grid((unsigned)(parts ? p.sms : std::min<int64_t>(blocks, ds.sm_count)));
     auto go = [&](auto kernel, int smem) { return launch_pdl(kernel, grid, dim3(kPrThreads), (size_t)smem, ds, p, qmap, kmap, vmap); };
     if (a.head_dim <= 64) RSTQ_CUDA(parts ? go(prompt_kernel<64, true>, PromptShape<64>::smem) : go(prompt_kernel<64, false>, PromptShape<64>::smem));
-    else RSTQ_CUDA(parts ? go(prompt_kernel<128, true>, PromptShape<128>::smem) : go(prompt_kernel<128, false>, PromptShape<128>::smem));
+    else if (a.head_dim <= 128) RSTQ_CUDA(parts ? go(prompt_kernel<128, true>, PromptShape<128>::smem) : go(prompt_kernel<128, false>, PromptShape<128>::smem));
+    else RSTQ_CUDA(go(prompt_kernel<256, false>, PromptShape<256>::smem));
     return parts ? launch_prompt_join(ds, p.join) : RSTQ_OK;
 }
 

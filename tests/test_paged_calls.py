@@ -512,3 +512,20 @@ def test_decode_of_wide_heads(ctx, dtype, n_q, n_kv, d, page, lens):
     bq.free()
     bo.free()
     p.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n_q,n_kv,d,page,lens,new", [
+    (4, 2, 256, 16, [1, 17, 130, 0, 300], [1, 17, 130, 0, 5]),
+    (16, 2, 256, 64, [700, 33], [40, 33]),
+    (7, 1, 192, 32, [200, 129], [150, 129]),
+    (3, 3, 136, 128, [400], [200]),
+    (8, 1, 248, 256, [1500, 20], [2, 20]),
+])
+def test_prompts_of_wide_heads(ctx, dtype, n_q, n_kv, d, page, lens, new):
+    x = Prompts(ctx, dtype, n_q, n_kv, d, page, lens, new, seed=d)
+    x.call()
+    ctx.sync()
+    x.check()
+    x.free()
