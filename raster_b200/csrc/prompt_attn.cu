@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
 prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
               const __grid_constant__ CUtensorMap vmap) {
     using Sh = PromptShape<HD>;
-    constexpr int NST = Sh::stages, TILE = Sh::tile, BLK = kPrRows * 128;     // 64 columns of a tile
+    constexpr int NST = Sh::stages, TILE = Sh::tile, BLK = kPrRows * 128, R = Sh::queries * kPrRows;     // BLK: 64 columns of a tile; R: rows of a slot
     extern __shared__ uint8_t s_raw0[];
     uint8_t* s_raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw0) + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) uint64_t s_bar[2 * NST + 19];
@@ -285,15 +285,15 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     } else if (PARTS && has_row && steps > 0) {
 #pragma unroll
                         for (int u = 0; u < 32; u += 4)
-                            *reinterpret_cast<uint4*>(slot + ((i + u) / 4 * 2 * kPrRows + slot_row) * 4) = make_uint4(o[u], o[u + 1], o[u + 2], o[u + 3]);
+                            *reinterpret_cast<uint4*>(slot + ((i + u) / 4 * R + slot_row) * 4) = make_uint4(o[u], o[u + 1], o[u + 2], o[u + 3]);
                     }
                 }
             if (PARTS && !whole) {
                 if (has_row) {
-                    slot[2 * kPrRows * HD + slot_row] = m2;
-                    slot[2 * kPrRows * (HD + 1) + slot_row] = sum;      // (0: the columns say nothing)
+                    slot[R * HD + slot_row] = m2;
+                    slot[R * (HD + 1) + slot_row] = sum;      // (0: the columns say nothing)
                 }
-                if (tid == 0) slot[2 * kPrRows * (HD + 2)] = again ? 1.f : 0.f;
+                if (tid == 0) slot[R * (HD + 2)] = again ? 1.f : 0.f;
             }
             tc_fence_before();       // O has been read before the next rows' P is handed on
             if (again && whole)
@@ -613,7 +613,11 @@ PromptJoin prompt_join(DeviceState& ds, const PromptArgs& a, int pack, int rpt, 
 int32_t launch_prompt_join(DeviceState& ds, const PromptJoin& j) {
     const dim3 grid((unsigned)(12 * ds.sm_count));
     auto go = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(256), 0, ds, j); };
-    if (j.a.dtype == RSTQ_BF16) RSTQ_CUDA(j.a.head_dim <= 64 ? go(prompt_join_kernel<__nv_bfloat16, 64, 256>) : go(prompt_join_kernel<__nv_bfloat16, 128, 256>));
+    using B = __nv_bfloat16;
+    if (j.a.dtype == RSTQ_BF16)
+        RSTQ_CUDA(j.a.head_dim <= 64    ? go(prompt_join_kernel<B, 64, 256>)
+                  : j.a.head_dim <= 128 ? go(prompt_join_kernel<B, 128, 256>)
+                                        : go(prompt_join_kernel<B, 256, 128>));
     else RSTQ_CUDA(j.a.head_dim <= 64 ? go(prompt_join_kernel<float, 64, 128>) : go(prompt_join_kernel<float, 128, 128>));
     return RSTQ_OK;
 }
@@ -625,6 +629,7 @@ int32_t prompt_configure(DeviceState& ds) {
     RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<128, false>), attr, PromptShape<128>::smem));
     RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<128, true>), attr, PromptShape<128>::smem));
     RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<256, false>), attr, PromptShape<256>::smem));
+    RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<256, true>), attr, PromptShape<256>::smem));
     const size_t slots = (size_t)kPromptSlots * (prompt_slot<128>() * 4 + sizeof(PromptItem));
     RSTQ_CUDA(cudaMalloc((void**)&ds.prompt_slots, slots + 64));
     RSTQ_CUDA(cudaMemsetAsync((char*)ds.prompt_slots + slots, 0, 64, ds.stream));
@@ -659,8 +664,8 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     // Few blocks of rows that may see many keys are cut into parts, which a second launch joins.  (A sequence's rows of more than a tile then
     // take two as well: there is no lack of parts.)
     const int64_t some = std::min<int64_t>(a.seqs, a.rows);
-    const int tiles = a.rows > p.rpt * some ? 2 : 1;
-    const bool parts = a.head_dim <= 128 && prompt_may_part(a, 1024) && (a.rows / (tiles * p.rpt) + some) * p.heads <= ds.sm_count;
+    const int tiles = a.head_dim <= 128 && a.rows > p.rpt * some ? 2 : 1;
+    const bool parts = prompt_may_part(a, 1024) && (a.rows / (tiles * p.rpt) + some) * p.heads <= ds.sm_count;
     if (parts) p.tiles = tiles;
     const int per = p.tiles * p.rpt;
     const int64_t blocks = (a.rows / per + some) * p.heads;     // no sequence has more than this of them
@@ -684,7 +689,7 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
     auto go = [&](auto kernel, int smem) { return launch_pdl(kernel, grid, dim3(kPrThreads), (size_t)smem, ds, p, qmap, kmap, vmap); };
     if (a.head_dim <= 64) RSTQ_CUDA(parts ? go(prompt_kernel<64, true>, PromptShape<64>::smem) : go(prompt_kernel<64, false>, PromptShape<64>::smem));
     else if (a.head_dim <= 128) RSTQ_CUDA(parts ? go(prompt_kernel<128, true>, PromptShape<128>::smem) : go(prompt_kernel<128, false>, PromptShape<128>::smem));
-    else RSTQ_CUDA(go(prompt_kernel<256, false>, PromptShape<256>::smem));
+    else RSTQ_CUDA(parts ? go(prompt_kernel<256, true>, PromptShape<256>::smem) : go(prompt_kernel<256, false>, PromptShape<256>::smem));
     return parts ? launch_prompt_join(ds, p.join) : RSTQ_OK;
 }
 

@@ -522,6 +522,8 @@ def test_decode_of_wide_heads(ctx, dtype, n_q, n_kv, d, page, lens):
     (7, 1, 192, 32, [200, 129], [150, 129]),
     (3, 3, 136, 128, [400], [200]),
     (8, 1, 248, 256, [1500, 20], [2, 20]),
+    (4, 2, 256, 32, [2500, 1100, 7, 1500], [2, 140, 7, 1]),
+    (6, 2, 136, 16, [3000, 0, 1030], [5, 0, 30]),
 ])
 def test_prompts_of_wide_heads(ctx, dtype, n_q, n_kv, d, page, lens, new):
     x = Prompts(ctx, dtype, n_q, n_kv, d, page, lens, new, seed=d)
