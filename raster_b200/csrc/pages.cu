@@ -8,7 +8,7 @@
 //
 // The bookkeeping is one block of 1024 threads: counts and ranks are prefix sums over refs, a few microseconds for ten thousand
 // pages.  The data moves in a second launch over all SMs that reads the list of (from, to) pages the first one left in
-// scratch; it is bound by HBM (each page in once, out once).  8 sequences branched in 8 each, 268 MB: 51 us with all of the
+// scratch; it is bound by HBM (each page in once, out once).  8 sequences branched in 8 each, 268 MB: 48 us with all of the
 // bookkeeping; a compaction of 369 MB 69 us.
 #include <algorithm>
 
@@ -207,10 +207,17 @@ pages_extend_kernel(const PageState s, const int32_t* __restrict__ list, const i
         const int at = base + block_scan(k, &total, s_warp);
         const int b = i < n ? list[i] : 0, len = i < n ? page_len(s, b) : 0;
         const int64_t e0 = (int64_t)b * s.width + pages_of(s, len);
-        for (uint32_t left = __ballot_sync(0xffffffffu, k > 0); left; left &= left - 1) {     // a warp writes its sequences' entries in turn
+        constexpr int kOwn = 2;      // pages that a thread writes itself
+        for (int j = 0; j < kOwn; ++j)
+            if (j < k) {
+                const int pg = w.map[at + j];
+                s.table[e0 + j] = pg;
+                s.refs[pg] = 1;
+            }
+        for (uint32_t left = __ballot_sync(0xffffffffu, k > kOwn); left; left &= left - 1) {     // a warp writes the others, sequence by sequence
             const int l = __ffs((int)left) - 1, kl = __shfl_sync(0xffffffffu, k, l), al = __shfl_sync(0xffffffffu, at, l);
             const int64_t el = __shfl_sync(0xffffffffu, e0, l);
-            for (int j = threadIdx.x & 31; j < kl; j += 32) {
+            for (int j = kOwn + (threadIdx.x & 31); j < kl; j += 32) {
                 const int pg = w.map[al + j];
                 s.table[el + j] = pg;
                 s.refs[pg] = 1;
@@ -234,11 +241,12 @@ pages_fork_kernel(const PageState s, const int32_t* __restrict__ src, const int3
     int bad = first_bad(n, &s_min, [&](int i) {
         return (uint32_t)src[i] >= (uint32_t)s.seqs || (uint32_t)dst[i] >= (uint32_t)s.seqs || take_bit(s_bits, dst[i]) || s.lens[dst[i]] != 0;
     });
-    if (bad == n) {   // a source is nobody's destination, and its pages are pages (a warp per source: its loads are under way together)
-        for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {
+    constexpr int LS = 8;      // lanes of a sequence: their loads are under way together, and those of many short sequences too
+    if (bad == n) {   // a source is nobody's destination, and its pages are pages
+        for (int i = threadIdx.x / LS; i < n; i += kPlanThreads / LS) {
             const int np = pages_of(s, page_len(s, src[i]));
             bool wrong = has_bit(s_bits, src[i]);
-            for (int j = threadIdx.x & 31; j < np; j += 32) wrong |= (uint32_t)s.table[(int64_t)src[i] * s.width + j] >= (uint32_t)s.n_pages;
+            for (int j = threadIdx.x % LS; j < np; j += LS) wrong |= (uint32_t)s.table[(int64_t)src[i] * s.width + j] >= (uint32_t)s.n_pages;
             if (wrong) atomicMin(&s_min, i);
         }
         __syncthreads();
@@ -275,14 +283,14 @@ pages_fork_kernel(const PageState s, const int32_t* __restrict__ src, const int3
         }
         base += total;
     }
-    for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {
+    for (int i = threadIdx.x / LS; i < n; i += kPlanThreads / LS) {
         const int len = page_len(s, src[i]), full = len / s.page;
-        for (int j = threadIdx.x & 31; j < full; j += 32) {
+        for (int j = threadIdx.x % LS; j < full; j += LS) {
             const int pg = s.table[(int64_t)src[i] * s.width + j];
             s.table[(int64_t)dst[i] * s.width + j] = pg;
             atomicAdd(&s.refs[pg], 1);
         }
-        if ((threadIdx.x & 31) == 0) s.lens[dst[i]] = len;
+        if (threadIdx.x % LS == 0) s.lens[dst[i]] = len;
     }
     if (threadIdx.x == 0) w.header[0] = want;
     say(s, kInfoOk, s.n_pages - free + want, want, 0);
