@@ -715,15 +715,19 @@ paged_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap km
             const int b = s_open[x].x, pass = s_open[x].y, c0 = s_open[x].z, c1 = s_open[x].w;
             __threadfence();
             if (tid == 0) p.counters[c0] = 0;
+            const int G = min(p.group - (p.gz == 1 ? 0 : pass % p.gz) * PER, PER);
 #pragma unroll
             for (int j = 0; j < (BF ? GH / 8 : 1); ++j) {
-                const int h = j * 8 + h8;
-                if (h8 >= (GH < 8 ? GH : 8)) continue;
+                if (G <= j * 8) continue;
+                // eight rows of threads: those that the heads leave over share the slots
+                int heads = 1;
+                while (heads < 8 && heads < G - j * 8) heads *= 2;
+                const int sets = 8 / heads, set = h8 / heads, h = j * 8 + h8 - set * heads;
                 float top = -INFINITY, sum = 0.f, a[E];
 #pragma unroll
                 for (int x = 0; x < E; ++x) a[x] = 0.f;
                 constexpr int U = 4;                  // slots asked for at a time
-                for (int c = c0; c <= c1; c += U) {
+                for (int c = c0 + set * U; c <= c1; c += sets * U) {
                     float mm[U], ll[U], vv[U][E];
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
@@ -754,7 +758,32 @@ paged_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap km
                             for (int x = 0; x < E; ++x) a[x] = fmaf(fu, vv[u][x], a[x]);
                         }
                 }
-                put(b, pass, h, a, sum);
+                if (sets > 1) {
+                    bar_consumers();                  // (the arrays have been read by whoever used them before)
+#pragma unroll
+                    for (int e = 0; e < E; e += 4) store4(s_slab + h8 * (HD + 4) + d0 + e, make_float4(a[e], a[e + 1], a[e + 2], a[e + 3]));
+                    if (d0 == 0) {
+                        s_m[0][h8] = top;
+                        s_l[0][h8] = sum;
+                    }
+                    bar_consumers();
+                    if (set == 0) {
+                        float all = -INFINITY;
+                        for (int q = 0; q < sets; ++q) all = fmaxf(all, s_m[0][q * heads + h8]);
+                        const float tf = finite_max(all);
+                        sum = 0.f;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) a[e] = 0.f;
+                        for (int q = 0; q < sets; ++q) {
+                            const int y = q * heads + h8;
+                            const float f = ex2(s_m[0][y] - tf);
+                            sum = fmaf(f, s_l[0][y], sum);
+#pragma unroll
+                            for (int e = 0; e < E; ++e) a[e] = fmaf(f, s_slab[y * (HD + 4) + d0 + e], a[e]);
+                        }
+                    }
+                }
+                if (set == 0) put(b, pass, h, a, sum);
             }
         }
     }
