@@ -3,7 +3,7 @@
 //   out[b, h] = sum_j p_j V[b, j] / sum_j p_j,   p_j = exp(scale q.K[b, j] - m),   j < lens[b]
 //
 // Bound by HBM: every cached row is read once, for all query heads of its KV head (up to 16, in f32 8; a larger group's other
-// heads find the rows in L2).  64 sequences of 4100 (64 heads over 8): 172 us, 96 % of the copy rate; 16 of 4000 48 us, 83 %; 16 of 1 to 8000
+// heads find the rows in L2).  64 sequences of 4100 (64 heads over 8): 175 us, 94 % of the copy rate; 16 of 4000 48 us, 83 %; 16 of 1 to 8000
 // 22 us, 51 %; four in f32 of 1300 35 us, 74 %; one of 300 9 us, of 8000 18.  What is not the stream: 1.6 us until the lengths are read and the range is
 // found, 3 until the first tile is there, 2 for a range's last sums, 3 and more for joining the parts of a pair.
 //
