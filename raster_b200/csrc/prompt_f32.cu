@@ -26,13 +26,13 @@
 
 namespace rstq {
 
-constexpr int kPfThreads = 288;      // softmax, split, MMA
 constexpr int kPfRows = 128, kPfKeys = 64, kPfPlaces = 2;      // places for S in tensor memory
 template <int HD>
 struct PromptShapeF {
     static constexpr int blks = HD / 64, qblk = kPfRows * 128, kblk = kPfKeys * 128;     // 64 columns of a term
     static constexpr int qplane = blks * qblk, kplane = blks * kblk;
     static constexpr int smem = 1024 + 3 * (qplane + 2 * kplane);
+    static constexpr int soft = 8, split = HD == 128 ? 8 : 4, threads = (soft + split + 1) * 32;      // warps: softmax, split, one for the MMAs
 };
 
 struct PromptParamsF {
@@ -54,13 +54,14 @@ __device__ __forceinline__ uint32_t next_term(float& a, float& b) {
 
 // PARTS: a block's keys may be cut into parts.
 template <int HD, bool PARTS>
-__global__ void __launch_bounds__(kPfThreads, 1)
+__global__ void __launch_bounds__(PromptShapeF<HD>::threads, 1)
 prompt_f32_kernel(const PromptParamsF p) {
     using Sh = PromptShapeF<HD>;
-    constexpr int NB = kPfPlaces;
+    constexpr int NB = kPfPlaces, SOFT = Sh::soft, SPLIT = Sh::split;
     extern __shared__ uint8_t s_raw0[];
     uint8_t* s_raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw0) + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) uint64_t s_bar[11];
+    __shared__ __align__(8) uint64_t s_bar[15];
+    __shared__ float s_pair[2][2][kPfRows];      // what the two threads of a row tell each other: [turn][half][row]
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_again;
     __shared__ PromptItem s_item;
@@ -69,26 +70,27 @@ prompt_f32_kernel(const PromptParamsF p) {
     // qfull, kfull, vfull: the terms are written; kfree, vfree: the products that read them are done; sfull, pfull: S, P of a place;
     // odone: P V is added; over: everything is, after a wait ran out
     const uint32_t qfull = smem_u32(s_bar), kfull = qfull + 8, kfree = qfull + 16, vfull = qfull + 24, vfree = qfull + 32, sfull = qfull + 40,
-                   pfull = qfull + 56, odone = qfull + 72, over = qfull + 80;
+                   pfull = qfull + 56, odone = qfull + 72, over = qfull + 80, pair = qfull + 88;
     volatile int* abort_flag = &s_abort;
     const int h = blockIdx.x % p.heads, hkv = p.pack > 1 ? h : h / p.a.group;      // query head, or the packed ones' KV head
     if (tid == 0) {
         s_abort = s_again = 0;
-        mbar_init(qfull, 4);
-        mbar_init(kfull, 4);
+        mbar_init(qfull, SPLIT);
+        mbar_init(kfull, SPLIT);
         mbar_init(kfree, 1);
-        mbar_init(vfull, 4);
+        mbar_init(vfull, SPLIT);
         mbar_init(vfree, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(sfull + 8 * i, 1);
-            mbar_init(pfull + 8 * i, 4);
+            mbar_init(pfull + 8 * i, SOFT);
         }
         mbar_init(odone, 1);
         mbar_init(over, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(pair + 8 * i, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
     }
-    if (warp == 8) {
+    if (warp == SOFT + SPLIT) {
         tmem_alloc(smem_u32(&s_tmem), 512);
         tmem_relinquish();
     }
@@ -118,38 +120,54 @@ prompt_f32_kernel(const PromptParamsF p) {
     const bool whole = !PARTS || it.rows == 0 || it.parts == 1;
     const uint32_t tO = tmem + NB * 128;
 
-    if (warp < 4) {
-        // ---- softmax: a thread per row ----
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-        const int rt = warp * 32 + lane, r = rt * p.over_pack >> 16, head = h * p.pack + rt - r * p.pack, mine = sees(r), least = sees(0);
+    if (warp < SOFT) {
+        // ---- softmax: two threads per row, half of the keys each ----
+        const int half = warp >> 2, quarter = warp & 3;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16, bar = pair + 8 * quarter;
+        const int rt = quarter * 32 + lane, r = rt * p.over_pack >> 16, head = h * p.pack + rt - r * p.pack, mine = sees(r) - half * 32, least = sees(0) - half * 32;
         float m = -INFINITY, m2 = 0.f, sum = 0.f;
+        uint32_t turn = 0;
         bool ok = true;
+        // What the row's other thread says.  Both warps have read what they read of tensor memory before either goes on.
+        auto other = [&](float x) {
+            s_pair[turn & 1][half][rt] = x;
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+            ok = wait_phase(bar, turn & 1, abort_flag);
+            tc_fence_after();
+            const float y = s_pair[turn & 1][half ^ 1][rt];
+            ++turn;
+            return y;
+        };
         for (int j = 0; j < n; ++j) {
             const int buf = j % NB;
             const uint32_t tS = tmem + buf * 128 + lanes;
             if (ok) ok = wait_phase(sfull + 8 * buf, (j / NB) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
-            float s[64];
+            float s[32];
 #pragma unroll
-            for (int c = 0; c < 64; c += 16) {
+            for (int c = 0; c < 32; c += 16) {
                 uint32_t a[16], b[16];
-                tmem_ld16(tS + c, a);
-                tmem_ld16(tS + 64 + c, b);
+                tmem_ld16(tS + half * 32 + c, a);
+                tmem_ld16(tS + 64 + half * 32 + c, b);
                 tmem_ld_wait();
 #pragma unroll
                 for (int i = 0; i < 16; i += 2)
                     unpack2(add2(pack2(__uint_as_float(a[i]), __uint_as_float(a[i + 1])), pack2(__uint_as_float(b[i]), __uint_as_float(b[i + 1]))), s[c + i], s[c + i + 1]);
             }
-            if ((j + 1) * kPfKeys > least) {
+            if (j * kPfKeys + 32 > least) {
                 const int lim = mine - j * kPfKeys;
 #pragma unroll
-                for (int i = 0; i < 64; ++i) s[i] = i < lim ? s[i] : -INFINITY;
+                for (int i = 0; i < 32; ++i) s[i] = i < lim ? s[i] : -INFINITY;
             }
             float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int i = 4; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
-            const float rowmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            for (int i = 4; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
+            float rowmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            rowmax = fmaxf(rowmax, other(rowmax));
+            if (!ok) break;
             const bool grown = rowmax > m && !(rowmax * p.scale2 <= m2 + kGrow && m != -INFINITY);
             if (__any_sync(0xffffffffu, grown)) {
                 float f = 1.f;
@@ -165,7 +183,7 @@ prompt_f32_kernel(const PromptParamsF p) {
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < 2 * HD; c += 16) {
+                    for (int c = half * HD; c < (half + 1) * HD; c += 16) {
                         uint32_t o[16];
                         tmem_ld16(tO + lanes + c, o);
                         tmem_ld_wait();
@@ -177,23 +195,20 @@ prompt_f32_kernel(const PromptParamsF p) {
             }
             uint64_t part[2] = {0ull, 0ull};
             const uint64_t scale = pack2(p.scale2, p.scale2), minus = pack2(-m2, -m2);
+            uint32_t w[3][16];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t w[3][16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float a, b;
-                    unpack2(fma2(pack2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), scale, minus), a, b);
-                    a = ex2f(a);
-                    b = ex2f(b);
-                    part[i & 1] = add2(part[i & 1], pack2(a, b));
-                    w[0][i] = next_term(a, b);
-                    w[1][i] = next_term(a, b);
-                    w[2][i] = next_term(a, b);
-                }
-#pragma unroll
-                for (int x = 0; x < 3; ++x) tmem_st16(tS + x * 32 + c * 16, w[x]);
+            for (int i = 0; i < 16; ++i) {
+                float a, b;
+                unpack2(fma2(pack2(s[2 * i], s[2 * i + 1]), scale, minus), a, b);
+                a = ex2f(a);
+                b = ex2f(b);
+                part[i & 1] = add2(part[i & 1], pack2(a, b));
+                w[0][i] = next_term(a, b);
+                w[1][i] = next_term(a, b);
+                w[2][i] = next_term(a, b);
             }
+#pragma unroll
+            for (int x = 0; x < 3; ++x) tmem_st16(tS + x * 32 + half * 16, w[x]);
             float a, b;
             unpack2(add2(part[0], part[1]), a, b);
             sum += a + b;
@@ -206,19 +221,24 @@ prompt_f32_kernel(const PromptParamsF p) {
             if (lane == 0) mbar_arrive(pfull + 8 * buf);
         }
         if (ok && n > 0) ok = wait_phase(odone, (n - 1) & 1, abort_flag);
+        if (ok) {
+            const float y = other(sum);
+            sum = half ? y + sum : sum + y;      // (the same in both)
+        }
         tc_fence_after();
         // (s_again is set before the terms it is about are handed on, and the last product came after all of them)
         const bool again = *(volatile int*)&s_again;
         if (ok && !whole) {
             // a part: sums, reference and sum of weights to its slot
             float* slot = p.join.part + (int64_t)blockIdx.x * prompt_slot<HD>();
-            if (rt < p.rpt * p.pack && r < it.rows) {
+            if (!half && rt < p.rpt * p.pack && r < it.rows) {
                 slot[kPfRows * HD + rt] = m2;
                 slot[kPfRows * (HD + 1) + rt] = sum;
             }
             if (tid == 0) slot[kPfRows * (HD + 2)] = again ? 1.f : 0.f;
 #pragma unroll
-            for (int c = 0; c < HD; c += 16) {
+            for (int k = 0; k < HD / 2; k += 16) {
+                const int c = half * (HD / 2) + k;
                 uint32_t a[16], b[16];
                 tmem_ld16(tO + lanes + c, a);
                 tmem_ld16(tO + lanes + HD + c, b);
@@ -234,7 +254,8 @@ prompt_f32_kernel(const PromptParamsF p) {
             const bool has_row = rt < p.rpt * p.pack && r < it.rows;
             float* out = (float*)p.a.out + ((it.row + r) * p.a.n_q + head) * p.a.head_dim;
 #pragma unroll
-            for (int c = 0; c < HD; c += 16) {
+            for (int k = 0; k < HD / 2; k += 16) {
+                const int c = half * (HD / 2) + k;
                 uint32_t a[16], b[16];
                 if (n > 0) {
                     tmem_ld16(tO + lanes + c, a);
@@ -253,11 +274,11 @@ prompt_f32_kernel(const PromptParamsF p) {
             }
         }
         if (ok && whole && again)
-            for (int i = 0; i < p.pack; ++i) prompt_rows<float>(p.a, it, h * p.pack + i, warp, 4);
-    } else if (warp < 8) {
+            for (int i = 0; i < p.pack; ++i) prompt_rows<float>(p.a, it, h * p.pack + i, warp, SOFT);
+    } else if (warp < SOFT + SPLIT) {
         // ---- split ----
-        constexpr int LPR = HD / 4, RPI = 32 / LPR, NI = 16 / RPI;      // lanes of a row; rows of a load; loads of a warp's 16 rows
-        const int w = warp - 4, d = (lane % LPR) * 4, sub = lane / LPR;
+        constexpr int LPR = HD / 4, RPI = 32 / LPR, ROWS = kPfKeys / SPLIT, NI = ROWS / RPI;      // lanes of a row; rows of a load; a warp's rows of a tile, and loads
+        const int w = warp - SOFT, d = (lane % LPR) * 4, sub = lane / LPR;
         const bool in = d < p.a.head_dim;
         const int din = in ? d : 0;
         uint32_t top = 0;             // largest magnitude seen, as bits
@@ -278,9 +299,9 @@ prompt_f32_kernel(const PromptParamsF p) {
             if (lane == 0) mbar_arrive(bar);
         };
         bool ok = n > 0;
-        // this warp's 16 rows of a tile of K and V: their places, a lane each
+        // this warp's rows of a tile of K and V: their places, a lane each
         auto places = [&](int j) {
-            const int pos = key0 + j * kPfKeys + w * 16 + (lane & 15);
+            const int pos = key0 + j * kPfKeys + w * ROWS + (lane & (ROWS - 1));
             int64_t row = -1;
             if (j < n && pos < it.keys) {
                 row = kv_row(p.a.kv, it.b, it.row0, pos);
@@ -311,16 +332,16 @@ prompt_f32_kernel(const PromptParamsF p) {
         if (ok) {
             fetch(k, p.a.k, r1);
             klive = rows_in(r1);
-            for (int half = 0; half < 2; ++half) {
+            for (int half = 0; half < 2; ++half) {      // (of its rows of Q, twice as many)
                 float4 x[NI];
 #pragma unroll
                 for (int i = 0; i < NI; ++i) {
-                    const int rt = w * 32 + half * 16 + i * RPI + sub, row = rt * p.over_pack >> 16, head = h * p.pack + rt - row * p.pack;
+                    const int rt = (w * 2 + half) * ROWS + i * RPI + sub, row = rt * p.over_pack >> 16, head = h * p.pack + rt - row * p.pack;
                     x[i] = *reinterpret_cast<const float4*>((const float*)p.a.q + (it.row + min(row, it.rows - 1)) * p.a.ldq + (int64_t)head * p.a.head_dim + din);
                 }
 #pragma unroll
                 for (int i = 0; i < NI; ++i) {
-                    const int rt = w * 32 + half * 16 + i * RPI + sub;
+                    const int rt = (w * 2 + half) * ROWS + i * RPI + sub;
                     write(sq, Sh::qplane, Sh::qblk, rt, only(in && rt < it.rows * p.pack, x[i]));
                 }
             }
@@ -332,7 +353,7 @@ prompt_f32_kernel(const PromptParamsF p) {
             ok = wait_phase(kfree, (j & 1) ^ 1u, abort_flag);
             if (!ok) return;
 #pragma unroll
-            for (int i = 0; i < NI; ++i) write(sk, Sh::kplane, Sh::kblk, w * 16 + i * RPI + sub, only(klive >> (i * RPI) & 1, k[i]));
+            for (int i = 0; i < NI; ++i) write(sk, Sh::kplane, Sh::kblk, w * ROWS + i * RPI + sub, only(klive >> (i * RPI) & 1, k[i]));
             hand(kfull);
         };
         write_k(0);
@@ -347,7 +368,7 @@ prompt_f32_kernel(const PromptParamsF p) {
             if (ok) ok = wait_phase(vfree, (j & 1) ^ 1u, abort_flag);
             if (!ok) break;
 #pragma unroll
-            for (int i = 0; i < NI; ++i) write(sv, Sh::kplane, Sh::kblk, w * 16 + i * RPI + sub, only(vlive >> (i * RPI) & 1, v[i]));
+            for (int i = 0; i < NI; ++i) write(sv, Sh::kplane, Sh::kblk, w * ROWS + i * RPI + sub, only(vlive >> (i * RPI) & 1, v[i]));
             hand(vfull);
         }
     } else {
@@ -402,7 +423,7 @@ prompt_f32_kernel(const PromptParamsF p) {
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) tmem_dealloc(tmem, 512);
+    if (warp == SOFT + SPLIT) tmem_dealloc(tmem, 512);
     if (tid == 0 && s_abort) atomicExch(p.status, 2);
 }
 
@@ -437,9 +458,9 @@ int32_t launch_prompt_f32(DeviceState& ds, const PromptArgs& a, int* launches) {
         ++*launches;
     }
     const dim3 grid((unsigned)(parts ? kPartRounds * p.sms : blocks));
-    auto go = [&](auto kernel, int smem) { return launch_pdl(kernel, grid, dim3(kPfThreads), (size_t)smem, ds, p); };
-    if (a.head_dim <= 64) RSTQ_CUDA(parts ? go(prompt_f32_kernel<64, true>, PromptShapeF<64>::smem) : go(prompt_f32_kernel<64, false>, PromptShapeF<64>::smem));
-    else RSTQ_CUDA(parts ? go(prompt_f32_kernel<128, true>, PromptShapeF<128>::smem) : go(prompt_f32_kernel<128, false>, PromptShapeF<128>::smem));
+    auto go = [&](auto kernel, auto shape) { return launch_pdl(kernel, grid, dim3(decltype(shape)::threads), (size_t)decltype(shape)::smem, ds, p); };
+    if (a.head_dim <= 64) RSTQ_CUDA(parts ? go(prompt_f32_kernel<64, true>, PromptShapeF<64>()) : go(prompt_f32_kernel<64, false>, PromptShapeF<64>()));
+    else RSTQ_CUDA(parts ? go(prompt_f32_kernel<128, true>, PromptShapeF<128>()) : go(prompt_f32_kernel<128, false>, PromptShapeF<128>()));
     return parts ? launch_prompt_join(ds, p.join) : RSTQ_OK;
 }
 
