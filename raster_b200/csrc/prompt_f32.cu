@@ -8,13 +8,14 @@
 // another: the tensor core's additions lose a little each, and so only every sixth counts (1000 keys: 3e-7 of the result,
 // against 2e-6 with one sum).  f32 FMAs would be bound by 72 TFLOP/s of the whole device, the six MMAs by a sixth of bf16's rate.
 //
-// A block has a tile of 128 (row, head) pairs of one sequence: rows of a head, or rows of all heads of a group as in prompt_attn.cu.  Four warps fetch K and V, a tile of 64 keys at a time and one ahead in
-// registers, split them and write the terms to shared memory, swizzled as the tensor core wants them (zeros behind the last key);
-// four warps are the softmax, a thread per row, P's three terms over S in tensor memory; one thread issues.  There are two places for S and
-// P, and the next tile's S is formed while this one's exponentials are.  (Of 64 columns two blocks with one place each would fit an SM: two
-// sequences of 1000 rows 63 us, against 46.)  A step of 64 keys takes 1.7 us with 64 columns, 3.7 with 128, of which the MMAs are 1 and 2
-// (an MMA of S is bound by reading Q and K from shared memory, 48 cycles): the rest is the way from S through the softmax to P V and, with
-// 128, V's terms, which wait for the last product with V.  1024 rows of 16 heads: 37 and 67 us.
+// A block has a tile of 128 (row, head) pairs of one sequence: rows of a head, or rows of all heads of a group as in prompt_attn.cu.  Four warps
+// (eight above 64 columns) fetch K and V, a tile of 64 keys at a time and one ahead in registers, split them and write the terms to shared memory,
+// swizzled as the tensor core wants them (zeros behind the last key); eight warps are the softmax, two threads per row with half of the keys
+// each, P's three terms over S in tensor memory; one thread issues.  There are two places for S and P, and the next tile's S is formed while this
+// one's exponentials are.  (Of 64 columns two blocks with one place each would fit an SM: two sequences of 1000 rows 63 us, against 46.)  A step of
+// 64 keys takes 1.7 us with 64 columns, 3.2 with 128, of which the MMAs are 1 and 2 (an MMA of S is bound by reading Q and K from shared memory, 48
+// cycles): the rest is the way of K and V through registers and their split, one tile at a time, which a second tile ahead only lengthens (spills).
+// 1024 rows of 16 heads: 38 and 59 us.
 // Few blocks that see many keys are cut into parts as in prompt_attn.cu: 2 rows behind 4000 keys of 8 heads of 128 212 -> 45 us, 300 of 64 columns
 // 129 -> 50.
 //
