@@ -719,15 +719,15 @@ paged_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap km
 #pragma unroll
             for (int j = 0; j < (BF ? GH / 8 : 1); ++j) {
                 if (G <= j * 8) continue;
-                // eight rows of threads: those that the heads leave over share the slots
-                int heads = 1;
+                constexpr int U = 4;                  // slots asked for at a time
+                // eight rows of threads: those that the heads leave over share the slots, if these are many
+                int heads = c1 - c0 < U ? 8 : 1;
                 while (heads < 8 && heads < G - j * 8) heads *= 2;
                 const int sets = 8 / heads, set = h8 / heads, h = j * 8 + h8 - set * heads;
                 float top = -INFINITY, sum = 0.f, a[E];
 #pragma unroll
                 for (int x = 0; x < E; ++x) a[x] = 0.f;
-                constexpr int U = 4;                  // slots asked for at a time
-                for (int c = c0 + set * U; c <= c1; c += sets * U) {
+                for (int c = h < G ? c0 + set * U : c1 + 1; c <= c1; c += sets * U) {
                     float mm[U], ll[U], vv[U][E];
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
