@@ -440,6 +440,21 @@ def test_prompts_of_many_sequences(ctx, dtype, seqs):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("seqs", [33, 1024, 1025])
+def test_few_active_of_many_sequences(ctx, dtype, seqs):
+    """Most have no new rows: the rows of the others, behind long caches, in parts and not."""
+    lens, new = [5] * seqs, [0] * seqs
+    for i, rows in ((0, 4), (seqs // 2, 1), (seqs - 1, 3)):
+        lens[i], new[i] = 1500 + i, rows
+    x = Prompts(ctx, dtype, 8, 2, 128, 16, lens, new)
+    x.call()
+    ctx.sync()
+    x.check()
+    x.free()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,seqs", [("bf16", 256), ("bf16", 257), ("bf16", 3000), ("f32", 300)])
 def test_decode_of_many_sequences(ctx, dtype, seqs):
     n_q, n_kv, d, page = 4, 2, 64, 16
