@@ -96,9 +96,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
                  : "memory");
 }
 // A wait of a whole warp, in line (kernels that move registers between warps cannot call a function): true once the phase is
-// complete, false after the limit or when another warp gave up.
+// complete, false after the limit or when another warp gave up.  BEAT: the word behind the flag changes while somebody is at work that takes
+// longer than the limit allows; the limit then begins anew.
+template <bool BEAT = false>
 __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
     unsigned long long t0 = 0;
+    int seen = 0;
 #pragma unroll 1
     for (uint32_t i = 1;; ++i) {
         if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
@@ -106,8 +109,13 @@ __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volati
             const unsigned long long now = gtime_ns();
             if (!t0) t0 = now;
             if (__any_sync(0xffffffffu, *abort_flag || now - t0 > kWaitLimitNs)) {
-                *abort_flag = 1;
-                return false;
+                const int is = BEAT ? __shfl_sync(0xffffffffu, abort_flag[1], 0) : 0;
+                if (is == seen || *abort_flag) {
+                    *abort_flag = 1;
+                    return false;
+                }
+                seen = is;
+                t0 = now;
             }
         }
     }
@@ -354,13 +362,14 @@ static __device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, in
 
 // The block's rows one by one, from the positions they see alone.
 template <typename T>
-__device__ __forceinline__ void prompt_rows(const PromptArgs& a, const PromptItem& it, int h, int warp, int warps) {     // (of one head)
+__device__ __forceinline__ void prompt_rows(const PromptArgs& a, const PromptItem& it, int h, int warp, int warps, volatile int* beat = nullptr) {     // (of one head)
     const int lane = threadIdx.x & 31;
     using S = RowState<T>;      // (f32: head_dim <= 128; one piece of a lane)
     bool bad = false;
     for (int r = warp; r < it.rows; r += warps) {
         S st;
         bad |= attend_row(a, it.b, it.row + r, h, it.behind - r, 0, kRowPos, &st);
+        if (beat && lane == 0) ++*beat;
         const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
         if (lane * S::V < a.head_dim)
 #pragma unroll

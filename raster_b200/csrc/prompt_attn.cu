@@ -79,7 +79,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     uint8_t* s_raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw0) + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) uint64_t s_bar[2 * NST + 19];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort;
+    __shared__ int s_abort[2];       // somebody gave up; rows taken again one by one, for which others may have to wait long
     __shared__ volatile int s_again[2];
     __shared__ PromptWork s_work[2];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;      // (the same in all lanes, for the compiler too)
@@ -91,9 +91,9 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     const uint32_t full = smem_u32(s_bar), empty = full + 8 * NST, qfull = empty + 8 * NST, qempty = qfull + 8, sfull = qempty + 8,
                    phalf = sfull + 16, pfull = phalf + 16, odone = pfull + 16, vfix = odone + 16, fixed = vfix + 16, wfull = fixed + 16,
                    wempty = wfull + 16, over = wempty + 16;
-    volatile int* abort_flag = &s_abort;
+    volatile int* abort_flag = s_abort;
     if (tid == 0) {
-        s_abort = 0;
+        s_abort[0] = s_abort[1] = 0;
         for (int i = 0; i < NST; ++i) {
             mbar_init(full + 8 * i, 1);
             mbar_init(empty + 8 * i, 2);
@@ -154,7 +154,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     bool ok = true;
     // The next block of rows, of which `w` is the number; false: there is none.
     auto next_work = [&](int w, PromptWork* x) {
-        if (!wait_phase(wfull + 8 * (w & 1), (w >> 1) & 1, abort_flag)) {
+        if (!wait_phase<true>(wfull + 8 * (w & 1), (w >> 1) & 1, abort_flag)) {
             ok = false;
             return false;
         }
@@ -181,7 +181,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             const int mine = sees(it, r) - it.j0 * kPrRows, least = sees(it, t * p.rpt) - it.j0 * kPrRows;
             float m = -INFINITY, m2 = 0.f, sum = 0.f;      // running maximum of S; scale2 times it (0: nothing seen yet)
             for (int j = 0; j < steps; ++j) {
-                ok = wait_phase(sfull + 8 * t, (c + j) & 1, abort_flag);
+                ok = wait_phase<true>(sfull + 8 * t, (c + j) & 1, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t s[128];
@@ -211,7 +211,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                         sum *= f;
                     }
                     if (j > 0) {      // (S of this step came after the P V of the last but one)
-                        ok = wait_phase(odone + 8 * t, (c + j - 1) & 1, abort_flag);
+                        ok = wait_phase<true>(odone + 8 * t, (c + j - 1) & 1, abort_flag);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll 1
@@ -252,8 +252,8 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             }
             // ---- the rows' results ----
             c += steps;
-            if (ok) ok = wait_phase(fixed + 8 * (w & 1), (w >> 1) & 1, abort_flag);
-            if (steps > 0 && ok) ok = wait_phase(odone + 8 * t, (c - 1) & 1, abort_flag);
+            if (ok) ok = wait_phase<true>(fixed + 8 * (w & 1), (w >> 1) & 1, abort_flag);
+            if (steps > 0 && ok) ok = wait_phase<true>(odone + 8 * t, (c - 1) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
             const bool has_row = t < p.tiles && rt < p.rpt * p.pack && r < it.rows;
@@ -297,7 +297,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             }
             tc_fence_before();       // O has been read before the next rows' P is handed on
             if (again && whole)
-                for (int i = 0; i < p.pack; ++i) prompt_rows<__nv_bfloat16>(p.a, it, x.h * p.pack + i, warp, 8);
+                for (int i = 0; i < p.pack; ++i) prompt_rows<__nv_bfloat16>(p.a, it, x.h * p.pack + i, warp, 8, abort_flag + 1);
             done_work(w);
         }
     } else {
@@ -322,7 +322,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 x.h = item % p.heads;
                 x.item = item;
                 const PromptItem& it = x.it;
-                ok = wait_phase(wempty + 8 * (w & 1), ((w >> 1) & 1) ^ 1u, abort_flag);
+                ok = wait_phase<true>(wempty + 8 * (w & 1), ((w >> 1) & 1) ^ 1u, abort_flag);
                 if (!ok) break;
                 if (lane == 0) {
                     s_again[w & 1] = 0;
@@ -341,7 +341,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 };
                 int ahead = rows_at(0);
                 if (n > 0) {
-                    ok = wait_phase(qempty, (cq & 1) ^ 1u, abort_flag);
+                    ok = wait_phase<true>(qempty, (cq & 1) ^ 1u, abort_flag);
                     if (!ok) break;
                     ++cq;
                     if (lane == 0) {
@@ -359,7 +359,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     const unsigned there = __ballot_sync(0xffffffffu, y >= 0);
                     const uint32_t bytes = (uint32_t)(__popc(there) * p.box * 128 * Sh::blks);
                     for (int kv = 0; kv < 2; ++kv) {
-                        if (ok) ok = wait_phase(empty + 8 * s, ph ^ 1u, abort_flag);
+                        if (ok) ok = wait_phase<true>(empty + 8 * s, ph ^ 1u, abort_flag);
                         if (!ok) break;
                         const uint32_t bar = full + 8 * s, dst = ring + s * TILE;
                         if (lane == 0) {
@@ -389,7 +389,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             int s = 0;                                            // the ring's next stage
             uint32_t ph = 0, c[2] = {0, 0}, cq = 0;               // steps so far; blocks of rows with any
             auto wait = [&](uint32_t bar, uint32_t parity) {
-                if (ok) ok = wait_phase(bar, parity, abort_flag);
+                if (ok) ok = wait_phase<true>(bar, parity, abort_flag);
                 tc_fence_after();
             };
             auto step = [&]() { if (++s == NST) { s = 0; ph ^= 1u; } };
@@ -470,7 +470,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 const PromptItem& it = x.it;
                 const int n = max(steps_of(it, 0), steps_of(it, 1)), base = it.j0 * kPrRows, seen_by_all = sees(it, 0) - base;
                 for (int i = 0; i < 2 * n; ++i) {
-                    ok = wait_phase(full + 8 * s, ph, abort_flag);
+                    ok = wait_phase<true>(full + 8 * s, ph, abort_flag);
                     if (!ok) break;
                     if (i & 1) {
                         const int j = i >> 1;
@@ -517,7 +517,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     __syncthreads();
     if (warp == 9) tmem_dealloc(tmem, 512);
     if (tid == 0) {
-        if (s_abort) atomicExch(p.status, 2);
+        if (s_abort[0]) atomicExch(p.status, 2);
         if (atomicAdd(p.counters + 1, 1) == (int)gridDim.x - 1) p.counters[0] = p.counters[1] = 0;      // the last block: for the next launch
     }
 }

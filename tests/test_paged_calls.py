@@ -546,3 +546,27 @@ def test_prompts_of_wide_heads(ctx, dtype, n_q, n_kv, d, page, lens, new):
     ctx.sync()
     x.check()
     x.free()
+
+
+@pytest.mark.gpu
+def test_a_long_prompt_whose_last_rows_are_taken_one_by_one(ctx):
+    """An infinity above the diagonal far behind: a block's rows by themselves take longer than any wait in the kernel may, and
+    those who wait see that they are at it."""
+    n, n_q, d = 80000, 4, 64                                     # (a block: 64 rows of four heads; the last one is full)
+    q, k, v = (normal(s, n, h, d) for s, h in ((1, n_q), (2, 1), (3, 1)))
+    q, k, v = (pm.from_bf16(pm.to_bf16(x)) for x in (q, k, v))
+    v[n - 9, 0, 5] = np.inf
+    up = ctx.array_to_buffer
+    bq, bk, bv, cu = up(pm.to_bf16(q)), up(pm.to_bf16(k)), up(pm.to_bf16(v)), up(np.array([0, n], np.int32))
+    bo = ctx.make_buffer(n * n_q * d, np.uint16)
+    ctx.prompt_attention(bq, bk, bv, bo, cu, cu, n, n, 1, n_q, n_q, 1, d, d ** -0.5, True, L.BF16)
+    ctx.sync()
+    got = pm.from_bf16(bo.download()).reshape(n, n_q, d)
+    assert np.isfinite(got[:n - 9]).all() and np.isposinf(got[n - 9:, :, 5]).all()
+    v[n - 9, 0, 5] = 0
+    keep = [i for i in range(d) if i != 5]
+    for r in (0, 63, 64, 70001, n - 64, n - 10, n - 9, n - 1):
+        want, tol = pm.attention(q[r:r + 1], k[:r + 1], v[:r + 1], d ** -0.5, False, "bf16")
+        close(got[r:r + 1][..., keep], want[..., keep], tol[..., keep], f"row {r}")
+    for b in (bq, bk, bv, cu, bo):
+        b.free()
