@@ -104,7 +104,7 @@ __device__ int list_free(const PageState& s, int want, int* list, int* s_warp) {
 __device__ __forceinline__ void say(const PageState& s, int status, int used, int copied, int what) {
     if (threadIdx.x == 0) *reinterpret_cast<int4*>(s.info) = make_int4(status, used, copied, what);
 }
-// The smallest index at which `bad` holds over the list, or n.  bits: a bitmap in shared memory (cleared here).
+// The smallest index of a list at which `bad` holds, or n.  (The second barrier: whoever goes on may write *s_min.)
 template <typename F>
 __device__ int first_bad(int n, int* s_min, F bad) {
     if (threadIdx.x == 0) *s_min = n;
@@ -112,7 +112,9 @@ __device__ int first_bad(int n, int* s_min, F bad) {
     for (int i = threadIdx.x; i < n; i += kPlanThreads)
         if (bad(i)) atomicMin(s_min, i);
     __syncthreads();
-    return *s_min;
+    const int first = *s_min;
+    __syncthreads();
+    return first;
 }
 __device__ __forceinline__ bool take_bit(uint32_t* bits, int i) {     // true: it was taken already
     return (atomicOr(&bits[i >> 5], 1u << (i & 31)) >> (i & 31)) & 1u;
