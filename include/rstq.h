@@ -494,8 +494,9 @@ RSTQ_API int32_t rstq_paged_prompt_attention(rstq_ctx* ctx, rstq_buf* q, rstq_bu
  * ceil(n / page) pages.  Free pages are taken lowest first, in the list's order.  kcache and vcache: [layers] pools one behind
  * the other, rows of row_bytes bytes (n_kv * head_dim elements; a page's bytes are a multiple of 16).  Lists: int32 [n], n <= 65536.
  * info int32 [4], written by every call: [0] = 0 done, else nothing was changed: 1 = too few free pages ([3] = pages wanted),
- * 2 = an entry of the list is no sequence (page), is there twice, or may not be there ([3] = its place), 3 = no room in the table,
- * 4 = the positions would go to a page that another sequence holds too; [1] = pages in use; [2] = pages copied.
+ * 2 = an entry of the list is no sequence (page), is there twice, or may not be there, 3 = no room in the table, 4 = the positions would
+ * go to a page that another sequence holds too (2 to 4: [3] = the first such place; of entries that are there twice, the later one's);
+ * [1] = pages in use; [2] = pages copied.
  *   rstq_pages_free     the listed sequences end: their pages lose a holder, their rows of the table become -1, lens 0.
  *   rstq_pages_extend   room for counts[i] more positions of sequence list[i] (lens grows by them).
  *   rstq_pages_fork     dst[i], a sequence of length 0, becomes src[i]: full pages shared, a partial last page copied to a page

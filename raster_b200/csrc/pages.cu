@@ -119,6 +119,21 @@ __device__ int first_bad(int n, int* s_min, F bad) {
 __device__ __forceinline__ bool take_bit(uint32_t* bits, int i) {     // true: it was taken already
     return (atomicOr(&bits[i >> 5], 1u << (i & 31)) >> (i & 31)) & 1u;
 }
+// The smallest index of a list whose entry is no number below `limit`, is wrong by itself, or is there for a second time; n: none.  One look
+// at the list says whether there is any, and fills the bitmap; of equal entries it takes for the second one which came later, so where it
+// finds any, the places are looked at again, by the first one of each number (first: scratch of `limit` words).
+template <typename F>
+__device__ int first_wrong(const int32_t* list, int n, int limit, uint32_t* bits, int* s_min, int* first, F wrong) {
+    auto outside = [&](int i) { return (uint32_t)list[i] >= (uint32_t)limit || wrong(i); };
+    if (first_bad(n, s_min, [&](int i) { return outside(i) || take_bit(bits, list[i]); }) == n) return n;
+    for (int i = threadIdx.x; i < n; i += kPlanThreads)
+        if ((uint32_t)list[i] < (uint32_t)limit) first[list[i]] = n;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kPlanThreads)
+        if ((uint32_t)list[i] < (uint32_t)limit) atomicMin(&first[list[i]], i);
+    __syncthreads();
+    return first_bad(n, s_min, [&](int i) { return outside(i) || __ldcg(&first[list[i]]) != i; });
+}
 __device__ __forceinline__ bool has_bit(const uint32_t* bits, int i) { return (bits[i >> 5] >> (i & 31)) & 1u; }
 __device__ void clear_bits(uint32_t* bits, int n) {
     for (int i = threadIdx.x; i < (n + 31) / 32; i += kPlanThreads) bits[i] = 0;
@@ -127,13 +142,13 @@ __device__ void clear_bits(uint32_t* bits, int n) {
 
 // Pages of the listed sequences given back.
 __global__ void __launch_bounds__(kPlanThreads)
-pages_free_kernel(const PageState s, const int32_t* __restrict__ list, const int n) {
+pages_free_kernel(const PageState s, const int32_t* __restrict__ list, const int n, const PageScratch w) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     __shared__ uint32_t s_bits[kMaxSeqs / 32];
     __shared__ int s_warp[32], s_min;
     clear_bits(s_bits, s.seqs);
-    const int bad = first_bad(n, &s_min, [&](int i) { return (uint32_t)list[i] >= (uint32_t)s.seqs || take_bit(s_bits, list[i]); });
+    const int bad = first_wrong(list, n, s.seqs, s_bits, &s_min, w.map, [](int) { return false; });
     if (bad < n) {
         const int used = s.n_pages - list_free(s, 0, nullptr, s_warp);
         say(s, kInfoList, used, 0, bad);
@@ -166,7 +181,7 @@ pages_extend_kernel(const PageState s, const int32_t* __restrict__ list, const i
     clear_bits(s_bits, s.seqs);
     const int64_t room = min((int64_t)s.width * s.page, (int64_t)INT32_MAX);
     int status = kInfoList;
-    int bad = first_bad(n, &s_min, [&](int i) { return (uint32_t)list[i] >= (uint32_t)s.seqs || counts[i] < 0 || take_bit(s_bits, list[i]); });
+    int bad = first_wrong(list, n, s.seqs, s_bits, &s_min, w.map, [&](int i) { return counts[i] < 0; });
     if (bad == n) {
         status = kInfoWidth;
         bad = first_bad(n, &s_min, [&](int i) { return (int64_t)page_len(s, list[i]) + counts[i] > room; });
@@ -240,9 +255,7 @@ pages_fork_kernel(const PageState s, const int32_t* __restrict__ src, const int3
     __shared__ int s_warp[32], s_min;
     if (threadIdx.x == 0) w.header[0] = 0;
     clear_bits(s_bits, s.seqs);
-    int bad = first_bad(n, &s_min, [&](int i) {
-        return (uint32_t)src[i] >= (uint32_t)s.seqs || (uint32_t)dst[i] >= (uint32_t)s.seqs || take_bit(s_bits, dst[i]) || s.lens[dst[i]] != 0;
-    });
+    int bad = first_wrong(dst, n, s.seqs, s_bits, &s_min, w.map, [&](int i) { return (uint32_t)src[i] >= (uint32_t)s.seqs || s.lens[dst[i]] != 0; });
     constexpr int LS = 8;      // lanes of a sequence: their loads are under way together, and those of many short sequences too
     if (bad == n) {   // a source is nobody's destination, and its pages are pages
         for (int i = threadIdx.x / LS; i < n; i += kPlanThreads / LS) {
@@ -473,9 +486,7 @@ pages_list_kernel(const int32_t* __restrict__ src, const int32_t* __restrict__ d
     extern __shared__ uint32_t s_map[];
     __shared__ int s_min;
     clear_bits(s_map, n_pages);
-    int bad = first_bad(n, &s_min, [&](int i) {
-        return (uint32_t)src[i] >= (uint32_t)n_pages || (uint32_t)dst[i] >= (uint32_t)n_pages || take_bit(s_map, dst[i]);
-    });
+    int bad = first_wrong(dst, n, n_pages, s_map, &s_min, w.map, [&](int i) { return (uint32_t)src[i] >= (uint32_t)n_pages; });
     if (bad == n) bad = first_bad(n, &s_min, [&](int i) { return has_bit(s_map, src[i]); });
     if (threadIdx.x == 0) {
         w.header[0] = bad == n ? n : 0;
@@ -555,7 +566,7 @@ int32_t rstq_pages_free(rstq_ctx* ctx, rstq_buf* table, rstq_buf* lens, rstq_buf
     if (rc == RSTQ_OK) rc = list_args(ctx, s, table, list, nullptr, n);
     if (rc != RSTQ_OK) return rc;
     DeviceState& ds = ctx->devs[table->dev];
-    RSTQ_CUDA(launch_pdl(pages_free_kernel, dim3(1), dim3(kPlanThreads), 0, ds, s, (const int32_t*)list->ptr, (int)n));
+    RSTQ_CUDA(launch_pdl(pages_free_kernel, dim3(1), dim3(kPlanThreads), 0, ds, s, (const int32_t*)list->ptr, (int)n, page_scratch(ds)));
     ctx->launches++;
     return RSTQ_OK;
 }

@@ -55,3 +55,63 @@ def test_fork_refuses_a_source_that_is_a_destination(ctx, places):
     src.free()
     dst.free()
     c.close()
+
+
+# ---- entries that are there twice ----------------------------------------------------------------------
+def twice(rng, n, many):
+    """A list of n different numbers of which `many` places repeat an earlier one; the first of these places."""
+    a = rng.permutation(4 * n)[:n]
+    at = np.sort(rng.permutation(np.arange(1, n))[:many])
+    for i in at:
+        a[i] = a[rng.integers(0, i)]
+    seen = set()
+    for i, x in enumerate(a.tolist()):
+        if x in seen:
+            return a.tolist(), i
+        seen.add(x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,many", [(2, 1), (33, 1), (700, 1), (700, 60), (3000, 2), (3000, 2900)])
+def test_the_place_of_an_entry_that_is_there_twice(ctx, n, many):
+    rng = np.random.default_rng(n + many)
+    c = Cache(ctx, 8 * n, 16, 1, 16, layers=1, row=1)
+    before = state(c)
+    for _ in range(25):
+        a, place = twice(rng, n, many)
+        la, other, ones = c.ints(a), c.ints(range(4 * n, 5 * n)), c.ints([1] * n)
+        for call in (lambda: ctx.pages_free(c.bt, c.bl, c.br, la, c.bi, n, *c.sizes),
+                     lambda: ctx.pages_extend(c.bt, c.bl, c.br, la, ones, c.bi, n, *c.sizes),
+                     lambda: ctx.pages_fork(c.bk, c.bv, c.bt, c.bl, c.br, other, la, c.bi, n, *c.sizes, 1, 1)):
+            call()
+            assert c.info() == [2, 0, 0, place]
+        for b in (la, other, ones):
+            b.free()
+    assert same(before, state(c))
+    c.close()
+    k, v, info = (ctx.make_buffer(8 * n * 16, np.uint8) for _ in range(3))
+    for _ in range(25):
+        a, place = twice(rng, n, many)
+        la, other = (ctx.array_to_buffer(np.array(x, np.int32)) for x in (a, range(4 * n, 5 * n)))
+        ctx.pages_copy(k, v, other, la, info, n, 8 * n, 1, 16)
+        ctx.sync()
+        assert info.download().view(np.int32)[:4].tolist() == [2, 0, 0, place]
+        la.free()
+        other.free()
+    for b in (k, v, info):
+        b.free()
+
+
+@pytest.mark.gpu
+def test_the_place_of_an_entry_that_is_wrong_by_itself_or_twice(ctx):
+    """Whichever comes first."""
+    c = Cache(ctx, 40, 16, 1, 16, layers=1, row=1)
+    for a, counts, place in (([3, 4, 3, 40], [1] * 4, 2), ([3, 40, 3, 4], [1] * 4, 1), ([3, 4, 5, 3], [1, -1, 1, 1], 1),
+                             ([3, 4, 3, 5], [1, 1, 1, -1], 2), ([3, 4, 3, 5], [-1, 1, -1, 1], 0), ([-5, -5], [1, 1], 0)):
+        la, lc = c.ints(a), c.ints(counts)
+        for _ in range(5):
+            ctx.pages_extend(c.bt, c.bl, c.br, la, lc, c.bi, len(a), *c.sizes)
+            assert c.info() == [2, 0, 0, place]
+        la.free()
+        lc.free()
+    c.close()
