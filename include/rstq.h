@@ -493,7 +493,7 @@ RSTQ_API int32_t rstq_paged_prompt_attention(rstq_ctx* ctx, rstq_buf* q, rstq_bu
  * sequences hold a page, 0 = free; a new cache has lens and refs of zeros and a table of -1.  A sequence of n positions holds
  * ceil(n / page) pages.  Free pages are taken lowest first, in the list's order.  kcache and vcache: [layers] pools one behind
  * the other, rows of row_bytes bytes (n_kv * head_dim elements; a page's bytes are a multiple of 16).  Lists: int32 [n], n <= 65536.
- * info int32 [4], written by every call: [0] = 0 done, else nothing was changed: 1 = too few free pages ([3] = pages wanted),
+ * info int32 [4], written by every call: [0] = 0 done, else nothing was changed: 1 = too few free pages ([3] = pages wanted, 2^31 - 1 at most),
  * 2 = an entry of the list is no sequence (page), is there twice, or may not be there, 3 = no room in the table, 4 = the positions would
  * go to a page that another sequence holds too (2 to 4: [3] = the first such place; of entries that are there twice, the later one's);
  * [1] = pages in use; [2] = pages copied.

@@ -204,16 +204,15 @@ pages_extend_kernel(const PageState s, const int32_t* __restrict__ list, const i
         const int len = page_len(s, list[i]);
         return pages_of(s, len + counts[i]) - pages_of(s, len);
     };
-    int64_t want = 0;     // (saturated: more than there can be)
+    int64_t want = 0;
     for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
         int total;
         block_scan(i0 + (int)threadIdx.x < n ? need(i0 + threadIdx.x) : 0, &total, s_warp);
         want += total;
-        if (want > s.n_pages) want = s.n_pages + 1;
     }
-    const int free = list_free(s, (int)want, w.map, s_warp);
+    const int free = list_free(s, (int)min(want, (int64_t)s.n_pages), w.map, s_warp);
     if (want > free) {
-        say(s, kInfoNoPages, s.n_pages - free, 0, (int)want);
+        say(s, kInfoNoPages, s.n_pages - free, 0, (int)min(want, (int64_t)INT32_MAX));
         return;
     }
     __syncthreads();

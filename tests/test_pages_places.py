@@ -115,3 +115,37 @@ def test_the_place_of_an_entry_that_is_wrong_by_itself_or_twice(ctx):
         la.free()
         lc.free()
     c.close()
+
+
+# ---- pages wanted ----------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_pages_wanted_are_said_in_full(ctx):
+    """Also where they are more than the pool has, and more than the word holds."""
+    c = Cache(ctx, 300, 8, 1 << 17, 256, layers=1, row=1)
+    for seqs, each, want in (([0], 9, 9), ([1, 0, 2], 1000, 3000), (list(range(300)), 100000, 30000000), ([5, 6], 0, 0)):
+        la, lc = c.ints(seqs), c.ints([each * 256] * len(seqs))
+        ctx.pages_extend(c.bt, c.bl, c.br, la, lc, c.bi, len(seqs), *c.sizes)
+        assert c.info() == [1 if want else 0, 0, 0, want]
+        la.free()
+        lc.free()
+    assert not c.bl.download().any() and not c.br.download().any()
+    c.close()
+    c = Cache(ctx, 4096, 2, 1 << 12, 16, layers=1, row=1)      # 2^24 pages
+    la, lc = c.ints(range(4096)), c.ints([1 << 16] * 4096)
+    ctx.pages_extend(c.bt, c.bl, c.br, la, lc, c.bi, 4096, *c.sizes)
+    assert c.info() == [1, 0, 0, 1 << 24]
+    la.free()
+    lc.free()
+    c.close()
+    n_pages, seqs, width = 2, 2200, 1 << 20                     # 2200 sequences of 2^20 pages: more than 2^31 - 1
+    table, lens, refs = ctx.make_buffer(seqs * width, np.int32), ctx.make_buffer(seqs, np.int32), ctx.make_buffer(n_pages, np.int32)
+    info, la = ctx.make_buffer(4, np.int32), ctx.array_to_buffer(np.arange(seqs, dtype=np.int32))
+    lc = ctx.array_to_buffer(np.full(seqs, 16 << 20, np.int32))
+    for b in (lens, refs):
+        b.upload(np.zeros(b.n_elements, np.int32))
+    ctx.pages_extend(table, lens, refs, la, lc, info, seqs, seqs, n_pages, width, 16)
+    ctx.sync()
+    assert info.download().tolist() == [1, 0, 0, (1 << 31) - 1]
+    assert not lens.download().any() and not refs.download().any()
+    for b in (table, lens, refs, info, la, lc):
+        b.free()
