@@ -569,7 +569,8 @@ prompt_join_kernel(const PromptJoin p) {
             float next = top;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                f[q] = q0 + q < it.parts && s[q] != 0.f ? f[q] : -INFINITY;
+                if (q0 + q >= it.parts) s[q] = 0.f;
+                f[q] = s[q] != 0.f ? f[q] : -INFINITY;
                 next = fmaxf(next, f[q]);
             }
             const float ref = next == -INFINITY ? 0.f : next, g = ex2f(top - ref);
@@ -579,8 +580,8 @@ prompt_join_kernel(const PromptJoin p) {
             for (int x = 0; x < 8; ++x) a[x] *= g;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
+                if (s[q] == 0.f) continue;      // (not where the weight is: 0 times what is no number is none either)
                 const float w = ex2f(f[q] - ref);
-                if (w == 0.f) continue;
                 total = fmaf(w, s[q], total);
                 a[0] = fmaf(w, u[q].x, a[0]); a[1] = fmaf(w, u[q].y, a[1]); a[2] = fmaf(w, u[q].z, a[2]); a[3] = fmaf(w, u[q].w, a[3]);
                 a[4] = fmaf(w, v[q].x, a[4]); a[5] = fmaf(w, v[q].y, a[5]); a[6] = fmaf(w, v[q].z, a[6]); a[7] = fmaf(w, v[q].w, a[7]);
