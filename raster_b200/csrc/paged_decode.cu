@@ -110,7 +110,9 @@ __device__ __forceinline__ void bar_consumers() { asm volatile("bar.sync 1, 128;
 // 16 sequences of 300 13.9, 12.9, 11.9, 12.9 us, of 4000 49.3, 48.5, 47.8, 48.9; four in f32 of 1300 35.8, 35.3, 34.9, 35.3.)
 constexpr int kDecEnd = 2;
 constexpr int kDecSums = 256;                         // sequences above which launch_sums adds the lengths up (1000 of 100: 115 -> 107 us)
-constexpr float kRest = 7.8886091e-31f;      // 2^-100
+// What a weight's second term has at least beside the rest of it: the weight times 2^-7, 2^-100 at most.  Nothing for a weight of nothing, and never
+// more than a weight's own rounding to bf16: for those below 2^-93 a 128th, for one of 2^-76 the 2^-24th part.
+__device__ __forceinline__ float some_rest(float w) { return fminf(w * 0.0078125f, 7.8886091e-31f); }
 
 // Where a block's range of units lies.  Units of sequence b: for each of H heads its tiles, and kDecEnd for what the end of a part costs.  All lanes of a warp hold the same,
 // but for the lengths: lane x has that of sequence first + x.
@@ -493,10 +495,10 @@ paged_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap km
                             const float a = ex2(sc[j][2 * x] - m0), b = ex2(sc[j][2 * x + 1] - m1);
                             l[2 * j] += a;
                             l[2 * j + 1] += b;
-                            // (cut, not rounded, and the rest never zero: both terms of an infinite value have one sign)
+                            // (cut, not rounded, and the rest zero with the weight alone: both terms of an infinite value have one sign)
                             const uint32_t h2 = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
                             hi[j][x] = turn8x8(h2);
-                            lo[j][x] = turn8x8(bf16_pair(a - __uint_as_float(h2 << 16) + kRest, b - __uint_as_float(h2 & 0xFFFF0000u) + kRest));
+                            lo[j][x] = turn8x8(bf16_pair(a - __uint_as_float(h2 << 16) + some_rest(a), b - __uint_as_float(h2 & 0xFFFF0000u) + some_rest(b)));
                         }
                     }
                 }

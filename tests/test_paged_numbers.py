@@ -47,3 +47,33 @@ def test_a_key_that_is_no_number_far_below_the_largest_score(ctx, dtype, d, rows
         got = pm.decode(x.raw(), dtype).reshape(rows, n_q, d)
         assert np.isnan(got).all(), (pos, np.isnan(got).mean())
     x.free()
+
+
+# ---- large values behind weights that vanish -----------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n_q,n_kv,d,lens", [(2, 1, 64, [40, 500]), (16, 1, 128, [100, 33]), (8, 2, 256, [300])])
+def test_decode_of_large_values_whose_weights_vanish(ctx, dtype, n_q, n_kv, d, lens):
+    """Weights of 2^-150 and less come to nothing, times 10^38 too."""
+    p = Pool(ctx, lens, n_kv, d, 16, dtype, seed=d)
+    q = np.abs(pm.decode(pm.encode(normal(d, len(lens), n_q, d), dtype), dtype)) + 1
+    k, v = p.k.copy(), p.v.copy()
+    keys, values = [a.copy() for a in p.keys], [a.copy() for a in p.values]
+    for b, n in enumerate(lens):
+        for pos in (0, 17, n - 2):
+            k[at(p, b, pos)] = keys[b][pos] = -60.0        # a score of -60 sum(q) / sqrt(d) or less: -480 and below
+            v[at(p, b, pos)] = values[b][pos] = pm.decode(pm.encode(np.array(2e38 if pos else -2e38), dtype), dtype)
+    p.bk.upload(pm.encode(k, dtype))
+    p.bv.upload(pm.encode(v, dtype))
+    bq, bo = ctx.array_to_buffer(pm.encode(q, dtype)), ctx.make_buffer(len(lens) * n_q * d, NP[dtype])
+    ctx.paged_decode_attention(bq, p.bk, p.bv, bo, p.bt, p.bl, len(lens), n_q, n_q // n_kv, n_kv, d, 16, p.n_pages, p.width, d ** -0.5, DT[dtype])
+    ctx.sync()
+    got = pm.decode(bo.download(), dtype).reshape(len(lens), n_q, d)
+    for b, n in enumerate(lens):
+        # the model in f64 keeps such weights; what is left of them in f32 is nothing, so these positions do not count
+        keep = [i for i in range(n) if i not in (0, 17, n - 2)]
+        want, tol = pm.attention(q[b:b + 1], keys[b][keep], values[b][keep], d ** -0.5, False, dtype)
+        close(got[b:b + 1], want, tol, f"sequence {b}")
+    for b in (bq, bo):
+        b.free()
+    p.free()
