@@ -4,18 +4,21 @@
 //   x = x1 + x2 + x3, each the leading 8 bits of what is left (24 bits in all: exact);
 //   x y = x1 y1 + (x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1)          to 2^-24 of it
 //
-// for Q K^T and for P V alike: six MMAs instead of one.  The first product has a sum of its own in tensor memory and the five small ones
-// another: the tensor core's additions lose a little each, and so only every sixth counts (1000 keys: 3e-7 of the result,
-// against 2e-6 with one sum).  f32 FMAs would be bound by 72 TFLOP/s of the whole device, the six MMAs by a sixth of bf16's rate.
+// for Q K^T and for P V alike: six MMAs instead of one.  The tensor core's additions cut off, always towards zero, so no sum stays there for
+// long: the first product has one of its own and the five small ones another, in tensor memory, and P V of every tile of keys is taken out and
+// added, to nearest, to sums in registers.  (Left in tensor memory over all keys a result lost 6e-9 of itself with every key: 1.2e-5 of it after
+// 4000, 7.7e-5 after 16000, 3.7e-4 after 64000; as it is 2e-7, 3e-7, 6e-7.  It costs nothing: O is not rescaled in tensor memory any more; 1024
+// rows of 16 heads x 64 38 us before and after, x 128 59 and 56.)  f32 FMAs would be bound by 72 TFLOP/s of the whole device, the six MMAs by a
+// sixth of bf16's rate.
 //
 // A block has a tile of 128 (row, head) pairs of one sequence: rows of a head, or rows of all heads of a group as in prompt_attn.cu.  Four warps
 // (eight above 64 columns) fetch K and V, a tile of 64 keys at a time and one ahead in registers, split them and write the terms to shared memory,
 // swizzled as the tensor core wants them (zeros behind the last key); eight warps are the softmax, two threads per row with half of the keys
 // each, P's three terms over S in tensor memory; one thread issues.  There are two places for S and P, and the next tile's S is formed while this
 // one's exponentials are.  (Of 64 columns two blocks with one place each would fit an SM: two sequences of 1000 rows 63 us, against 46.)  A step of
-// 64 keys takes 1.7 us with 64 columns, 3.2 with 128, of which the MMAs are 1 and 2 (an MMA of S is bound by reading Q and K from shared memory, 48
+// 64 keys takes 1.7 us with 64 columns, 3.0 with 128, of which the MMAs are 1 and 2 (an MMA of S is bound by reading Q and K from shared memory, 48
 // cycles): the rest is the way of K and V through registers and their split, one tile at a time, which a second tile ahead only lengthens (spills).
-// 1024 rows of 16 heads: 38 and 59 us.
+// 1024 rows of 16 heads: 38 and 56 us.
 // Few blocks that see many keys are cut into parts as in prompt_attn.cu: 2 rows behind 4000 keys of 8 heads of 128 212 -> 45 us, 300 of 64 columns
 // 129 -> 50.
 //
@@ -33,7 +36,13 @@ struct PromptShapeF {
     static constexpr int blks = HD / 64, qblk = kPfRows * 128, kblk = kPfKeys * 128;     // 64 columns of a term
     static constexpr int qplane = blks * qblk, kplane = blks * kblk;
     static constexpr int smem = 1024 + 3 * (qplane + 2 * kplane);
-    static constexpr int soft = 8, split = HD == 128 ? 8 : 4, threads = (soft + split + 1) * 32;      // warps: softmax, split, one for the MMAs
+    static constexpr int soft = 8, split = HD == 128 ? 8 : 4;      // warps: softmax, split, and one for the MMAs
+    // Registers of a thread: 128 columns' softmax has 64 sums of its row, so there the split's and the MMAs' threads (a warpgroup of which one warp
+    // works) give some of theirs up.  (With 17 warps none could have more than 96, and the sums would be spilled.)
+    static constexpr bool moved = HD == 128;
+    static constexpr int threads = (soft + split + (moved ? 4 : 1)) * 32;
+    static constexpr int launched = 96, soft_regs = 128, split_regs = 96, mma_regs = 32;
+    static_assert(soft * soft_regs + split * split_regs + 4 * mma_regs <= (soft + split + 4) * launched || !moved, "more than there are: the wait for them would not end");
 };
 
 struct PromptParamsF {
@@ -123,6 +132,7 @@ prompt_f32_kernel(const PromptParamsF p) {
 
     if (warp < SOFT) {
         // ---- softmax: two threads per row, half of the keys each ----
+        if constexpr (Sh::moved) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Sh::soft_regs));
         const int half = warp >> 2, quarter = warp & 3;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16, bar = pair + 8 * quarter;
         const int rt = quarter * 32 + lane, r = rt * p.over_pack >> 16, head = h * p.pack + rt - r * p.pack, mine = sees(r) - half * 32, least = sees(0) - half * 32;
@@ -141,6 +151,20 @@ prompt_f32_kernel(const PromptParamsF p) {
             ++turn;
             return y;
         };
+        // Sums of P V so far, of this thread's half of the columns; a tile's P V added to them.
+        uint64_t o[HD / 4];
+#pragma unroll
+        for (int i = 0; i < HD / 4; ++i) o[i] = 0ull;
+        auto fold = [&]() {
+#pragma unroll
+            for (int c = 0; c < HD / 2; c += 16) {
+                uint32_t a[16], b[16];
+                tmem_ld_x2_wait(tO + lanes + half * (HD / 2) + c, tO + lanes + HD + half * (HD / 2) + c, a, b);
+#pragma unroll
+                for (int i = 0; i < 16; i += 2)
+                    o[(c + i) / 2] = add2(o[(c + i) / 2], add2(pack2(__uint_as_float(a[i]), __uint_as_float(a[i + 1])), pack2(__uint_as_float(b[i]), __uint_as_float(b[i + 1]))));
+            }
+        };
         for (int j = 0; j < n; ++j) {
             const int buf = j % NB;
             const uint32_t tS = tmem + buf * 128 + lanes;
@@ -148,14 +172,13 @@ prompt_f32_kernel(const PromptParamsF p) {
             if (!ok) break;
             tc_fence_after();
             float s[32];
+            constexpr int SW = Sh::moved ? 8 : 16;      // columns at a time: what the registers hold beside the sums
 #pragma unroll
-            for (int c = 0; c < 32; c += 16) {
-                uint32_t a[16], b[16];
-                tmem_ld16(tS + half * 32 + c, a);
-                tmem_ld16(tS + 64 + half * 32 + c, b);
-                tmem_ld_wait();
+            for (int c = 0; c < 32; c += SW) {
+                uint32_t a[SW], b[SW];
+                tmem_ld_x2_wait(tS + half * 32 + c, tS + 64 + half * 32 + c, a, b);
 #pragma unroll
-                for (int i = 0; i < 16; i += 2)
+                for (int i = 0; i < SW; i += 2)
                     unpack2(add2(pack2(__uint_as_float(a[i]), __uint_as_float(a[i + 1])), pack2(__uint_as_float(b[i]), __uint_as_float(b[i + 1]))), s[c + i], s[c + i + 1]);
             }
             if (j * kPfKeys + 32 > least) {
@@ -170,58 +193,59 @@ prompt_f32_kernel(const PromptParamsF p) {
             rowmax = fmaxf(rowmax, other(rowmax));
             if (!ok) break;
             const bool grown = rowmax > m && !(rowmax * p.scale2 <= m2 + kGrow && m != -INFINITY);
-            if (__any_sync(0xffffffffu, grown)) {
-                float f = 1.f;
-                if (grown) {
-                    const float next = rowmax * p.scale2;
-                    f = m == -INFINITY ? 0.f : ex2f(m2 - next);
-                    m = rowmax;
-                    m2 = next;
-                    sum *= f;
-                }
-                if (j > 0) {
-                    ok = wait_phase(odone, (j - 1) & 1, abort_flag);
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int c = half * HD; c < (half + 1) * HD; c += 16) {
-                        uint32_t o[16];
-                        tmem_ld16(tO + lanes + c, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tmem_st16(tO + lanes + c, o);
-                    }
-                }
+            const bool any = __any_sync(0xffffffffu, grown);
+            float f = 1.f;
+            if (grown) {
+                const float next = rowmax * p.scale2;
+                f = m == -INFINITY ? 0.f : ex2f(m2 - next);
+                m = rowmax;
+                m2 = next;
+                sum *= f;
             }
             uint64_t part[2] = {0ull, 0ull};
             const uint64_t scale = pack2(p.scale2, p.scale2), minus = pack2(-m2, -m2);
-            uint32_t w[3][16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float a, b;
-                unpack2(fma2(pack2(s[2 * i], s[2 * i + 1]), scale, minus), a, b);
-                a = ex2f(a);
-                b = ex2f(b);
-                part[i & 1] = add2(part[i & 1], pack2(a, b));
-                w[0][i] = next_term(a, b);
-                w[1][i] = next_term(a, b);
-                w[2][i] = next_term(a, b);
+            for (int g = 0; g < 2; ++g) {
+                uint32_t w[3][8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float a, b;
+                    unpack2(fma2(pack2(s[16 * g + 2 * i], s[16 * g + 2 * i + 1]), scale, minus), a, b);
+                    a = ex2f(a);
+                    b = ex2f(b);
+                    part[i & 1] = add2(part[i & 1], pack2(a, b));
+                    w[0][i] = next_term(a, b);
+                    w[1][i] = next_term(a, b);
+                    w[2][i] = next_term(a, b);
+                }
+#pragma unroll
+                for (int x = 0; x < 3; ++x) tmem_st8(tS + x * 32 + half * 16 + g * 8, w[x]);
             }
-#pragma unroll
-            for (int x = 0; x < 3; ++x) tmem_st16(tS + x * 32 + half * 16, w[x]);
             float a, b;
             unpack2(add2(part[0], part[1]), a, b);
             sum += a + b;
+            // the last tile's P V, before this one's takes its place
+            if (j > 0) {
+                ok = wait_phase(odone, (j - 1) & 1, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                fold();
+                if (any) {
+                    const uint64_t f2 = pack2(f, f);
+#pragma unroll
+                    for (int i = 0; i < HD / 4; ++i) o[i] = mul2(o[i], f2);
+                }
+            }
             tmem_st_wait();
             tc_fence_before();
-            // S of the last tile came before the last P V but one was done.  That is waited for here, while the last one cannot
-            // be done yet: afterwards a parity would not tell the two apart.
-            if (j == n - 1 && j > 0) ok = wait_phase(odone, (j - 1) & 1, abort_flag);
             __syncwarp();
             if (lane == 0) mbar_arrive(pfull + 8 * buf);
         }
-        if (ok && n > 0) ok = wait_phase(odone, (n - 1) & 1, abort_flag);
+        if (ok && n > 0) {
+            ok = wait_phase(odone, (n - 1) & 1, abort_flag);
+            tc_fence_after();
+            if (ok) fold();
+        }
         if (ok) {
             const float y = other(sum);
             sum = half ? y + sum : sum + y;      // (the same in both)
@@ -238,46 +262,32 @@ prompt_f32_kernel(const PromptParamsF p) {
             }
             if (tid == 0) slot[kPfRows * (HD + 2)] = again ? 1.f : 0.f;
 #pragma unroll
-            for (int k = 0; k < HD / 2; k += 16) {
-                const int c = half * (HD / 2) + k;
-                uint32_t a[16], b[16];
-                tmem_ld16(tO + lanes + c, a);
-                tmem_ld16(tO + lanes + HD + c, b);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    auto x = [&](int e) { return __uint_as_float(a[i + e]) + __uint_as_float(b[i + e]); };
-                    store4(slot + ((c + i) / 4 * kPfRows + rt) * 4, make_float4(x(0), x(1), x(2), x(3)));
-                }
+            for (int i = 0; i < HD / 2; i += 4) {
+                float4 v;
+                unpack2(o[i / 2], v.x, v.y);
+                unpack2(o[i / 2 + 1], v.z, v.w);
+                store4(slot + ((half * (HD / 2) + i) / 4 * kPfRows + rt) * 4, v);
             }
         } else if (ok && !again) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const bool has_row = rt < p.rpt * p.pack && r < it.rows;
             float* out = (float*)p.a.out + ((it.row + r) * p.a.n_q + head) * p.a.head_dim;
+            if (has_row)
 #pragma unroll
-            for (int k = 0; k < HD / 2; k += 16) {
-                const int c = half * (HD / 2) + k;
-                uint32_t a[16], b[16];
-                if (n > 0) {
-                    tmem_ld16(tO + lanes + c, a);
-                    tmem_ld16(tO + lanes + HD + c, b);
-                    tmem_ld_wait();
+                for (int i = 0; i < HD / 2; i += 4) {
+                    const int c = half * (HD / 2) + i;
+                    if (c >= p.a.head_dim) continue;
+                    float4 v;
+                    unpack2(o[i / 2], v.x, v.y);
+                    unpack2(o[i / 2 + 1], v.z, v.w);
+                    store4(out + c, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
                 }
-                if (has_row)
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        if (c + i >= p.a.head_dim) continue;
-                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        auto x = [&](int e) { return (__uint_as_float(a[i + e]) + __uint_as_float(b[i + e])) * inv; };
-                        if (sum != 0.f) v = make_float4(x(0), x(1), x(2), x(3));
-                        store4(out + c + i, v);
-                    }
-            }
         }
         if (ok && whole && again)
             for (int i = 0; i < p.pack; ++i) prompt_rows<float>(p.a, it, h * p.pack + i, warp, SOFT);
     } else if (warp < SOFT + SPLIT) {
         // ---- split ----
+        if constexpr (Sh::moved) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::split_regs));
         constexpr int LPR = HD / 4, RPI = 32 / LPR, ROWS = kPfKeys / SPLIT, NI = ROWS / RPI;      // lanes of a row; rows of a load; a warp's rows of a tile, and loads
         const int w = warp - SOFT, d = (lane % LPR) * 4, sub = lane / LPR;
         const bool in = d < p.a.head_dim;
@@ -374,6 +384,8 @@ prompt_f32_kernel(const PromptParamsF p) {
         }
     } else {
         // ---- MMAs ----
+        if constexpr (Sh::moved) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::mma_regs));
+        if (warp == SOFT + SPLIT) {
         constexpr uint32_t id_s = idesc_bf16(kPfKeys), id_o = idesc_bf16(HD) | (1u << 16);     // (bit 16: B with N innermost)
         const bool leader = elect_one();
         bool ok = n > 0;
@@ -382,7 +394,9 @@ prompt_f32_kernel(const PromptParamsF p) {
             tc_fence_after();
         };
         // terms of the products: the first to the first sum, the others to the second
-        constexpr int ta[6] = {0, 0, 1, 1, 0, 2}, tb[6] = {0, 1, 0, 1, 2, 0};
+        // (two bits of a word each: the six are a loop, whose descriptors as constants would take a hundred registers)
+        constexpr uint32_t terms_a = 0x850u, terms_b = 0x244u;      // 0 0 1 1 0 2 and 0 1 0 1 2 0, the first in the lowest bits
+        auto term = [](uint32_t terms, int x) { return (terms >> (2 * x)) & 3u; };
         // low words of descriptors (in 16 bytes) and their high word; V's: the blocks of 64 columns apart
         const uint32_t hi = (uint32_t)(smem_desc_sw128(0) >> 32), lead = (uint32_t)smem_desc_sw128(0), lead_v = (uint32_t)smem_desc_rows(0, Sh::kblk);
         const uint32_t q0 = lead + (sq >> 4), k0 = lead + (sk >> 4), v0 = lead_v + (sv >> 4);
@@ -390,12 +404,13 @@ prompt_f32_kernel(const PromptParamsF p) {
             const uint32_t tS = tmem + (j % NB) * 128;
             wait(kfull, j & 1);
             if (!ok) return;
-#pragma unroll
-            for (int x = 0; x < 6; ++x)
+#pragma unroll 1
+            for (int x = 0; x < 6; ++x) {
+                const uint32_t d = tS + (x ? 64 : 0), q = q0 + term(terms_a, x) * (Sh::qplane >> 4), kk = k0 + term(terms_b, x) * (Sh::kplane >> 4);
 #pragma unroll
                 for (int k = 0; k < HD / 16; ++k)
-                    if (leader) umma_ss(tS + (x ? 64 : 0), q0 + ta[x] * (Sh::qplane >> 4) + (k >> 2) * (Sh::qblk >> 4) + (k & 3) * 2,
-                            k0 + tb[x] * (Sh::kplane >> 4) + (k >> 2) * (Sh::kblk >> 4) + (k & 3) * 2, hi, id_s, x > 1 || k > 0);
+                    if (leader) umma_ss(d, q + (k >> 2) * (Sh::qblk >> 4) + (k & 3) * 2, kk + (k >> 2) * (Sh::kblk >> 4) + (k & 3) * 2, hi, id_s, x > 1 || k > 0);
+            }
             umma_commit_if(sfull + 8 * (j % NB), leader);
             umma_commit_if(kfree, leader);
         };
@@ -407,19 +422,21 @@ prompt_f32_kernel(const PromptParamsF p) {
             wait(vfull, j & 1);
             wait(pfull + 8 * (j % NB), (j / NB) & 1);
             if (!ok) break;
-#pragma unroll
-            for (int x = 0; x < 6; ++x)
+#pragma unroll 1
+            for (int x = 0; x < 6; ++x) {
+                const uint32_t d = tO + (x ? HD : 0), pp = tP + term(terms_a, x) * 32, vv = v0 + term(terms_b, x) * (Sh::kplane >> 4);
 #pragma unroll
                 for (int k = 0; k < kPfKeys / 16; ++k)
-                    if (leader) umma_ts(tO + (x ? HD : 0), tP + ta[x] * 32 + k * 8, v0 + tb[x] * (Sh::kplane >> 4) + k * (2048 >> 4), hi, id_o,
-                            j > 0 || x > 1 || k > 0);
+                    if (leader) umma_ts(d, pp + k * 8, vv + k * (2048 >> 4), hi, id_o, x > 1 || k > 0);
+            }
             umma_commit_if(odone, leader);
             umma_commit_if(vfree, leader);
         }
         if (!ok && n > 0) {      // products under way are waited for (with a limit) before the memory they use is given up
             volatile int none = 0;
             umma_commit_if(over, leader);
-            mbar_wait(over, 0, const_cast<volatile int*>(&none));
+            wait_phase(over, 0, const_cast<volatile int*>(&none));
+        }
         }
     }
     tc_fence_before();
@@ -434,6 +451,13 @@ int32_t prompt_f32_configure() {
     RSTQ_CUDA(cudaFuncSetAttribute((prompt_f32_kernel<64, true>), attr, PromptShapeF<64>::smem));
     RSTQ_CUDA(cudaFuncSetAttribute((prompt_f32_kernel<128, false>), attr, PromptShapeF<128>::smem));
     RSTQ_CUDA(cudaFuncSetAttribute((prompt_f32_kernel<128, true>), attr, PromptShapeF<128>::smem));
+    // registers are moved between warps: a block has to be launched with as many as are shared out
+    using Sh = PromptShapeF<128>;
+    cudaFuncAttributes a[2];
+    RSTQ_CUDA(cudaFuncGetAttributes(&a[0], (prompt_f32_kernel<128, false>)));
+    RSTQ_CUDA(cudaFuncGetAttributes(&a[1], (prompt_f32_kernel<128, true>)));
+    RSTQ_REQUIRE(a[0].numRegs >= Sh::launched && a[1].numRegs >= Sh::launched, RSTQ_E_CUDA, "prompt_f32_kernel was built for %d and %d registers",
+                 a[0].numRegs, a[1].numRegs);
     return RSTQ_OK;
 }
 

@@ -77,3 +77,83 @@ def test_decode_of_large_values_whose_weights_vanish(ctx, dtype, n_q, n_kv, d, l
     for b in (bq, bo):
         b.free()
     p.free()
+
+
+# ---- f32 prompts: all the terms, and sums over many keys -------------------------------------------------
+def f32_bound(d, n):
+    """Relative 2-norm of an f32 prompt's error, for scores of about 1 (2 at the most where the weight is).  An addition of the tensor core
+    cuts off at most 2^-23 of its sum, always towards zero:
+      * four of them in a row for the first terms of a tile's P V (the small terms' are 2^-8 of that);
+      * d / 16 of them for the first terms of a score, and five for the rest of it (the small terms, the exponential, the scale), times
+        the score, which moves a weight by that much;
+      * a tile's result is added to the row's in f32 to nearest, and so are the sums of weights: 2^-24 each, n / 64 of them, which
+        go either way."""
+    return 2.0 ** -23 * (4 + 2 * (d / 16 + 5) + (n / 64) ** 0.5)
+
+
+def f64_rows(q, k, v, rows, scale, causal=False):
+    """[len(rows), n_q, d] of one KV head in 64 bits; causal: q's last row is k's last."""
+    out = []
+    for r in rows:
+        m = len(k) - len(q) + r + 1 if causal else len(k)
+        s = q[r].astype(np.float64) @ k[:m, 0].astype(np.float64).T * scale
+        w = np.exp(s - s.max(-1, keepdims=True))
+        out.append(w / w.sum(-1, keepdims=True) @ v[:m, 0].astype(np.float64))
+    return np.array(out)
+
+
+def off(got, want):
+    return np.linalg.norm(got - want) / np.linalg.norm(want)
+
+
+def three_terms(x):
+    out = []
+    for _ in range(3):
+        t = (x.view(np.uint32) & 0xFFFF0000).view(np.float32)
+        out.append(t.astype(np.float64))
+        x = x - t
+    return out
+
+
+@pytest.mark.parametrize("d,n", [(64, 40), (64, 500), (128, 130)])
+def test_the_f32_bound_tells_terms_that_are_left_out(d, n):
+    """Of the six products of terms, three alone miss it (planted in a model here), all six hold it by far."""
+    q, k, v = normal(1, 4, d), normal(2, n, d), normal(3, n, d)
+    kept = [(0, 0), (0, 1), (1, 0), (1, 1), (0, 2), (2, 0)]
+
+    def product(a, b, pairs):
+        ta, tb = three_terms(a.astype(np.float32)), three_terms(b.astype(np.float32))
+        return sum(ta[i] @ tb[j] for i, j in pairs)
+
+    want = f64_rows(q[:, None], k[:, None], v[:, None], range(4), d ** -0.5)[:, 0]
+    for s_pairs, p_pairs, holds in ((kept, kept, True), (kept[:3], kept, False), (kept, kept[:3], False), (kept[:3], kept[:3], False)):
+        s = product(q, np.ascontiguousarray(k.T), s_pairs) * d ** -0.5
+        w = np.exp(s - s.max(-1, keepdims=True))
+        got = product(w, v, p_pairs) / w.sum(-1, keepdims=True)
+        if holds:
+            assert off(got, want) < f32_bound(d, n) / 10
+        else:
+            assert off(got, want) > 2 * f32_bound(d, n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,rows,n,values", [
+    (64, 40, 40, "normal"), (64, 500, 500, "normal"), (128, 130, 130, "normal"), (96, 300, 300, "normal"), (128, 1300, 1300, "normal"),
+    (64, 1300, 4000, "positive"), (128, 1300, 4000, "positive"), (64, 1300, 16000, "positive"), (128, 1300, 16000, "positive"),
+    (64, 20, 16000, "positive"), (128, 20, 16000, "positive"), (64, 1300, 16000, "normal")])      # (20 rows: keys in parts)
+def test_f32_prompts_hold_f32(ctx, d, rows, n, values):
+    n_q = 16
+    q, k, v = normal(1, rows, n_q, d), normal(2, n, 1, d), normal(3, n, 1, d)
+    if values == "positive":
+        v = np.abs(v) + 0.5
+    up = ctx.array_to_buffer
+    bq, bk, bv, cq, ck = up(q), up(k), up(v), up(np.array([0, rows], np.int32)), up(np.array([0, n], np.int32))
+    bo = ctx.make_buffer(rows * n_q * d, np.float32)
+    ctx.prompt_attention(bq, bk, bv, bo, cq, ck, rows, n, 1, n_q, n_q, 1, d, d ** -0.5, True, L.F32)
+    ctx.sync()
+    pick = sorted({0, 1, rows // 2, rows - 2, rows - 1})
+    got, want = bo.download().reshape(rows, n_q, d)[pick], f64_rows(q, k, v, pick, d ** -0.5, True)
+    for i, r in enumerate(pick):
+        assert off(got[i], want[i]) <= f32_bound(d, n), (r, off(got[i], want[i]))
+    for b in (bq, bk, bv, bo, cq, ck):
+        b.free()
