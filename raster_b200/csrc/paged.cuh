@@ -17,6 +17,14 @@ constexpr int64_t kMaxRows = 1ll << 30;     // packed rows of a call
 constexpr int kStatusPage = 1;              // word of DeviceState::status: a table named a page outside the pool
 constexpr int kPagedGroup = 16;             // query heads of a KV head that one thread block of the decode kernel serves
 
+// What attention keeps in memory between (and for long sums, beside) the registers of its blocks of threads: slots of floats.
+constexpr int kPromptSlots = 512;      // items of a call whose blocks' keys are cut into parts
+// a slot, in floats: up to 256 rows' sums (of more than 128 columns 128 rows'), four columns at a time; their references; their sums of weights; whether they have to be taken again
+template <int HD>
+__host__ __device__ constexpr int prompt_slot() { return (HD > 128 ? 128 : 256) * (HD + 2) + 32; }
+static_assert(prompt_slot<256>() <= prompt_slot<128>() && prompt_slot<64>() <= prompt_slot<128>(), "the slots are laid out for 128 columns");
+constexpr int64_t kPromptSlotFloats = (int64_t)kPromptSlots * prompt_slot<128>();
+
 template <typename T>
 struct Elem;
 template <>

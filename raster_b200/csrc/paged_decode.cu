@@ -59,6 +59,7 @@ struct DecodeParams {
     int* status;
     int box;                                          // rows of a box: min(page, tile)
     const int64_t* start;                             // units of a head before each sequence; null: few sequences
+    float* sums;                                      // [blocks][kDecWarps] x dec_sums: bf16, what warps have summed over kDecFold tiles
 };
 template <typename T>
 __host__ __device__ constexpr int dec_tile() { return sizeof(T) == 2 ? 64 : 32; }
@@ -67,6 +68,13 @@ __host__ __device__ constexpr int dec_stage() { return dec_tile<T>() * HD * (int
 // query heads of a KV head that one pass serves: what its sums leave of the registers
 template <typename T>
 __host__ __device__ constexpr int dec_heads() { return sizeof(T) == 2 ? kPagedGroup : kPagedGroup / 2; }
+// bf16: tiles that a warp sums up in its MMAs' registers.  An MMA's additions cut off, towards zero, so a longer sum is taken out every so often and
+// added to one in memory.  (300 sequences over the same 2^20 positions, a block each: results 3.7e-3 too small without, no smaller than those of
+// one sequence, which all blocks share, with it.  It costs groups of more than eight heads 2 %; every tile's sum taken out, in registers, 6 to 16.)
+constexpr int kDecFold = 512;
+// ... in floats: a warp's registers and maxima
+template <int HD, int GH>
+__host__ __device__ constexpr int dec_sums() { return 32 * (HD * GH / 32 + GH / 4); }
 // a slot, in floats: the heads' weighted V, their maxima, their sums of weights
 template <int HD>
 __host__ __device__ constexpr int dec_slot() { return kPagedGroup * (HD + 2); }
@@ -427,6 +435,25 @@ paged_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap km
                     }
             __syncwarp();
             if (lane == 0) mbar_arrive(qempty + 8 * sq);
+            // the weighted V so far to the sums in memory, or these to it
+            float* sums = p.sums + (blockIdx.x * kDecWarps + warp) * dec_sums<HD, GH>() + lane;
+            auto fold = [&](bool first, bool last) {
+                constexpr int X = MT * NT * 4;
+                float f[NH];
+#pragma unroll
+                for (int x = 0; x < NH; ++x) {
+                    f[x] = first ? 0.f : ex2(sums[(X + x) * 32] - finite_max(m[x]));
+                    if (!last) sums[(X + x) * 32] = m[x];
+                }
+#pragma unroll
+                for (int x = 0; x < X; ++x) {
+                    if (!first) o[x] = fmaf(sums[x * 32], f[(x >> 2) % NT * 2 + (x & 1)], o[x]);
+                    if (!last) {
+                        sums[x * 32] = o[x];
+                        o[x] = 0.f;
+                    }
+                }
+            };
             // rows and pieces of the four 8 x 8 matrices of a load: K as it lies, V transposed
             const int kr = lane & 15, kc = lane >> 4, vr = (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;
             for (int i = 0; i < n; ++i) {
@@ -526,7 +553,9 @@ paged_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap km
                     }
                 }
                 release();
+                if ((i + 1) % kDecFold == 0) fold(i + 1 == kDecFold, false);
             }
+            if (n >= kDecFold) fold(false, true);
 #pragma unroll
             for (int x = 0; x < NH; ++x) {
 #pragma unroll
@@ -848,7 +877,10 @@ int32_t launch_paged_decode(DeviceState& ds, const PromptArgs& a, int* launches)
     if (rc != RSTQ_OK) return rc;
     const int64_t blocks = (a.head_dim > 128 ? dec_blocks<256>() : dec_blocks<128>()) * (int64_t)ds.sm_count;
     const int64_t slot = a.head_dim > 128 ? dec_slot<256>() : dec_slot<128>();
-    RSTQ_REQUIRE(2 * blocks * slot * 4 <= ds.partials_bytes && blocks <= ds.counters_len, RSTQ_E_LIMIT, "%lld thread blocks", (long long)blocks);
+    constexpr int sums = kDecWarps * dec_sums<256, kPagedGroup>();
+    p.sums = ds.prompt_slots;
+    RSTQ_REQUIRE(2 * blocks * slot * 4 <= ds.partials_bytes && blocks <= ds.counters_len && blocks * sums <= kPromptSlotFloats, RSTQ_E_LIMIT,
+                 "%lld thread blocks", (long long)blocks);
     *launches = 1;
     p.start = nullptr;
     if (a.seqs > kDecSums) {

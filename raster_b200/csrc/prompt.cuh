@@ -8,11 +8,6 @@ namespace rstq {
 
 // ---- keys cut into parts ----
 // What a part of a block of rows has found goes to its slot; a second launch joins the parts in their order.  (prompt_attn.cu)
-constexpr int kPromptSlots = 512;      // items of a call whose blocks' keys are cut into parts
-// a slot, in floats: up to 256 rows' sums (of more than 128 columns 128 rows'), four columns at a time; their references; their sums of weights; whether they have to be taken again
-template <int HD>
-__host__ __device__ constexpr int prompt_slot() { return (HD > 128 ? 128 : 256) * (HD + 2) + 32; }
-static_assert(prompt_slot<256>() <= prompt_slot<128>() && prompt_slot<64>() <= prompt_slot<128>(), "the slots are laid out for 128 columns");
 struct PromptItem;
 struct PromptJoin {
     PromptArgs a;

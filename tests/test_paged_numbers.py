@@ -157,3 +157,49 @@ def test_f32_prompts_hold_f32(ctx, d, rows, n, values):
         assert off(got[i], want[i]) <= f32_bound(d, n), (r, off(got[i], want[i]))
     for b in (bq, bk, bv, bo, cq, ck):
         b.free()
+
+
+# ---- bf16 over a million positions -----------------------------------------------------------------------
+class Repeated:
+    """A cache of 2^20 positions a sequence, whose pages are the same 64 over and over, in other orders: attention over all of it is attention
+    over those 64.  V is 1 or somewhat more or less, so that what is lost of a sum is lost of the result."""
+    n, page = 1 << 20, 256
+
+    def __init__(self, ctx, seqs, d):
+        rng = np.random.default_rng(seqs + d)
+        some = 64 * self.page
+        self.k = pm.decode(pm.encode(normal(7, some, 1, d), "bf16"), "bf16")
+        self.v = pm.decode(pm.encode(0.5 + rng.random((some, 1, d)).astype(np.float32), "bf16"), "bf16")
+        self.width = self.n // self.page
+        order = np.concatenate([rng.permutation(64) for _ in range(self.width // 64)]).astype(np.int32)
+        self.bufs = [ctx.array_to_buffer(x) for x in (pm.encode(self.k, "bf16"), pm.encode(self.v, "bf16"), np.stack([np.roll(order, 64 * b) for b in range(seqs)]),
+                                                      np.full(seqs, self.n, np.int32))]
+        self.bk, self.bv, self.bt, self.bl = self.bufs
+
+    def check(self, got, q, d):
+        """A step of the result's own (h), and 2^-11 of it: a thousand additions that cut off 2^-23 of a growing sum, over and over (2^-14), the
+        scores' rounding and, of prompts, that of the weights, whose mean over so many is far below that."""
+        for i in range(len(q)):
+            want = f64_rows(q[i:i + 1], self.k, self.v, [0], d ** -0.5)[0]
+            assert (np.abs(got[i] - want) <= (pm.HALF["bf16"] + 2.0 ** -11) * want).all(), (i, (got[i] / want - 1).mean(), np.abs(got[i] / want - 1).max())
+
+    def free(self):
+        for b in self.bufs:
+            b.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q,d,seqs", [(4, 128, 300), (16, 64, 296), (12, 256, 150)])
+def test_decode_over_a_million_positions(ctx, n_q, d, seqs):
+    """As many sequences as there are blocks of threads: each sums one by itself."""
+    x = Repeated(ctx, seqs, d)
+    q = pm.decode(pm.encode(normal(5, seqs, n_q, d), "bf16"), "bf16")
+    bq, bo = ctx.array_to_buffer(pm.encode(q, "bf16")), ctx.make_buffer(seqs * n_q * d, np.uint16)
+    ctx.paged_decode_attention(bq, x.bk, x.bv, bo, x.bt, x.bl, seqs, n_q, n_q, 1, d, x.page, 64, x.width, d ** -0.5, L.BF16)
+    ctx.sync()
+    got = pm.decode(bo.download(), "bf16").reshape(seqs, n_q, d)
+    pick = [0, seqs // 3, seqs - 1]
+    x.check(got[pick], q[pick], d)
+    bq.free()
+    bo.free()
+    x.free()
