@@ -34,6 +34,7 @@
 // and a launch 5 to 7 us until the first S.  512 rows behind 16000 keys 158 us (in parts; 255 with one query tile per block), 2 rows 32 us.
 // A polynomial in place of a part of the exponentials was slower, so were 64 keys per tile with two places for S.
 #include <algorithm>
+#include <type_traits>
 
 #include "prompt.cuh"
 
@@ -41,6 +42,9 @@ namespace rstq {
 
 constexpr int kPrThreads = 384;      // two warpgroups of softmax; copies, MMAs, V's edges
 constexpr int kPrRows = 128;         // rows of a query tile, keys of a tile
+// Tiles of keys whose P V stays in tensor memory.  Its additions cut off, towards zero, so after as many O goes to a slot in memory, where it is added
+// to the rows' sums in f32, and starts anew: 2^20 keys lost 7e-3 of a result, 2^18 1.3e-3; now 1e-4.
+constexpr int kPromptFold = 256;
 template <int HD>
 struct PromptShape {
     // (of 256 columns one query tile: K and V of a step and Q take 192 KB, S and O 384 columns of tensor memory)
@@ -68,8 +72,27 @@ struct PromptWork {
     int h;                           // query head, or the packed ones' KV head
     int item;
 };
-// PARTS: a block's keys may be cut into parts.
-template <int HD, bool PARTS>
+// 16 columns of a row, and g times (`there`) what a slot of R rows has of them; `back`: to the slot.
+template <int R>
+__device__ __forceinline__ void add_slot(uint32_t (&o)[16], float* slot, bool there, float g, bool back) {
+#pragma unroll
+    for (int u = 0; u < 16; u += 4) {
+        float* at = slot + u * R;
+        float4 v = make_float4(__uint_as_float(o[u]), __uint_as_float(o[u + 1]), __uint_as_float(o[u + 2]), __uint_as_float(o[u + 3]));
+        if (there) {
+            const float4 x = load4(at);
+            v = make_float4(fmaf(x.x, g, v.x), fmaf(x.y, g, v.y), fmaf(x.z, g, v.z), fmaf(x.w, g, v.w));
+        }
+        o[u] = __float_as_uint(v.x);
+        o[u + 1] = __float_as_uint(v.y);
+        o[u + 2] = __float_as_uint(v.z);
+        o[u + 3] = __float_as_uint(v.w);
+        if (back) store4(at, v);
+    }
+}
+// PARTS: a block's keys may be cut into parts.  LONG: they may be more than kPromptFold tiles.  (Calls that cannot have as many do without: 12 ragged
+// prompts 79 us, and 82 with it; 512 rows behind 16000 keys 163 and 167; of 64 columns it makes no difference for the worse.)
+template <int HD, bool PARTS, bool LONG>
 __global__ void __launch_bounds__(kPrThreads, 1)
 prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
               const __grid_constant__ CUtensorMap vmap) {
@@ -180,6 +203,8 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             // keys of this row, of the tile's first, from the item's first on
             const int mine = sees(it, r) - it.j0 * kPrRows, least = sees(it, t * p.rpt) - it.j0 * kPrRows;
             float m = -INFINITY, m2 = 0.f, sum = 0.f;      // running maximum of S; scale2 times it (0: nothing seen yet)
+            auto slot_of = [&]() { return p.join.part + (int64_t)(PARTS ? x.item : (int)blockIdx.x) * prompt_slot<HD>(); };
+            float ref = -INFINITY;                         // what the sums in the slot refer to, as m2 (-inf: nothing)
             for (int j = 0; j < steps; ++j) {
                 ok = wait_phase<true>(sfull + 8 * t, (c + j) & 1, abort_flag);
                 if (!ok) break;
@@ -201,7 +226,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     for (int u = 0; u < 4; ++u) top[u] = fmaxf(fmaxf(top[u], __uint_as_float(s[i + u])), __uint_as_float(s[i + 4 + u]));
                 const float rowmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                 const bool grown = rowmax > m && !(rowmax * p.scale2 <= m2 + kGrow && m != -INFINITY);
-                if (__any_sync(0xffffffffu, grown)) {
+                if (__any_sync(0xffffffffu, grown) || (LONG && j % kPromptFold == 0)) {
                     float f = 1.f;
                     if (grown) {
                         const float next = rowmax * p.scale2;
@@ -214,14 +239,18 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                         ok = wait_phase<true>(odone + 8 * t, (c + j - 1) & 1, abort_flag);
                         if (!ok) break;
                         tc_fence_after();
+                        const bool taken = LONG && j % kPromptFold == 0;
+                        const float g = j > kPromptFold ? ex2f(ref - m2) : 0.f;
 #pragma unroll 1
                         for (int i = 0; i < HD; i += 16) {
                             uint32_t o[16];
                             tmem_ld16_wait(tOt + i, o);
 #pragma unroll
                             for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
-                            tmem_st16(tOt + i, o);
+                            if (taken) add_slot<R>(o, slot_of() + (i / 4 * R + slot_row) * 4, j > kPromptFold, g, true);
+                            else tmem_st16(tOt + i, o);
                         }
+                        if (taken) ref = m == -INFINITY ? m : m2;
                     }
                 }
                 const uint64_t scale = pack2(p.scale2, p.scale2), minus = pack2(-m2, -m2);
@@ -262,7 +291,18 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             // (a part of a block's keys: what it has found goes to its slot, for prompt_join_kernel)
             const bool whole = !PARTS || it.parts == 1;
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            float* slot = p.join.part + (whole ? 0 : (int64_t)x.item * prompt_slot<HD>());
+            if (LONG && steps > kPromptFold) {      // what is in the slot back to O
+                const float g = ex2f(ref - m2);
+#pragma unroll 1
+                for (int i = 0; i < HD; i += 16) {
+                    uint32_t o[16];
+                    tmem_ld16_wait(tOt + i, o);
+                    add_slot<R>(o, slot_of() + (i / 4 * R + slot_row) * 4, true, g, false);
+                    tmem_st16(tOt + i, o);
+                }
+                tmem_st_wait();
+            }
+            float* slot = slot_of();
             if (!whole || !again)
 #pragma unroll
                 for (int i = 0; i < HD; i += 32) {
@@ -437,7 +477,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                                 wait((half ? pfull : phalf) + 8 * t, (c[t] + j) & 1);
                                 if (!ok) break;
 #pragma unroll
-                                for (int k = half * 4; k < half * 4 + 4; ++k) if (leader) umma_ts(tO[t], tS[t] + k * 8, b + k * (2048 >> 4), hi, id_o, j > 0 || k > 0);
+                                for (int k = half * 4; k < half * 4 + 4; ++k) if (leader) umma_ts(tO[t], tS[t] + k * 8, b + k * (2048 >> 4), hi, id_o, (LONG ? j % kPromptFold : j) > 0 || k > 0);
                             }
                             if (ok) umma_commit_if(odone + 8 * t, leader);
                         }
@@ -625,12 +665,16 @@ int32_t launch_prompt_join(DeviceState& ds, const PromptJoin& j) {
 
 int32_t prompt_configure(DeviceState& ds) {
     constexpr auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<64, false>), attr, PromptShape<64>::smem));
-    RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<64, true>), attr, PromptShape<64>::smem));
-    RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<128, false>), attr, PromptShape<128>::smem));
-    RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<128, true>), attr, PromptShape<128>::smem));
-    RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<256, false>), attr, PromptShape<256>::smem));
-    RSTQ_CUDA(cudaFuncSetAttribute((prompt_kernel<256, true>), attr, PromptShape<256>::smem));
+    auto set = [&](auto hd) {
+        constexpr int HD = decltype(hd)::value, smem = PromptShape<HD>::smem;
+        cudaError_t e = cudaFuncSetAttribute((prompt_kernel<HD, false, false>), attr, smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute((prompt_kernel<HD, false, true>), attr, smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute((prompt_kernel<HD, true, false>), attr, smem);
+        return e == cudaSuccess ? cudaFuncSetAttribute((prompt_kernel<HD, true, true>), attr, smem) : e;
+    };
+    RSTQ_CUDA(set(std::integral_constant<int, 64>()));
+    RSTQ_CUDA(set(std::integral_constant<int, 128>()));
+    RSTQ_CUDA(set(std::integral_constant<int, 256>()));
     const size_t slots = (size_t)kPromptSlots * (prompt_slot<128>() * 4 + sizeof(PromptItem));
     RSTQ_CUDA(cudaMalloc((void**)&ds.prompt_slots, slots + 64));
     RSTQ_CUDA(cudaMemsetAsync((char*)ds.prompt_slots + slots, 0, 64, ds.stream));
@@ -686,11 +730,17 @@ int32_t launch_prompt(DeviceState& ds, const PromptArgs& a, int* launches) {
         p.a.start = ds.seq_starts;
         ++*launches;
     }
-    const dim3 grid((unsigned)(parts ? p.sms : std::min<int64_t>(blocks, ds.sm_count)));
-    auto go = [&](auto kernel, int smem) { return launch_pdl(kernel, grid, dim3(kPrThreads), (size_t)smem, ds, p, qmap, kmap, vmap); };
-    if (a.head_dim <= 64) RSTQ_CUDA(parts ? go(prompt_kernel<64, true>, PromptShape<64>::smem) : go(prompt_kernel<64, false>, PromptShape<64>::smem));
-    else if (a.head_dim <= 128) RSTQ_CUDA(parts ? go(prompt_kernel<128, true>, PromptShape<128>::smem) : go(prompt_kernel<128, false>, PromptShape<128>::smem));
-    else RSTQ_CUDA(parts ? go(prompt_kernel<256, true>, PromptShape<256>::smem) : go(prompt_kernel<256, false>, PromptShape<256>::smem));
+    const dim3 grid((unsigned)(parts ? p.sms : std::min<int64_t>(blocks, std::min(ds.sm_count, kPromptSlots))));
+    const bool many = (a.kv.table ? (int64_t)a.kv.width << a.kv.shift : a.kv_rows) > kPromptFold * kPrRows;
+    auto go = [&](auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        auto run = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(kPrThreads), (size_t)PromptShape<HD>::smem, ds, p, qmap, kmap, vmap); };
+        if (parts) return many ? run(prompt_kernel<HD, true, true>) : run(prompt_kernel<HD, true, false>);
+        return many ? run(prompt_kernel<HD, false, true>) : run(prompt_kernel<HD, false, false>);
+    };
+    const cudaError_t e = a.head_dim <= 64 ? go(std::integral_constant<int, 64>()) : a.head_dim <= 128 ? go(std::integral_constant<int, 128>())
+                                                                                                     : go(std::integral_constant<int, 256>());
+    RSTQ_CUDA(e);
     return parts ? launch_prompt_join(ds, p.join) : RSTQ_OK;
 }
 

@@ -203,3 +203,20 @@ def test_decode_over_a_million_positions(ctx, n_q, d, seqs):
     bq.free()
     bo.free()
     x.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q,d,rows", [(16, 128, 1300), (16, 64, 1300), (8, 256, 2500), (4, 64, 5), (16, 128, 40), (2, 256, 130)])
+def test_prompts_over_a_million_positions(ctx, n_q, d, rows):
+    """Enough rows that the keys are not cut into parts, and few, whose parts are 2^16 keys and more."""
+    x = Repeated(ctx, 1, d)
+    q = pm.decode(pm.encode(normal(5, rows, n_q, d), "bf16"), "bf16")
+    bq, bo, cu = ctx.array_to_buffer(pm.encode(q, "bf16")), ctx.make_buffer(rows * n_q * d, np.uint16), ctx.array_to_buffer(np.array([0, rows], np.int32))
+    ctx.paged_prompt_attention(bq, x.bk, x.bv, bo, x.bt, cu, x.bl, rows, 1, n_q, n_q, 1, d, x.page, 64, x.width, d ** -0.5, False, L.BF16)
+    ctx.sync()
+    got = pm.decode(bo.download(), "bf16").reshape(rows, n_q, d)
+    pick = sorted({0, rows // 2, rows - 1})
+    x.check(got[pick], q[pick], d)
+    for b in (bq, bo, cu):
+        b.free()
+    x.free()
