@@ -463,7 +463,9 @@ RSTQ_API int32_t rstq_gqa_decode_attention(rstq_ctx* ctx, rstq_buf* q, rstq_buf*
  * (graphs replayed on two streams) need a context each.
  *
  *   rstq_paged_rope_append       q turned to qout [rows][n_q][head_dim]; k turned and v written to their pages, in `dtype`
- *                                (q, k, v are in_dtype).  cu may be NULL: rows == seqs, one per sequence.  qout may be q
+ *                                (q, k, v are in_dtype).  cu may be NULL: rows == seqs, one per sequence, for its
+ *                                last position; a sequence of length 0 that holds no page (its first entry is -1, as in a new cache and behind
+ *                                rstq_pages_free) is idle then, and its row left out without an error.  qout may be q
  *                                where q is packed and of the type stored.
  *   rstq_paged_decode_attention  one row of q per sequence against all its positions; a sequence of none gives zeros.
  *   rstq_prompt_attention        rows of packed sequences (cu_q) against packed keys and values [kv_rows][n_kv][head_dim]

@@ -64,7 +64,8 @@ paged_rope_append_kernel(const AppendParams p, const int per_block) {
             const int64_t behind = p.cu ? (int64_t)p.cu[b + 1] - t : 1;    // rows from this one to the sequence's end
             pos = (int64_t)p.kv.lens[b] - behind;
             if (pos >= 0 && pos < ((int64_t)p.kv.width << p.kv.shift)) row = kv_row(p.kv, b, 0, pos);
-            if (row < 0) p.kv.status[kStatusPage] = 1;
+            // (a sequence that holds nothing has no row in a step of all sequences: its slot is idle, which is no error)
+            if (row < 0 && (p.cu || pos >= 0 || p.kv.table[(int64_t)b * p.kv.width] != -1)) p.kv.status[kStatusPage] = 1;
         }
         s_row[tid] = row;
         s_pos[tid] = pos;
