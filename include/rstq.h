@@ -449,7 +449,7 @@ RSTQ_API int32_t rstq_gqa_decode_attention(rstq_ctx* ctx, rstq_buf* q, rstq_buf*
  *   head_dim: rows as in the contiguous caches [position][n_kv][head_dim], of which a pool with a table that counts up is
  *   one.  n_pages, max_pages <= 2^20.
  * table int32 [seqs][max_pages]: the pages of each sequence in order, what lies behind them is not read.  lens int32 [seqs]:
- *   positions of each sequence, the call's own rows among them; beyond max_pages * page it counts as that.
+ *   positions of each sequence, the call's own rows among them; those from max_pages * page on have no page.
  * cu int32 [seqs + 1]: rows of a packed array, sequence b has rows [cu[b], cu[b+1]).  Its rows are its LAST ones: row t
  *   stands at position lens[b] - (cu[b+1] - t).  Rows that no sequence has are left as they were.
  * seqs <= 65536; all of these arrays are read on the device, so one recorded graph serves every step.

@@ -82,7 +82,7 @@ __device__ __forceinline__ void packed_range(const int32_t* cu, int b, int64_t r
     *first = clamp64(cu[b], 0, rows);
     *last = clamp64(cu[b + 1], *first, rows);
 }
-// Positions of sequence b; packed: *row0 = its first row.  A length beyond the sequence's pages counts as their end.
+// Positions of sequence b that have a place; packed: *row0 = its first row.
 __device__ __forceinline__ int64_t kv_length(const KvPlace& kv, int b, int64_t* row0) {
     if (kv.table) {
         *row0 = 0;
@@ -92,6 +92,9 @@ __device__ __forceinline__ int64_t kv_length(const KvPlace& kv, int b, int64_t* 
     packed_range(kv.cu, b, kv.rows, row0, &last);
     return last - *row0;
 }
+// Where sequence b, of n positions that have a place, ends: the position behind its last row.  That is n, but for a length beyond the
+// sequence's pages.
+__device__ __forceinline__ int64_t kv_end(const KvPlace& kv, int b, int64_t n) { return kv.table && kv.lens[b] > n ? kv.lens[b] : n; }
 // Row of the pool (of the packed array) that holds position `pos` of sequence b; -1: the table names no page of the pool.
 __device__ __forceinline__ int64_t kv_row(const KvPlace& kv, int b, int64_t row0, int64_t pos) {
     if (!kv.table) return row0 + pos;
@@ -172,15 +175,15 @@ struct RowState {
     static constexpr int V = Elem<T>::kVec, C = 256 / (32 * V) < 1 ? 1 : 256 / (32 * V);   // elements of a piece; pieces of a lane
     float o[C][V], m, l;
 };
-// Row `row` of head h, `behind` rows from its sequence's end (its own among them), against positions first .. first + kRowPos - 1, and
-// so on every `step`.  True: a position had no page.
+// Row `row` of head h, which sees `len` positions of sequence b, against positions first .. first + kRowPos - 1, and so on every `step`.
+// True: a position had no page.
 template <typename T>
-__device__ __forceinline__ bool attend_row(const PromptArgs& p, int b, int64_t row, int h, int64_t behind, int64_t first, int64_t step,
+__device__ __forceinline__ bool attend_row(const PromptArgs& p, int b, int64_t row, int h, int64_t len, int64_t first, int64_t step,
                                            RowState<T>* st) {
     constexpr int V = RowState<T>::V, C = RowState<T>::C;
     const int lane = threadIdx.x & 31, hd = p.head_dim, hkv = h / p.group;
-    int64_t row0, len = kv_length(p.kv, b, &row0);
-    if (p.causal) len = clamp64(len - behind + 1, 0, len);
+    int64_t row0;
+    kv_length(p.kv, b, &row0);
     float q[C][V];
     st->m = -INFINITY;
     st->l = 0.f;

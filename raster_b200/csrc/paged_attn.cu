@@ -206,8 +206,10 @@ attention_rows_kernel(const PromptArgs p) {
         if (b < 0) return;
         behind = (int64_t)p.cu_q[b + 1] - row;
     }
+    int64_t row0;
+    const int64_t keys = kv_length(p.kv, b, &row0), sees = p.causal ? clamp64(kv_end(p.kv, b, keys) - behind + 1, 0, keys) : keys;
     RowState<T> st;
-    if (attend_row(p, b, row, h, behind, warp * kRowPos, kRowWarps * kRowPos, &st) && lane == 0) p.kv.status[kStatusPage] = 1;
+    if (attend_row(p, b, row, h, sees, warp * kRowPos, kRowWarps * kRowPos, &st) && lane == 0) p.kv.status[kStatusPage] = 1;
 #pragma unroll
     for (int c = 0; c < RowState<T>::C; ++c)
 #pragma unroll

@@ -184,26 +184,27 @@ __device__ __forceinline__ float ex2f(float x) {
 struct PromptItem {
     int b, rows;           // sequence, rows of it in this block (0: nothing left to do)
     int64_t row;           // the first one, packed
-    int behind;            // rows from the first one to the sequence's end
+    int place;             // the first one's position in the sequence (below 0, or beyond its keys: it has none)
     int keys, row0;        // keys of the sequence; packed: the first one's row
     int j0, j1;            // tiles of keys
     int part, parts;       // which of how many parts of the block's keys
     // keys that row r of the block sees
     __device__ __forceinline__ int sees(int r, int causal) const {
-        return causal ? min(max(keys - behind + 1 + r, 0), keys) : keys;
+        return causal ? min(max(place + 1 + r, 0), keys) : keys;
     }
 };
 constexpr int kMaxParts = 16, kPartRounds = 3;
 inline int prompt_sms(const DeviceState& ds) { return ds.sm_count < kPromptSlots / kPartRounds ? ds.sm_count : kPromptSlots / kPartRounds; }
 // One lane's sequence cut into blocks of `per` rows, and the tiles of `tile` keys that block k sees.
 struct PromptSequence {
-    int n, keys, row0, first, blocks;
+    int n, keys, end, row0, first, blocks;      // rows; keys; the position behind its last row; packed: first key; first row; blocks
     __device__ __forceinline__ void load(const PromptArgs& a, int b, int per) {
-        n = keys = row0 = first = 0;
+        n = keys = end = row0 = first = 0;
         if (b < a.seqs) {
             int64_t f, l, r;
             packed_range(a.cu_q, b, a.rows, &f, &l);
             keys = (int)kv_length(a.kv, b, &r);
+            end = (int)min(kv_end(a.kv, b, keys), keys + kMaxRows);      // (farther, every row sees everything too)
             n = (int)(l - f);
             first = (int)f;
             row0 = (int)r;
@@ -211,7 +212,7 @@ struct PromptSequence {
         blocks = (n + per - 1) / per;
     }
     __device__ __forceinline__ int tiles(int k, int per, int causal, int tile) const {
-        const int last = min(n, (k + 1) * per) - 1, s = causal ? min(max(keys - n + 1 + last, 0), keys) : keys;
+        const int last = min(n, (k + 1) * per) - 1, s = causal ? min(max(end - n + 1 + last, 0), keys) : keys;
         return (s + tile - 1) / tile;
     }
 };
@@ -290,8 +291,8 @@ static __device__ __forceinline__ PromptItem prompt_block(const PromptArgs& a, i
         it.b = b;
         it.keys = q.keys;
         it.row = q.first + (int64_t)k * per;
-        it.behind = q.n - k * per;
-        it.rows = it.behind < per ? it.behind : per;
+        it.place = q.end - q.n + k * per;
+        it.rows = min(q.n - k * per, per);
         it.row0 = q.row0;
         it.parts = 1;
         it.part = it.j0 = 0;
@@ -317,10 +318,11 @@ static __device__ __forceinline__ PromptItem prompt_block(const PromptArgs& a, i
         q.n = __shfl_sync(0xffffffffu, q.n, src);
         if (k < 0 || (int64_t)k * per >= q.n) return it;
         it.keys = q.keys = __shfl_sync(0xffffffffu, q.keys, src);
+        q.end = __shfl_sync(0xffffffffu, q.end, src);
         it.b = b0 + 31 - src;
         it.row = __shfl_sync(0xffffffffu, q.first, src) + (int64_t)k * per;
-        it.behind = q.n - k * per;
-        it.rows = it.behind < per ? it.behind : per;
+        it.place = q.end - q.n + k * per;
+        it.rows = min(q.n - k * per, per);
         it.row0 = __shfl_sync(0xffffffffu, q.row0, src);
         it.parts = 1;
         it.part = it.j0 = 0;
@@ -357,6 +359,7 @@ static __device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, in
         const bool whole = __shfl_sync(0xffffffffu, m, src) == blocks;
         q.n = __shfl_sync(0xffffffffu, q.n, src);
         q.keys = __shfl_sync(0xffffffffu, q.keys, src);
+        q.end = __shfl_sync(0xffffffffu, q.end, src);
         int k = blocks - 1 - (whole ? left : 0), parts = 1;
         if (!whole)
             for (;; --k) {
@@ -369,8 +372,8 @@ static __device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, in
         const int w = q.tiles(k, per, a.causal, tile);
         it.b = b0 + 31 - src;
         it.row = __shfl_sync(0xffffffffu, q.first, src) + (int64_t)k * per;
-        it.behind = q.n - k * per;
-        it.rows = it.behind < per ? it.behind : per;
+        it.place = q.end - q.n + k * per;
+        it.rows = min(q.n - k * per, per);
         it.keys = q.keys;
         it.row0 = __shfl_sync(0xffffffffu, q.row0, src);
         it.parts = parts;
@@ -390,7 +393,7 @@ __device__ __forceinline__ void prompt_rows(const PromptArgs& a, const PromptIte
     bool bad = false;
     for (int r = warp; r < it.rows; r += warps) {
         S st;
-        bad |= attend_row(a, it.b, it.row + r, h, it.behind - r, 0, kRowPos, &st);
+        bad |= attend_row(a, it.b, it.row + r, h, it.sees(r, a.causal), 0, kRowPos, &st);
         if (beat && lane == 0) ++*beat;
         const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
         if (lane * S::V < a.head_dim)

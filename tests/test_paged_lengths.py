@@ -63,3 +63,81 @@ def test_an_idle_slot_is_no_error(ctx, dtype):
     for b in (bq, bk, bv, bqt, bo):
         b.free()
     p.free()
+
+
+# ---- lengths beyond the table ----------------------------------------------------------------------------
+BEYOND = [
+    # dtype, n_q, n_kv, d, page, pages of a sequence, lengths, new rows
+    ("bf16", 4, 2, 64, 16, 6, [100, 96, 130, 97, 1000], [30, 96, 20, 5, 3]),
+    ("bf16", 8, 1, 128, 32, 5, [170, 2000, 161], [150, 40, 170]),
+    ("bf16", 4, 1, 128, 256, 8, [2051, 2100], [4, 60]),            # keys in parts
+    ("bf16", 2, 1, 256, 16, 6, [100, 130], [30, 20]),
+    ("f32", 4, 2, 64, 16, 6, [100, 96, 130, 97], [30, 96, 20, 5]),
+    ("f32", 4, 1, 128, 256, 8, [2051, 2100], [4, 60]),
+    ("f32", 2, 1, 256, 16, 6, [100, 130], [30, 20]),               # row by row
+    ("bf16", 2, 2, 64, 16, 2, [40 + i % 3 for i in range(150)], [10] * 150),
+    ("bf16", 1, 1, 64, 16, 2, [(1 << 31) - 1, 33], [50, 2]),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,n_q,n_kv,d,page,width,lens,new", BEYOND)
+def test_rows_keep_their_places_where_lengths_go_beyond_the_table(ctx, dtype, n_q, n_kv, d, page, width, lens, new):
+    """Row t stands at lens - (cu[b + 1] - t) in every call: rows whose position has a page are written there and see what is before them, the
+    others are not written and see all that there is."""
+    room = width * page
+    p = Pool(ctx, [min(n, room) for n in lens], n_kv, d, page, dtype, seed=d, width=width)
+    p.bl.upload(np.array(lens, np.int32))
+    rows, cu = sum(new), np.cumsum([0] + new).astype(np.int32)
+    up = ctx.array_to_buffer
+    q = pm.decode(pm.encode(normal(4, rows, n_q, d), dtype), dtype)
+    bq, bo, bcu = up(pm.encode(q, dtype)), ctx.make_buffer(rows * n_q * d, NP[dtype]), up(cu)
+    ctx.paged_prompt_attention(bq, p.bk, p.bv, bo, p.bt, bcu, p.bl, rows, len(lens), n_q, n_q // n_kv, n_kv, d, page, p.n_pages, width, d ** -0.5, True,
+                               DT[dtype])
+    ctx.sync()
+    got = pm.decode(bo.download(), dtype).reshape(rows, n_q, d)
+    for b in range(len(lens)) if len(lens) < 20 else (0, 1, 77, 149):
+        for r in sorted({0, new[b] // 2, new[b] - 1, min(max(room - lens[b] + new[b] - 1, 0), new[b] - 1)}):
+            m = min(max(lens[b] - new[b] + r + 1, 0), room)
+            want, tol = pm.attention(q[cu[b] + r][None], p.keys[b][:m], p.values[b][:m], d ** -0.5, False, dtype)
+            close(got[cu[b] + r][None], want, tol, f"sequence {b} row {r} of {m} keys")
+    # the same rows written
+    k, v = normal(5, rows, n_kv, d), normal(6, rows, n_kv, d)
+    x, bk, bv = up(normal(7, rows, n_q, d)), up(k), up(v)
+    before = p.bv.download().reshape(-1, n_kv * d)
+    ctx.paged_rope_append(x, bk, bv, bo, p.bk, p.bv, p.bt, p.bl, bcu, rows, len(lens), n_q, n_kv, d, page, p.n_pages, width, 1e4, L.F32, DT[dtype])
+    if any(n > room for n in lens):
+        with pytest.raises(L.RstqError) as e:
+            ctx.sync()
+        assert e.value.code == L.E_RANGE
+    ctx.sync()
+    want = before.copy()
+    for b, n in enumerate(lens):
+        for r in range(new[b]):
+            pos = n - new[b] + r
+            if 0 <= pos < room:
+                want[p.table[b, pos // page] * page + pos % page] = pm.encode(v[cu[b] + r].reshape(-1), dtype)
+    after = p.bv.download().reshape(-1, n_kv * d)
+    assert np.array_equal(after.view(np.uint8), want.view(np.uint8))
+    for b in (bq, bo, bcu, x, bk, bv):
+        b.free()
+    p.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_decode_of_lengths_beyond_the_table_sees_all_of_it(ctx, dtype):
+    n_q, n_kv, d, page, width, lens = 4, 2, 64, 16, 3, [49, (1 << 31) - 1, 48, 5]
+    p = Pool(ctx, [min(n, 48) for n in lens], n_kv, d, page, dtype, width=width)
+    p.bl.upload(np.array(lens, np.int32))
+    q = pm.decode(pm.encode(normal(3, 4, n_q, d), dtype), dtype)
+    bq, bo = ctx.array_to_buffer(pm.encode(q, dtype)), ctx.make_buffer(4 * n_q * d, NP[dtype])
+    ctx.paged_decode_attention(bq, p.bk, p.bv, bo, p.bt, p.bl, 4, n_q, 2, n_kv, d, page, p.n_pages, width, 0.125, DT[dtype])
+    ctx.sync()
+    got = pm.decode(bo.download(), dtype).reshape(4, n_q, d)
+    for b in range(4):
+        want, tol = pm.attention(q[b:b + 1], p.keys[b], p.values[b], 0.125, False, dtype)
+        close(got[b:b + 1], want, tol, f"sequence {b}")
+    bq.free()
+    bo.free()
+    p.free()
