@@ -176,10 +176,10 @@ struct RowState {
     float o[C][V], m, l;
 };
 // Row `row` of head h, which sees `len` positions of sequence b, against positions first .. first + kRowPos - 1, and so on every `step`.
-// True: a position had no page.
+// True: a position had no page.  beat: a word that changes every few thousand positions, for those who wait.
 template <typename T>
 __device__ __forceinline__ bool attend_row(const PromptArgs& p, int b, int64_t row, int h, int64_t len, int64_t first, int64_t step,
-                                           RowState<T>* st) {
+                                           RowState<T>* st, int* beat = nullptr) {
     constexpr int V = RowState<T>::V, C = RowState<T>::C;
     const int lane = threadIdx.x & 31, hd = p.head_dim, hkv = h / p.group;
     int64_t row0;
@@ -197,6 +197,7 @@ __device__ __forceinline__ bool attend_row(const PromptArgs& p, int b, int64_t r
     bool bad = false;
     const float scale2 = p.scale * 1.4426950408889634f;
     for (int64_t j0 = first; j0 < len; j0 += step) {
+        if (beat && (j0 & 16383) < step && lane == 0) atomicAdd(beat, 1);
         float s[kRowPos];
         int64_t at[kRowPos];
 #pragma unroll

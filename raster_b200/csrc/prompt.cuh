@@ -387,14 +387,13 @@ static __device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, in
 
 // The block's rows one by one, from the positions they see alone.
 template <typename T>
-__device__ __forceinline__ void prompt_rows(const PromptArgs& a, const PromptItem& it, int h, int warp, int warps, volatile int* beat = nullptr) {     // (of one head)
+__device__ __forceinline__ void prompt_rows(const PromptArgs& a, const PromptItem& it, int h, int warp, int warps, int* beat = nullptr) {     // (of one head)
     const int lane = threadIdx.x & 31;
     using S = RowState<T>;      // (f32: head_dim <= 128; one piece of a lane)
     bool bad = false;
     for (int r = warp; r < it.rows; r += warps) {
         S st;
-        bad |= attend_row(a, it.b, it.row + r, h, it.sees(r, a.causal), 0, kRowPos, &st);
-        if (beat && lane == 0) ++*beat;
+        bad |= attend_row(a, it.b, it.row + r, h, it.sees(r, a.causal), 0, kRowPos, &st, beat);
         const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
         if (lane * S::V < a.head_dim)
 #pragma unroll

@@ -337,7 +337,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             }
             tc_fence_before();       // O has been read before the next rows' P is handed on
             if (again && whole)
-                for (int i = 0; i < p.pack; ++i) prompt_rows<__nv_bfloat16>(p.a, it, x.h * p.pack + i, warp, 8, abort_flag + 1);
+                for (int i = 0; i < p.pack; ++i) prompt_rows<__nv_bfloat16>(p.a, it, x.h * p.pack + i, warp, 8, s_abort + 1);
             done_work(w);
         }
     } else {

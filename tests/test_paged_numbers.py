@@ -220,3 +220,34 @@ def test_prompts_over_a_million_positions(ctx, n_q, d, rows):
     for b in (bq, bo, cu):
         b.free()
     x.free()
+
+
+@pytest.mark.gpu
+def test_one_row_of_many_keys_taken_by_itself(ctx):
+    """An infinity above the diagonal of one of many sequences of 2^23 keys: its rows by themselves take longer than any wait in the kernel
+    may, one row alone does, and the block has its next rows in hand meanwhile."""
+    n, page, d, seqs, rows, distinct = 1 << 23, 256, 64, 300, 2, 64
+    width = n // page
+    k = pm.decode(pm.encode(normal(1, (distinct + 1) * page, 1, d), "bf16"), "bf16")
+    v = pm.decode(pm.encode(np.random.default_rng(2).random(((distinct + 1) * page, 1, d)).astype(np.float32) + 0.5, "bf16"), "bf16")
+    v[-1, 0, 5] = np.inf                                      # the last position of the last page, which ends one sequence
+    table = np.tile(np.arange(width, dtype=np.int32) % distinct, (seqs, 1))
+    table[-1, -1] = distinct                                  # (the last sequence's rows come first)
+    up = ctx.array_to_buffer
+    q = pm.decode(pm.encode(normal(3, seqs * rows, 1, d), "bf16"), "bf16")
+    bq, bk, bv, bt = up(pm.encode(q, "bf16")), up(pm.encode(k, "bf16")), up(pm.encode(v, "bf16")), up(table)
+    bl, cu, bo = up(np.full(seqs, n, np.int32)), up(np.arange(seqs + 1, dtype=np.int32) * rows), ctx.make_buffer(seqs * rows * d, np.uint16)
+    ctx.paged_prompt_attention(bq, bk, bv, bo, bt, cu, bl, seqs * rows, seqs, 1, 1, 1, d, page, distinct + 1, width, d ** -0.5, True, L.BF16)
+    ctx.sync()
+    got = pm.decode(bo.download(), "bf16").reshape(seqs * rows, d)
+    assert np.isposinf(got[-1, 5]) and np.isfinite(np.delete(got[-1], 5)).all() and np.isfinite(got[:-1]).all()
+    for r in (0, seqs, 2 * seqs - 2):                         # first rows of theirs, which do not see the last key
+        b = r // rows
+        times = np.bincount(table[b], minlength=distinct + 1).repeat(page)
+        times[table[b, -1] * page + page - 1] -= 1
+        s = k[:, 0].astype(np.float64) @ q[r, 0].astype(np.float64) * d ** -0.5
+        w = np.exp(s - s.max()) * times
+        want = (w / w.sum()) @ np.where(np.isinf(v[:, 0]), 0, v[:, 0]).astype(np.float64)
+        assert (np.abs(got[r] - want) <= (pm.HALF["bf16"] + 2.0 ** -11) * want).all(), (r, np.abs(got[r] / want - 1).max())
+    for b in (bq, bk, bv, bt, bl, cu, bo):
+        b.free()
