@@ -251,3 +251,95 @@ def test_one_row_of_many_keys_taken_by_itself(ctx):
         assert (np.abs(got[r] - want) <= (pm.HALF["bf16"] + 2.0 ** -11) * want).all(), (r, np.abs(got[r] / want - 1).max())
     for b in (bq, bk, bv, bt, bl, cu, bo):
         b.free()
+
+
+# ---- the second term of a decode weight --------------------------------------------------------------------
+def cancelling(seed, n, heads, d, scale):
+    """q [heads, d], k and v [n, heads, d], all bf16, whose weighted values cancel but for the last value's rounding: what the weights are
+    rounded by stands alone in the result."""
+    q, k, v = (pm.decode(pm.encode(normal(seed + i, *shape), "bf16"), "bf16") for i, shape in enumerate(((heads, d), (n, heads, d), (n, heads, d))))
+    for h in range(heads):
+        w = np.exp(k[:, h].astype(np.float64) @ q[h].astype(np.float64) * scale)
+        v[n - 1, h] = pm.decode(pm.encode((-(w[:-1] @ v[:-1, h]) / w[-1]).astype(np.float32), "bf16"), "bf16")
+    return q, k, v
+
+
+def test_the_tolerance_tells_a_weight_of_one_term():
+    """A weight rounded or cut to bf16 misses what two terms hold (planted in a model here)."""
+    d, heads = 64, 4
+    q, k, v = cancelling(5, 64, heads, d, d ** -0.5)
+    want, tol = pm.attention(q[None], k, v, d ** -0.5, False, "bf16", p_terms=2)
+    up = lambda x: pm.from_bf16(pm.to_bf16(x))  # noqa: E731
+    cut = lambda x: (x.view(np.uint32) & 0xFFFF0000).view(np.float32)  # noqa: E731
+    for form, holds in ((lambda w: cut(w).astype(np.float64) + up(w - cut(w)), True), (up, False), (cut, False)):
+        got = np.zeros((heads, d))
+        for h in range(heads):
+            s = k[:, h].astype(np.float64) @ q[h].astype(np.float64) * d ** -0.5
+            w = np.exp(s - s.max()).astype(np.float32)
+            got[h] = up((form(w) @ v[:, h].astype(np.float64) / w.astype(np.float64).sum()).astype(np.float32))
+        over = np.abs(got - want[0]) / tol[0]
+        assert (over.max() <= 1) == holds and (holds or over.max() > 3), over.max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,n_kv,d,lens", [(1, 4, 64, [64, 40, 17]), (4, 2, 128, [64, 100]), (8, 1, 64, [33, 64]), (16, 1, 128, [64]), (12, 2, 256, [64, 50])])
+def test_decode_weights_have_two_terms(ctx, group, n_kv, d, lens):
+    p = Pool(ctx, lens, n_kv, d, 16, "bf16")
+    k, v, q = p.k.copy(), p.v.copy(), np.zeros((len(lens), n_kv * group, d), np.float32)
+    some = []
+    for b, n in enumerate(lens):
+        qq, kk, vv = cancelling(10 * b + d, n, n_kv, d, d ** -0.5)
+        q[b] = np.repeat(qq, group, 0)
+        some.append((kk, vv))
+        for pos in range(n):
+            k[at(p, b, pos)], v[at(p, b, pos)] = kk[pos], vv[pos]
+    p.bk.upload(pm.encode(k, "bf16"))
+    p.bv.upload(pm.encode(v, "bf16"))
+    bq, bo = ctx.array_to_buffer(pm.encode(q, "bf16")), ctx.make_buffer(q.size, np.uint16)
+    ctx.paged_decode_attention(bq, p.bk, p.bv, bo, p.bt, p.bl, len(lens), n_kv * group, group, n_kv, d, 16, p.n_pages, p.width, d ** -0.5, L.BF16)
+    ctx.sync()
+    got = pm.decode(bo.download(), "bf16").reshape(q.shape)
+    for b in range(len(lens)):
+        want, tol = pm.attention(q[b:b + 1], *some[b], d ** -0.5, False, "bf16", p_terms=2)
+        close(got[b:b + 1], want, tol, f"sequence {b}")
+    bq.free()
+    bo.free()
+    p.free()
+
+
+# ---- scales that are not positive --------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("scale", [0.0, -0.125, -1.0, 1e-30])
+@pytest.mark.parametrize("n_q,n_kv,d,page,lens,new", [(4, 2, 64, 16, [70, 0, 33], [70, 0, 5]), (8, 1, 128, 32, [1500, 40], [3, 40]), (2, 1, 256, 16, [50, 20], [50, 2])])
+def test_scales_that_are_not_positive(ctx, dtype, scale, n_q, n_kv, d, page, lens, new):
+    """The largest score is then the smallest product, or all of them are the same."""
+    x = Prompts(ctx, dtype, n_q, n_kv, d, page, lens, new, seed=d)
+    x.scale = scale
+    x.call()
+    ctx.sync()
+    x.check()
+    p, B = x.pool, len(lens)
+    q = pm.decode(pm.encode(normal(9, B, n_q, d), dtype), dtype)
+    bq, bo = ctx.array_to_buffer(pm.encode(q, dtype)), ctx.make_buffer(B * n_q * d, NP[dtype])
+    ctx.paged_decode_attention(bq, p.bk, p.bv, bo, p.bt, p.bl, B, n_q, n_q // n_kv, n_kv, d, page, p.n_pages, p.width, scale, DT[dtype])
+    ctx.sync()
+    got = pm.decode(bo.download(), dtype).reshape(B, n_q, d)
+    for b in range(B):
+        want, tol = pm.attention(q[b:b + 1], p.keys[b], p.values[b], scale, False, dtype)
+        close(got[b:b + 1], want, tol, f"sequence {b}")
+    # packed, without causality
+    keys, values = np.concatenate(p.keys), np.concatenate(p.values)
+    up = ctx.array_to_buffer
+    bk, bv, bku = up(pm.encode(keys, dtype)), up(pm.encode(values, dtype)), up(np.cumsum([0] + lens).astype(np.int32))
+    ctx.prompt_attention(x.bq, bk, bv, x.bo, x.bcu, bku, x.rows, len(keys), B, n_q, n_q // n_kv, n_kv, d, scale, False, DT[dtype])
+    ctx.sync()
+    got = pm.decode(x.raw(), dtype).reshape(x.rows, n_q, d)
+    for b in range(B):
+        if new[b]:
+            r = x.cu[b + 1] - 1
+            want, tol = pm.attention(x.q[r][None], p.keys[b], p.values[b], scale, False, dtype)
+            close(got[r][None], want, tol, f"sequence {b}, packed")
+    for b in (bq, bo, bk, bv, bku):
+        b.free()
+    x.free()
