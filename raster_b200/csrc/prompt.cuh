@@ -30,7 +30,7 @@ inline bool prompt_may_part(const PromptArgs& a, int most) {
 // Heads of a group that share a query tile of 128 rows, (row of q, head) with the head innermost: all of them where they fill seven eighths of it.
 inline int prompt_pack(int group) { return 128 / group * group >= 112 ? group : 1; }
 
-constexpr float kGrow = 8.f;         // log2 of how far a row's largest weight may go beyond 1
+constexpr float kGrow = 8.f;         // bf16: log2 of how far a row's scores may go beyond the running maximum before it moves
 
 // 32 columns of this thread's row, there when the instruction is over: what follows cannot be moved before the wait.
 __device__ __forceinline__ void tmem_ld32_wait(uint32_t taddr, uint32_t* r) {

@@ -11,8 +11,9 @@
 //   O += P V    (tcgen05, P from tensor memory, V from shared memory as it lies: an operand with head_dim innermost)
 //
 // While one tile's warpgroup is at its exponentials the tensor core works for the other tile.  The running maximum of a row moves
-// only when it grows by more than 2^8: until then P is up to 256 and O need not be rescaled (sums are f32; P's relative rounding
-// does not depend on its size), so O is read and written back for a few tiles at the start of a row and hardly ever after.
+// only when it grows by more than 2^8 (a published refinement of the softmax taken in one pass), so O is read and written back for a few tiles at
+// the start of a row and hardly ever after.  Weights are taken relative to 2^8 times it: none is more than 1.  (Sums are f32 and P's relative
+// rounding does not depend on its size; the 2^8 leaves with the sum of the weights.)
 // P is rounded to bf16, the type of V (2^-9 rms of each weight, no more than the result's own rounding); its sum is taken before that.
 // P is handed to the tensor core in halves, as soon as each is written.
 //
@@ -253,7 +254,9 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                         if (taken) ref = m == -INFINITY ? m : m2;
                     }
                 }
-                const uint64_t scale = pack2(p.scale2, p.scale2), minus = pack2(-m2, -m2);
+                // (2^-8 in every weight, so that none is more than 1 and a large value stays one)
+                const float below = -m2 - kGrow;
+                const uint64_t scale = pack2(p.scale2, p.scale2), minus = pack2(below, below);
                 uint64_t part[2] = {0ull, 0ull};
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {

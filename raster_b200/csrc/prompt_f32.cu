@@ -192,7 +192,7 @@ prompt_f32_kernel(const PromptParamsF p) {
             float rowmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             rowmax = fmaxf(rowmax, other(rowmax));
             if (!ok) break;
-            const bool grown = rowmax > m && !(rowmax * p.scale2 <= m2 + kGrow && m != -INFINITY);
+            const bool grown = rowmax > m;
             const bool any = __any_sync(0xffffffffu, grown);
             float f = 1.f;
             if (grown) {

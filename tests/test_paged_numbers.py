@@ -343,3 +343,64 @@ def test_scales_that_are_not_positive(ctx, dtype, scale, n_q, n_kv, d, page, len
     for b in (bq, bo, bk, bv, bku):
         b.free()
     x.free()
+
+
+# ---- values near the type's largest -------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d,lens,new", [(64, [400, 90], [40, 90]), (128, [2600], [3]), (128, [300], [300]), (256, [200], [30])])
+def test_values_near_the_largest_there_are(ctx, dtype, d, lens, new):
+    """A weight is never more than 1, so a value of 3e38 stays one where its score goes beyond the earlier ones by a few."""
+    n_q, page = 2, 16
+    x = Prompts(ctx, dtype, n_q, 1, d, page, lens, new, seed=d)
+    p = x.pool
+    k, v = p.k.copy(), p.v.copy()
+    x.q = np.broadcast_to(pm.decode(pm.encode(np.abs(normal(1, 1, 1, d)) + 0.5, dtype), dtype), x.q.shape).copy()      # (a row's scores are a key's, whatever the row)
+    x.bq.upload(pm.encode(x.q, dtype))
+    for b, n in enumerate(lens):
+        for i, (pos, score) in enumerate(((n // 2, 4.0), (n - new[b] // 2 - 1, 5.0))):
+            key = score * d ** 0.5 * x.q[0, 0] / (x.q[0, 0] ** 2).sum() + 0.5 * p.keys[b][pos]
+            k[at(p, b, pos)] = p.keys[b][pos] = pm.decode(pm.encode(key.astype(np.float32), dtype), dtype)
+            v[at(p, b, pos)][0, ::2] = p.values[b][pos][0, ::2] = pm.decode(pm.encode(np.array(-3e38 if i else 3e38), dtype), dtype)
+    p.bk.upload(pm.encode(k, dtype))
+    p.bv.upload(pm.encode(v, dtype))
+    x.call()
+    ctx.sync()
+    x.check()
+    q = pm.encode(x.q[:len(lens)], dtype)
+    bq, bo = ctx.array_to_buffer(q), ctx.make_buffer(q.size, NP[dtype])
+    ctx.paged_decode_attention(bq, p.bk, p.bv, bo, p.bt, p.bl, len(lens), n_q, n_q, 1, d, page, p.n_pages, p.width, d ** -0.5, DT[dtype])
+    ctx.sync()
+    got = pm.decode(bo.download(), dtype).reshape(len(lens), n_q, d)
+    for b in range(len(lens)):
+        want, tol = pm.attention(x.q[b:b + 1], p.keys[b], p.values[b], d ** -0.5, False, dtype)
+        close(got[b:b + 1], want, tol, f"decode {b}")
+    bq.free()
+    bo.free()
+    x.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,n_q,d", [("f32", 2, 128), ("f32", 7, 128), ("bf16", 7, 128), ("f32", 4, 96), ("bf16", 4, 256)])
+def test_rows_taken_by_themselves(ctx, dtype, n_q, d):
+    """Infinities above the diagonal of blocks that share a tile with other heads, or have registers moved between their warps."""
+    x = Prompts(ctx, dtype, n_q, 1, d, 16, [300, 150], [300, 150], seed=d)
+    p = x.pool
+    k, v = p.k.copy(), p.v.copy()
+    v[at(p, 0, 200)][0, 7] = np.inf
+    k[at(p, 1, 100)][0, 3] = np.nan
+    p.bk.upload(pm.encode(k, dtype))
+    p.bv.upload(pm.encode(v, dtype))
+    x.call()
+    ctx.sync()
+    got = pm.decode(x.raw(), dtype).reshape(x.rows, n_q, d)
+    assert np.isposinf(got[200:300, :, 7]).all() and np.isnan(got[400:]).all()
+    for b, rows in ((0, (0, 127, 128, 199)), (1, (0, 64, 99))):
+        for r in rows:
+            i = x.cu[b] + r
+            close(got[i][None], *pm.attention(x.q[i][None], p.keys[b][:r + 1], p.values[b][:r + 1], x.scale, False, dtype), f"sequence {b} row {r}")
+    for r in (200, 299):
+        keep = [i for i in range(d) if i != 7]
+        want, tol = pm.attention(x.q[r][None], p.keys[0][:r + 1], p.values[0][:r + 1], x.scale, False, dtype)
+        close(got[r][None][..., keep], want[..., keep], tol[..., keep], f"row {r}")
+    x.free()
