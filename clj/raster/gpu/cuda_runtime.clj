@@ -116,7 +116,7 @@
 (defrstq residual-rms-norm-quant-act* "rstq_residual_rms_norm_quant_act" I [P P P P P P P P L L D D])
 (defrstq silu-mul-quant-act* "rstq_silu_mul_quant_act"  I [P P P P P P L])
 (defrstq gelu-mul-quant-act* "rstq_gelu_mul_quant_act"  I [P P P P P P L])
-;; ---- sharded weights
+;; ---- many sequences from one paged cache
 (defrstq paged-rope-append*  "rstq_paged_rope_append" I [P P P P P P P P P P L L L L L L L L L L D I I])
                              ; ctx q k v qout kcache vcache table lens cu rows seqs n-q n-kv head-dim page n-pages max-pages ldq ldkv theta in-dtype dtype
 (defrstq paged-decode-attention* "rstq_paged_decode_attention" I [P P P P P P P L L L L L L L L L D I])
@@ -132,7 +132,7 @@
 (defrstq pages-compact*      "rstq_pages_compact"     I [P P P P P P P P P L L L L L L])
                              ; ctx kcache vcache table lens refs table-out refs-out info seqs n-pages max-pages page layers row-bytes
 (defrstq pages-copy*         "rstq_pages_copy"        I [P P P P P P L L L L])        ; ctx kcache vcache src dst info n n-pages layers page-bytes
-
+;; ---- sharded weights
 (defrstq tp-region-bytes*    "rstq_tp_region_bytes"   L [I L])
 (defrstq tp-attach*          "rstq_tp_attach"         I [P P P I I I L])           ; ctx regions tp** dev rank nranks region-bytes
 (defrstq tp-create-local*    "rstq_tp_create_local"   I [P P P I L])               ; ctx devs tps nranks max-payload

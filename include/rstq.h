@@ -444,6 +444,9 @@ RSTQ_API int32_t rstq_gqa_decode_attention(rstq_ctx* ctx, rstq_buf* q, rstq_buf*
  *
  * Elements are RSTQ_F32 or RSTQ_BF16 (`dtype`), one type for q, K, V and out; sums, softmax statistics and angles are held in
  * 32 bits or more and a result is rounded once.  head_dim % 8 == 0 and <= 256; n_q = group * n_kv.
+ * Weights (the exponentials) meet V as they are in f32; in bf16 as two bf16 terms (16 bits) in decode attention, and rounded to
+ * bf16 in prompt attention (their sum before that), which makes its error against 64 bits 2.0 - 2.2e-3 of a result (root mean
+ * square) where the result's own rounding leaves 1.6e-3.  A caller who needs more takes f32.
  *
  * Pool: kcache and vcache hold n_pages pages of `page` positions (16, 32, 64, 128 or 256), a position n_kv heads of
  *   head_dim: rows as in the contiguous caches [position][n_kv][head_dim], of which a pool with a table that counts up is
@@ -464,9 +467,9 @@ RSTQ_API int32_t rstq_gqa_decode_attention(rstq_ctx* ctx, rstq_buf* q, rstq_buf*
  *
  *   rstq_paged_rope_append       q turned to qout [rows][n_q][head_dim]; k turned and v written to their pages, in `dtype`
  *                                (q, k, v are in_dtype).  cu may be NULL: rows == seqs, one per sequence, for its
- *                                last position; a sequence of length 0 that holds no page (its first entry is -1, as in a new cache and behind
- *                                rstq_pages_free) is idle then, and its row left out without an error.  qout may be q
- *                                where q is packed and of the type stored.
+ *                                last position; a sequence of length 0 that holds no page (its first entry is -1, as
+ *                                in a new cache and behind rstq_pages_free) is idle then, and its row left out
+ *                                without an error.  qout may be q where q is packed and of the type stored.
  *   rstq_paged_decode_attention  one row of q per sequence against all its positions; a sequence of none gives zeros.
  *   rstq_prompt_attention        rows of packed sequences (cu_q) against packed keys and values [kv_rows][n_kv][head_dim]
  *                                (cu_k; may be cu_q); causal = 1: a row sees the keys up to its own place, the last row
@@ -495,7 +498,8 @@ RSTQ_API int32_t rstq_paged_prompt_attention(rstq_ctx* ctx, rstq_buf* q, rstq_bu
  * sequences hold a page, 0 = free; a new cache has lens and refs of zeros and a table of -1.  A sequence of n positions holds
  * ceil(n / page) pages.  Free pages are taken lowest first, in the list's order.  kcache and vcache: [layers] pools one behind
  * the other, rows of row_bytes bytes (n_kv * head_dim elements; a page's bytes are a multiple of 16).  Lists: int32 [n], n <= 65536.
- * info int32 [4], written by every call: [0] = 0 done, else nothing was changed: 1 = too few free pages ([3] = pages wanted, 2^31 - 1 at most),
+ * info int32 [4], written by every call: [0] = 0 done, else nothing was changed: 1 = too few free pages ([3] = pages wanted,
+ * 2^31 - 1 at most),
  * 2 = an entry of the list is no sequence (page), is there twice, or may not be there, 3 = no room in the table, 4 = the positions would
  * go to a page that another sequence holds too (2 to 4: [3] = the first such place; of entries that are there twice, the later one's);
  * [1] = pages in use; [2] = pages copied.

@@ -28,11 +28,12 @@
 // into parts along the keys (prompt_share); a part leaves its sums, maximum and weight in a slot, and a second launch joins them in order, so
 // that results do not depend on who was first.
 //
-// What it takes.  A step (256 rows, 128 keys, head_dim 128) takes 1.9 us, of which the MMAs are 1.05 and the exponentials, on the
-// SM's 16 special-function lanes, as much: the chain S, maximum, exponentials, P V, next S of each tile does not close any tighter in 512
-// columns of tensor memory, two places for S per tile would need 768.  8192 rows, 32 heads over 8: 436 us, 1260 TFLOP/s (510 in a row, at
-// the power limit: 1080); 4096 rows 122 us; 8192 of 64 columns 380 us.  Beside the steps a block of rows costs 2.6 us, mostly its stores,
-// and a launch 5 to 7 us until the first S.  512 rows behind 16000 keys 158 us (in parts; 255 with one query tile per block), 2 rows 32 us.
+// What it takes.  A step (256 rows, 128 keys, head_dim 128) takes 1.9 us, of which the MMAs are 1.05 at the tensor core's own pace (1.5 at the rate
+// that a large matrix product reaches on the device) and the exponentials, on the SM's 16 special-function lanes, as much: the chain S, maximum,
+// exponentials, P V, next S of each tile does not close any tighter in 512 columns of tensor memory, two places for S per tile would need 768
+// (of 64 columns 640; there a third one for both tiles would fit).  8192 rows, 32 heads over 8: 442 us, 1245 TFLOP/s (515 in a row, at the power
+// limit: 1070); 4096 rows 127 us; 8192 of 64 columns 400 us.  Beside the steps a block of rows costs 2.6 us, mostly its stores, and a launch 5 to
+// 7 us until the first S.  512 rows behind 16000 keys 162 us (in parts; 255 with one query tile per block), 2 rows 33 us.
 // A polynomial in place of a part of the exponentials was slower, so were 64 keys per tile with two places for S.
 #include <algorithm>
 #include <type_traits>

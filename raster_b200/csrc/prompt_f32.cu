@@ -8,7 +8,7 @@
 // long: the first product has one of its own and the five small ones another, in tensor memory, and P V of every tile of keys is taken out and
 // added, to nearest, to sums in registers.  (Left in tensor memory over all keys a result lost 6e-9 of itself with every key: 1.2e-5 of it after
 // 4000, 7.7e-5 after 16000, 3.7e-4 after 64000; as it is 2e-7, 3e-7, 6e-7.  It costs nothing: O is not rescaled in tensor memory any more; 1024
-// rows of 16 heads x 64 38 us before and after, x 128 59 and 56.)  f32 FMAs would be bound by 72 TFLOP/s of the whole device, the six MMAs by a
+// rows of 16 heads x 64 38 and 39 us, x 128 59 and 57.)  f32 FMAs would be bound by 72 TFLOP/s of the whole device, the six MMAs by a
 // sixth of bf16's rate.
 //
 // A block has a tile of 128 (row, head) pairs of one sequence: rows of a head, or rows of all heads of a group as in prompt_attn.cu.  Four warps
@@ -18,8 +18,8 @@
 // one's exponentials are.  (Of 64 columns two blocks with one place each would fit an SM: two sequences of 1000 rows 63 us, against 46.)  A step of
 // 64 keys takes 1.7 us with 64 columns, 3.0 with 128, of which the MMAs are 1 and 2 (an MMA of S is bound by reading Q and K from shared memory, 48
 // cycles): the rest is the way of K and V through registers and their split, one tile at a time, which a second tile ahead only lengthens (spills).
-// 1024 rows of 16 heads: 38 and 56 us.
-// Few blocks that see many keys are cut into parts as in prompt_attn.cu: 2 rows behind 4000 keys of 8 heads of 128 212 -> 45 us, 300 of 64 columns
+// 1024 rows of 16 heads: 39 and 57 us.
+// Few blocks that see many keys are cut into parts as in prompt_attn.cu: 2 rows behind 4000 keys of 8 heads of 128 212 -> 39 us, 300 of 64 columns
 // 129 -> 50.
 //
 // An infinity or NaN has no such terms: a block that meets one (in keys or values its rows may not even see) computes its rows one by one
