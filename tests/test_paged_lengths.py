@@ -141,3 +141,76 @@ def test_decode_of_lengths_beyond_the_table_sees_all_of_it(ctx, dtype):
     bq.free()
     bo.free()
     p.free()
+
+
+# ---- arrays that begin on 16 bytes and on no more ---------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,n_q,n_kv,d", [("bf16", 4, 2, 64), ("bf16", 7, 1, 8), ("bf16", 2, 2, 136), ("bf16", 3, 1, 128), ("f32", 4, 2, 64), ("f32", 3, 1, 40),
+                                              ("f32", 2, 1, 256)])
+def test_arrays_on_16_bytes(ctx, dtype, n_q, n_kv, d):
+    """Every array 16 bytes behind a boundary of 256, rows a multiple of 16 bytes long and of nothing more."""
+    page, lens, new = 16, [40, 150, 3], [40, 20, 1]
+    p = Pool(ctx, lens, n_kv, d, page, dtype, seed=d)
+    B, rows, cu = 3, sum(new), np.cumsum([0] + new).astype(np.int32)
+    made = []
+
+    def up(a):
+        a = np.ascontiguousarray(a)
+        base = ctx.make_buffer(a.nbytes + 272, np.uint8)
+        base.fill_bytes(0xFF)
+        b = ctx.wrap_buffer(base.device_ptr + 16, a.size, a.dtype.type)
+        b.upload(a.reshape(-1))
+        made.extend((b, base))
+        return b
+
+    item = NP[dtype]().itemsize
+    step = n_q * d + 16 // item * (1 if (n_q * d * item // 16) % 2 == 0 else 2)        # an odd number of 16 bytes
+    full = pm.encode(normal(4, rows, step), dtype)
+    q = pm.decode(full, dtype)[:, :n_q * d].reshape(rows, n_q, d)
+    bk, bv, bt, bl, bcu, bq = up(pm.encode(p.k, dtype)), up(pm.encode(p.v, dtype)), up(p.table), up(np.array(lens, np.int32)), up(cu), up(full)
+    bo = up(np.full(rows * n_q * d, 7, NP[dtype]))
+    heads, scale = (n_q, n_q // n_kv, n_kv, d, page, p.n_pages, p.width), d ** -0.5
+    ctx.paged_prompt_attention(bq, bk, bv, bo, bt, bcu, bl, rows, B, *heads, scale, True, DT[dtype], ldq=step)
+    ctx.sync()
+    got = pm.decode(bo.download(), dtype).reshape(rows, n_q, d)
+    for b in range(B):
+        s = slice(cu[b], cu[b + 1])
+        close(got[s], *pm.attention(q[s], p.keys[b], p.values[b], scale, True, dtype), f"prompt {b}")
+    keys, values, ku = np.concatenate(p.keys), np.concatenate(p.values), np.cumsum([0] + lens).astype(np.int32)
+    kstep = n_kv * d + 16 // item * (1 if (n_kv * d * item // 16) % 2 == 0 else 2)
+    pad = lambda x: np.concatenate([pm.encode(x.reshape(len(x), -1), dtype), np.full((len(x), kstep - n_kv * d), 9, NP[dtype])], 1)  # noqa: E731
+    ctx.prompt_attention(bq, up(pad(keys)), up(pad(values)), bo, bcu, up(ku), rows, len(keys), B, n_q, n_q // n_kv, n_kv, d, scale, True, DT[dtype], ldq=step,
+                         ldk=kstep)
+    ctx.sync()
+    assert np.abs(pm.decode(bo.download(), dtype).reshape(rows, n_q, d) - got).max() <= 4 * pm.HALF[dtype] * np.abs(got).max()
+    ctx.paged_decode_attention(bq, bk, bv, bo, bt, bl, B, *heads, scale, DT[dtype], ldq=step)
+    ctx.sync()
+    got = pm.decode(bo.download(n=B * n_q * d), dtype).reshape(B, n_q, d)
+    for b in range(B):
+        close(got[b:b + 1], *pm.attention(q[b:b + 1], p.keys[b], p.values[b], scale, False, dtype), f"decode {b}")
+    x, k, v = normal(7, rows, n_q, d), normal(8, rows, n_kv, d), normal(9, rows, n_kv, d)
+    ctx.paged_rope_append(up(x), up(k), up(v), bo, bk, bv, bt, bl, bcu, rows, B, n_q, n_kv, d, page, p.n_pages, p.width, 1e4, L.F32, DT[dtype])
+    ctx.sync()
+    got, pool = pm.decode(bo.download(), dtype).reshape(rows, n_q, d), bv.download().reshape(p.v.shape)
+    for b in range(B):
+        for t in range(cu[b], cu[b + 1]):
+            pos = lens[b] - (cu[b + 1] - t)
+            want = pm.rope(x[t], pos, 1e4)
+            assert np.abs(got[t] - want).max() <= (pm.HALF[dtype] + 2.0 ** -20) * np.abs(want).max()
+            assert np.array_equal(pool[p.table[b, pos // page], pos % page], pm.encode(v[t], dtype))
+    refs, info, gone = np.zeros(p.n_pages, np.int32), up(np.zeros(4, np.int32)), up(np.array([1], np.int32))
+    for b, n in enumerate(lens):
+        refs[p.table[b, :-(-n // page)]] = 1
+    br = up(refs)
+    before = bk.download().reshape(p.k.shape)
+    ctx.pages_free(bt, bl, br, gone, info, 1, B, p.n_pages, p.width, page)
+    ctx.pages_compact(bk, bv, bt, bl, br, bt, br, info, B, p.n_pages, p.width, page, 1, n_kv * d * item)
+    ctx.sync()
+    assert info.download()[:2].tolist() == [0, sum(-(-n // page) for b, n in enumerate(lens) if b != 1)]
+    after, table = bk.download().reshape(p.k.shape), bt.download().reshape(p.table.shape)
+    for b in (0, 2):
+        for j in range(-(-lens[b] // page)):
+            assert np.array_equal(after[table[b, j]].view(np.uint8), before[p.table[b, j]].view(np.uint8))
+    for b in made:
+        b.free()
+    p.free()
